@@ -1,0 +1,156 @@
+// Attention over the quantised paged cache: how a call is split, and the join of the splits (tgm_kv_attend).
+#include "tgm_kv_attend.h"
+
+namespace tgm {
+
+// One wave per row: weights of its splits (lane s: slot s), then their weighted sum, HD / 64 dims a lane.  Slots of the
+// common prefix (below `pslots`) are always written, those of a sequence's own positions as far as it reaches.
+template <int DT, int HD>
+__global__ void __launch_bounds__(256) attend_merge(const AttendArgs A, int pslots) {
+  constexpr int E = HD / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= at_rows(A)) return;
+  const int b = (int)(row / ((int64_t)A.T * A.H));
+  const int own = min(at_length(A, b), A.kcap) - A.k0;
+  const int n = pslots + (own > 0 ? (own + A.chunk - 1) / A.chunk : 0);
+  float m = -INFINITY, l = 0.f;
+  if (lane < n) {
+    const float* ml = at_ml(A, HD, row, lane);
+    m = ml[0];
+    l = ml[1];
+  }
+  float M = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  const float w = l > 0.f ? __builtin_amdgcn_exp2f(m - M) : 0.f;
+  float L = l * w;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+  float acc[E] = {};
+  const float* p = A.part + row * A.slots * HD + E * lane;
+  for (int s = 0; s < n; ++s) {
+    const float ws = __shfl(w, s, 64);  // 0: the slot's sums were not written
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += ws > 0.f ? ws * p[s * HD + e] : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) at_store<DT>(A.out, row * HD + E * lane + e, L > 0.f ? acc[e] / L : 0.f);
+}
+
+constexpr int kMaxSlots = 64;  // splits of a row: a lane each in attend_merge
+
+struct AttendPlan {
+  bool many;           // a sequence's own positions by attend_many
+  int chunk, splits;   // of a sequence's own positions
+  int pchunk, psplits; // of the common prefix
+  int64_t bytes;
+};
+
+static int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+// Splits of `span` positions over about `want` workgroups per row tile, in chunks that are a multiple of `unit`.
+static void split_span(int64_t span, int64_t want, int64_t unit, int64_t most, int& chunk, int& splits) {
+  int64_t n = want < 1 ? 1 : (want > most ? most : want);
+  const int64_t c = round_up((span + n - 1) / n, unit);
+  chunk = (int)(c < unit ? unit : c);
+  splits = (int)(span > 0 ? (span + chunk - 1) / chunk : 1);
+}
+
+static AttendPlan attend_plan(const tgm_kv_cache* c, int64_t dt, int64_t heads, int64_t batch, int64_t tokens, int64_t cols,
+                              int64_t shared) {
+  AttendPlan p{};
+  const int64_t G = heads / c->kv_heads, rows = tokens * G, cap = cols * c->page_size;
+  p.many = rows > attend_few_rows((int)dt);
+  const int64_t own = cap > shared ? cap - shared : 0;
+  // enough workgroups for two rounds of 256 CUs with two of them each; a split of decode is at least one block a wave
+  if (shared > 0) {
+    const int64_t tiles = (batch * rows + kManyRows - 1) / kManyRows * c->kv_heads;
+    split_span(shared, (512 + tiles - 1) / tiles, kManyKeys, kMaxSlots / 2, p.pchunk, p.psplits);
+  }
+  const int64_t most = kMaxSlots - p.psplits;
+  if (p.many) {
+    const int64_t tiles = (rows + kManyRows - 1) / kManyRows * c->kv_heads * batch;
+    split_span(own, 512 / tiles, kManyKeys, most, p.chunk, p.splits);
+  } else {
+    split_span(own, (1536 + c->kv_heads * batch - 1) / (c->kv_heads * batch), kFewWaves * kFewBlock, most, p.chunk, p.splits);
+  }
+  const int slots = p.splits + p.psplits;
+  p.bytes = slots == 1 ? 0 : batch * tokens * heads * slots * (c->head_dim + 2) * 4;
+  return p;
+}
+
+template <int DT>
+static void attend_go(const AttendPlan& p, AttendLaunch l, int shared, int cap, hipStream_t st) {
+  AttendArgs& a = l.a;
+  a.slots = p.splits + p.psplits;
+  if (p.psplits) {
+    AttendLaunch c = l;
+    c.a.k0 = 0, c.a.kcap = shared, c.a.chunk = p.pchunk, c.a.slot0 = 0, c.a.common = 1;
+    c.splits = p.psplits;
+    attend_many<DT>(c, st);
+  }
+  a.k0 = shared, a.kcap = cap, a.chunk = p.chunk, a.slot0 = p.psplits, a.common = 0;
+  l.splits = p.splits;
+  if (p.many) attend_many<DT>(l, st);
+  else attend_few<DT>(l, st);
+  if (a.slots > 1) {
+    const dim3 grid((unsigned)(((int64_t)a.B * a.T * a.H + 3) / 4));
+    if (l.hd == 64) hipLaunchKernelGGL((attend_merge<DT, 64>), grid, dim3(256), 0, st, a, p.psplits);
+    else hipLaunchKernelGGL((attend_merge<DT, 128>), grid, dim3(256), 0, st, a, p.psplits);
+  }
+}
+
+static bool attend_sizes_ok(const tgm_kv_cache* c, int64_t heads, int64_t batch, int64_t tokens, int64_t cols, int64_t shared) {
+  return c && c->kv_heads > 0 && c->page_size > 0 && heads > 0 && heads % c->kv_heads == 0 && heads <= 65535 && batch >= 0 &&
+         batch <= 65535 && tokens >= 0 && batch * tokens < (1ll << 24) && batch * tokens * heads < (1ll << 30) && cols >= 0 &&
+         cols * c->page_size < (1ll << 30) && shared >= 0 && shared <= cols * c->page_size && shared % c->page_size == 0;
+}
+
+}  // namespace tgm
+
+using namespace tgm;
+
+extern "C" int64_t tgm_kv_attend_workspace(const tgm_kv_cache* cache, int64_t q_dtype, int64_t heads, int64_t batch,
+                                           int64_t tokens, int64_t table_cols, int64_t shared) {
+  if (!attend_sizes_ok(cache, heads, batch, tokens, table_cols, shared) || batch == 0 || tokens == 0) return 0;
+  return attend_plan(cache, q_dtype, heads, batch, tokens, table_cols, shared).bytes;
+}
+
+extern "C" int tgm_kv_attend(const tgm_kv_cache* cache, const tgm_heads* q, const int32_t* table, int64_t ld_table,
+                             int64_t table_cols, const int32_t* lengths, int64_t batch, int64_t tokens, int64_t shared,
+                             double scale, void* workspace, int64_t workspace_bytes, void* out, void* stream) {
+  clear_error();
+  AttendLaunch l{};
+  AttendArgs& a = l.a;
+  if (const int e = kv_check(cache, table, ld_table, table_cols, a.ks, a.vs, a.pg)) return e;
+  TGM_CHECK_ARG(q, "null argument");
+  TGM_CHECK_ARG(q->dtype == TGM_F32 || q->dtype == TGM_F16 || q->dtype == TGM_BF16, "q must be f32, f16 or bf16");
+  TGM_CHECK_ARG(q->heads > 0 && q->heads % cache->kv_heads == 0, "heads must be a multiple of kv_heads");
+  TGM_CHECK_ARG(shared >= 0 && shared % cache->page_size == 0 && shared <= table_cols * cache->page_size,
+                "shared must be a multiple of page_size within the table");
+  TGM_CHECK_ARG(attend_sizes_ok(cache, q->heads, batch, tokens, table_cols, shared), "sizes out of range");
+  TGM_CHECK_ARG(scale > 0 && scale < 1e30, "scale must be positive");
+  if (batch == 0 || tokens == 0) return TGM_OK;
+  TGM_CHECK_ARG(q->data && lengths && out && ((uintptr_t)out & 15) == 0, "null or misaligned operand");
+  const AttendPlan p = attend_plan(cache, q->dtype, q->heads, batch, tokens, table_cols, shared);
+  TGM_CHECK_ARG(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 15) == 0),
+                "workspace too small or misaligned");
+  a.q = q->data, a.qb = q->stride_b, a.qt = q->stride_t, a.qh = q->stride_h;
+  const int64_t step = 16 / dtype_size((int)q->dtype);
+  a.qvec = ((uintptr_t)q->data & 15) == 0 && a.qb % step == 0 && a.qt % step == 0 && a.qh % step == 0;
+  a.lengths = lengths;
+  a.B = (int)batch, a.T = (int)tokens, a.H = (int)q->heads, a.HK = (int)cache->kv_heads, a.G = a.H / a.HK;
+  a.sl = (float)(scale * 1.4426950408889634);
+  a.part = (float*)workspace;
+  a.out = out;
+  l.kb = cache->k_format == TGM_KV_FP8_E4M3 ? 8 : 4;
+  l.vb = cache->v_format == TGM_KV_FP8_E4M3 ? 8 : 4;
+  l.hd = (int)cache->head_dim;
+  const int cap = (int)(table_cols * cache->page_size);
+  const hipStream_t st = (hipStream_t)stream;
+  if (q->dtype == TGM_F32) attend_go<TGM_F32>(p, l, (int)shared, cap, st);
+  else if (q->dtype == TGM_F16) attend_go<TGM_F16>(p, l, (int)shared, cap, st);
+  else attend_go<TGM_BF16>(p, l, (int)shared, cap, st);
+  return launch_status("tgm_kv_attend");
+}

@@ -1,5 +1,5 @@
 """ctypes binding of the gfx950 kernel library ``libtgm_mi355x.so`` (include/tgm_packed.h,
-include/tgm_decoder.h), with no torch dependency.
+include/tgm_decoder.h, include/tgm_serving.h), with no torch dependency.
 
 This is the only route from Python into the packed kernels: the plugin-buffer path
 (``codegen/program.py``) calls it with plugin buffer addresses and the device stream, the
@@ -88,9 +88,15 @@ SIGNATURES = {
     "tgm_dec_silu_mul": (_P, _I64, _I64, _P, _INT, _P),
     "tgm_dec_gemv_bf16": (_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P),
     "tgm_dec_argmax": (_P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P),
+    # serving operators (include/tgm_serving.h)
+    "tgm_rotate": (_P, _P, _P, _P, _I64, _I64, _I64, _P),
+    "tgm_kv_append": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P),
+    "tgm_kv_read": (_P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _INT, _P),
+    "tgm_kv_attend": (_P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, ctypes.c_double, _P, _I64, _P, _P),
+    "tgm_sample": (_P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P),
 }
 EXPORTS = ("tgm_abi_version", "tgm_last_error", "tgm_dec_attention_workspace", "tgm_gemm_w_split_workspace",
-           "tgm_gemm_w_split_noalloc_capacity", *SIGNATURES)
+           "tgm_gemm_w_split_noalloc_capacity", "tgm_kv_attend_workspace", "tgm_sample_workspace", *SIGNATURES)
 
 
 def library_path() -> Path:
@@ -126,6 +132,10 @@ def load_library() -> ctypes.CDLL:
         lib.tgm_gemm_w_split_workspace.restype = _I64
         lib.tgm_gemm_w_split_noalloc_capacity.argtypes = ()
         lib.tgm_gemm_w_split_noalloc_capacity.restype = _I64
+        lib.tgm_kv_attend_workspace.argtypes = (_P, _I64, _I64, _I64, _I64, _I64, _I64)
+        lib.tgm_kv_attend_workspace.restype = _I64
+        lib.tgm_sample_workspace.argtypes = (_I64, _I64, _I64)
+        lib.tgm_sample_workspace.restype = _I64
         _lib = lib
         return lib
 
