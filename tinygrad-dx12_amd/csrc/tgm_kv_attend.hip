@@ -3,12 +3,13 @@
 
 namespace tgm {
 
-// One wave per row: weights of its splits (lane s: slot s), then their weighted sum, HD / 64 dims a lane.  Slots of the
-// common prefix (below `pslots`) are always written, those of a sequence's own positions as far as it reaches.
+// One wave per row: weights of its splits (lane s: slot s), then their weighted sum, four dims a lane and the wave's
+// halves (quarters for 64 dims) on slots of their own, several loads in flight.  Slots of the common prefix (below
+// `pslots`) are always written, those of a sequence's own positions as far as it reaches.
 template <int DT, int HD>
 __global__ void __launch_bounds__(256) attend_merge(const AttendArgs A, int pslots) {
-  constexpr int E = HD / 64;
-  const int lane = threadIdx.x & 63;
+  constexpr int L = HD / 4, N = 64 / L, U = 4;  // lanes a slot, slots at a time, loads a lane in flight
+  const int lane = threadIdx.x & 63, sub = lane / L, d = 4 * (lane % L);
   const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= at_rows(A)) return;
   const int b = (int)(row / ((int64_t)A.T * A.H));
@@ -16,7 +17,7 @@ __global__ void __launch_bounds__(256) attend_merge(const AttendArgs A, int pslo
   const int n = pslots + (own > 0 ? (own + A.chunk - 1) / A.chunk : 0);
   float m = -INFINITY, l = 0.f;
   if (lane < n) {
-    const float* ml = at_ml(A, HD, row, lane);
+    const kv_f32x2 ml = *(const kv_f32x2*)at_ml(A, HD, row, lane);
     m = ml[0];
     l = ml[1];
   }
@@ -24,18 +25,33 @@ __global__ void __launch_bounds__(256) attend_merge(const AttendArgs A, int pslo
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
   const float w = l > 0.f ? __builtin_amdgcn_exp2f(m - M) : 0.f;
-  float L = l * w;
+  float sum = l * w;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
-  float acc[E] = {};
-  const float* p = A.part + row * A.slots * HD + E * lane;
-  for (int s = 0; s < n; ++s) {
-    const float ws = __shfl(w, s, 64);  // 0: the slot's sums were not written
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float* p = A.part + row * A.slots * HD + d;
+  for (int s0 = 0; s0 < n; s0 += N * U) {
+    f32x4 x[U];
+    float ws[U];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += ws > 0.f ? ws * p[s * HD + e] : 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * N + sub;  // 63 at most where s0 < n <= 64
+      ws[u] = __shfl(w, s, 64);        // 0 past the last one, and where a slot's sums were not written
+      x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (ws[u] > 0.f) x[u] = *(const f32x4*)(p + s * HD);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc += x[u] * ws[u];
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) at_store<DT>(A.out, row * HD + E * lane + e, L > 0.f ? acc[e] / L : 0.f);
+  for (int o = L; o < 64; o <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o, 64);
+  if (sub == 0) {
+    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) at_store<DT>(A.out, row * HD + d + e, acc[e] * inv);
+  }
 }
 
 constexpr int kMaxSlots = 64;  // splits of a row: a lane each in attend_merge
