@@ -44,16 +44,22 @@ struct AttendTerms {
 };
 
 // The bf16 terms of 8 fp32 values: t[0] = bf16(x), each next one the bf16 of what is left.
+// Two values a conversion: the compiler does not pair them by itself.
 template <int N>
 __device__ __forceinline__ void at_split(float (&r)[8], at_bf16x8 (&t)[N]) {
 #pragma unroll
-  for (int s = 0; s < N; ++s)
+  for (int s = 0; s < N; ++s) {
+    u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const __bf16 v = (__bf16)r[i];
-      t[s][i] = v;
-      r[i] -= (float)v;
+    for (int i = 0; i < 4; ++i) {
+      w[i] = bf16x2_bits(r[2 * i], r[2 * i + 1]);
+      if (s + 1 < N) {
+        r[2 * i] -= bits_f32(w[i] << 16);
+        r[2 * i + 1] -= bits_f32(w[i] & 0xFFFF0000u);
+      }
     }
+    t[s] = __builtin_bit_cast(at_bf16x8, w);
+  }
 }
 
 __device__ __forceinline__ at_bf16x8 at_tr_pair(const unsigned char* lo, const unsigned char* hi) {

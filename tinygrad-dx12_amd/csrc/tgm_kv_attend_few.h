@@ -191,19 +191,26 @@ __global__ void __launch_bounds__(256, 2) kv_attend_few(const AttendArgs A) {
       }
       m[ct] = mn;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int hf = 0; hf < 2; ++hf) {
+        u32x4 words;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
+        for (int e = 0; e < 4; ++e) {  // two values: tile i = 2 hf + e / 2, v = 2 (e % 2) and the next
+          const f32x4& s4 = S[ct][2 * hf + (e >> 1)];
           // v_exp_f32: within one unit in the last place; 0 for masked positions
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[ct][i][v], A.sl, -ref));
-          l[ct] += p;
+          float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s4[2 * (e & 1)], A.sl, -ref));
+          float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s4[2 * (e & 1) + 1], A.sl, -ref));
+          l[ct] += p0 + p1;
 #pragma unroll
           for (int t = 0; t + 1 < NP; ++t) {
-            const float rest = p - (float)(__bf16)p;
-            p = term > t ? rest : p;
+            const unsigned w = bf16x2_bits(p0, p1);
+            const float r0 = p0 - bits_f32(w << 16), r1 = p1 - bits_f32(w & 0xFFFF0000u);
+            p0 = term > t ? r0 : p0;
+            p1 = term > t ? r1 : p1;
           }
-          pb[ct][i >> 1][4 * (i & 1) + v] = (__bf16)p;
+          words[e] = bf16x2_bits(p0, p1);
         }
+        pb[ct][hf] = __builtin_bit_cast(at_bf16x8, words);
+      }
     }
     // values: rows with key % 4 in {2 hf, 2 hf + 1}, staged as row 2 (key / 4) + key % 2
 #pragma unroll

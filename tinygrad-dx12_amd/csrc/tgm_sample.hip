@@ -6,19 +6,18 @@
 // unit, and n weights of at most 2^F fit 63 bits.
 //
 // The kept set.  Sorted by value and, within a value, by index, what top-k, top-p and min-p keep is a prefix, so one cut
-// has to be found, and no row is sorted.  Three launches, a row in several workgroups for the first two:
+// has to be found, and no row is sorted.  Two launches:
 //
-//   sample_bins    counts and masses in bins of 1/40 of a power of two of the weight, from the largest down; weights
-//                  that round to 0 are left out (they are never drawn but for u = 0)
-//   sample_sift    finds the bin that the cut falls into.  Few tokens down to it (the rule with top-k): they are
-//                  listed.  Many: those of the cut's bin alone are listed, and the masses above it summed over segments
-//                  of the vocabulary.
-//   sample_draw    a workgroup a row: sorts the list in LDS, settles the cut exactly, and draws: over the sorted list,
-//                  or over the segments and then inside one of them.
+//   sample_bins   (a row in several workgroups) counts and masses in bins of 1/40 of a power of two of the weight, from
+//                 the largest down; weights that round to 0 are left out (they are never drawn but for u = 0)
+//   sample_draw   (a workgroup a row) finds the bin that the cut falls into.  Few tokens down to it (the rule with
+//                 top-k): it lists them in LDS, sorts them, settles the cut and draws among them.  Many: it lists those of
+//                 the cut's bin alone; the bins above it give the kept mass of each workgroup's part of the vocabulary,
+//                 which picks the part that the draw falls into, and only that part is weighed again.
 //
 // A list holds 2048 tokens.  A row that needs a longer one (thousands of equal logits at the cut, a top_k of thousands),
-// and one with u = 0, is settled inside sample_draw by descending a radix tree over order-preserving keys of the logits
-// (sample_descend), which needs no list.
+// and one with u = 0, is settled by descending a radix tree over order-preserving keys of the logits (sample_descend),
+// which needs no list.
 #include <math.h>
 
 #include "../../include/tgm_serving.h"
@@ -30,21 +29,15 @@ constexpr int kSampThreads = 1024, kSampWaves = 16, kSampBins = 2048;
 typedef unsigned long long samp_u64;
 typedef unsigned samp_u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kSampList = 2048, kSampSegs = 1024, kSampMostChunks = 16;
+constexpr int kSampList = 2048, kSampMostChunks = 16;
 constexpr double kSampPerBin = 40.0;  // bins per power of two of a weight: 2047 of them reach 2^-51
-
-struct SampPlan {  // of a row, from sample_sift
-  samp_u64 total, above;  // mass of all, and above the listed tokens
-  unsigned mode, bin;
-  int top_k, pad;  // 0: no cut
-};
-enum SampMode { kSampListAll = 0, kSampListBin = 1, kSampDescend = 2 };
 
 struct SampleArgs {
   const void* logits;
   int64_t ld;
   int n, fbits, vec;
-  int chunks, chunk, seg, segs;  // workgroups of a row, tokens of each (a multiple of seg), tokens and count of segments
+  int chunks, chunk;  // workgroups of a row in sample_bins, tokens of each
+  int rows;
   const float* u;
   const float* temperature;
   const int32_t* top_k;
@@ -53,11 +46,7 @@ struct SampleArgs {
   int32_t* tokens;
   // workspace, per row
   samp_u64* mass;   // [chunks][bins]
-  samp_u64* list;   // [kSampList], unordered
-  samp_u64* segsum; // [segs]
-  SampPlan* plan;
   unsigned* count;  // [chunks][bins]
-  unsigned* listed;
   float* max;
 };
 
@@ -151,6 +140,7 @@ __device__ __forceinline__ void samp_each(const void* row, int first, int last, 
   int done = first;
   if (vec) {
     const int v1 = last / V;
+#pragma unroll 4
     for (int i = first / V + threadIdx.x; i < v1; i += THREADS) {
       const samp_u32x4 w = ((const samp_u32x4*)row)[i];
 #pragma unroll
@@ -422,8 +412,8 @@ __device__ __forceinline__ void samp_load_table(double* table) {
   if (threadIdx.x < 64) table[threadIdx.x] = samp_table.v[threadIdx.x];
 }
 
-// Grid (chunks, rows).  Every workgroup of a row finds the row's maximum for itself: reading a row from the L2 is
-// cheaper than a launch.
+// Workgroups go to the 8 XCDs in turn: every workgroup of row r is number r mod 8 of its eight, so that a row stays in one
+// XCD's L2.  Each finds the row's maximum for itself, which costs less than a launch.
 constexpr int kBinThreads = 512;
 template <int DT>
 __global__ void __launch_bounds__(kBinThreads) sample_bins(const SampleArgs A) {
@@ -431,8 +421,9 @@ __global__ void __launch_bounds__(kBinThreads) sample_bins(const SampleArgs A) {
   __shared__ unsigned count[kSampBins];
   __shared__ double table[64];
   __shared__ float part[kBinThreads / 64];
-  const int64_t r = blockIdx.y;
-  const int c = blockIdx.x, tid = threadIdx.x;
+  const int local = blockIdx.x / 8, c = local % A.chunks, tid = threadIdx.x;
+  const int64_t r = (int64_t)(local / A.chunks) * 8 + blockIdx.x % 8;
+  if (r >= A.rows) return;
   const char* row = (const char*)A.logits + r * A.ld * (DT == TGM_F32 ? 4 : 2);
   samp_load_table(table);
   for (int i = tid; i < kSampBins; i += kBinThreads) {
@@ -440,10 +431,7 @@ __global__ void __launch_bounds__(kBinThreads) sample_bins(const SampleArgs A) {
     count[i] = 0;
   }
   const float best = samp_max<DT, kBinThreads>(row, A.n, A.vec, part);
-  if (c == 0 && tid == 0) {
-    A.max[r] = best;
-    A.listed[r] = 0;
-  }
+  if (c == 0 && tid == 0) A.max[r] = best;
   const float temp = A.temperature[r];
   if (!(temp > 0.f) || !(best > -INFINITY)) return;
   const SampExp ex{table, (double)best, 1.4426950408889634074 / (double)temp, A.fbits};
@@ -491,121 +479,6 @@ __device__ __forceinline__ T samp_scan(T v, T* part, T& total) {
 // A listed token: descending order of these is descending by value, ascending by index.
 __device__ __forceinline__ samp_u64 samp_entry(unsigned key, int i) { return ((samp_u64)key << 32) | (unsigned)~i; }
 
-// Grid (chunks, rows).
-template <int DT>
-__global__ void __launch_bounds__(kBinThreads) sample_sift(const SampleArgs A) {
-  constexpr int BPT = kSampBins / kBinThreads;
-  __shared__ double table[64];
-  __shared__ samp_u64 mpart[kBinThreads / 64];
-  __shared__ unsigned cpart[kBinThreads / 64];
-  __shared__ unsigned kbin, pbin, ksize, psize, pcount;
-  __shared__ samp_u64 pabove;
-  const int64_t r = blockIdx.y;
-  const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const char* row = (const char*)A.logits + r * A.ld * (DT == TGM_F32 ? 4 : 2);
-  const float temp = A.temperature[r], best = A.max[r];
-  if (!(temp > 0.f) || !(best > -INFINITY)) return;
-  samp_load_table(table);
-  if (tid == 0) kbin = pbin = kSampBins;
-  samp_u64 m[BPT], msum = 0;
-  unsigned n[BPT], nsum = 0;
-  const int64_t o = r * A.chunks * kSampBins + BPT * tid;
-#pragma unroll
-  for (int e = 0; e < BPT; ++e) m[e] = n[e] = 0;
-  for (int i = 0; i < A.chunks; ++i)
-#pragma unroll
-    for (int e = 0; e < BPT; ++e) {
-      m[e] += A.mass[o + (int64_t)i * kSampBins + e];
-      n[e] += A.count[o + (int64_t)i * kSampBins + e];
-    }
-#pragma unroll
-  for (int e = 0; e < BPT; ++e) {
-    msum += m[e];
-    nsum += n[e];
-  }
-  samp_u64 total;
-  unsigned all;
-  samp_u64 mb = samp_scan<kBinThreads>(msum, mpart, total);
-  unsigned nb = samp_scan<kBinThreads>(nsum, cpart, all);
-  int k = A.top_k ? A.top_k[r] : 0;
-  if (k < 0 || k >= A.n || (unsigned)k >= all) k = 0;  // whatever is not counted weighs nothing
-  const double p = A.top_p ? (double)A.top_p[r] : 1.0;
-  const double goal = p * (double)total;
-#pragma unroll
-  for (int e = 0; e < BPT; ++e) {
-    if (k > 0 && nb < (unsigned)k && nb + n[e] >= (unsigned)k) {
-      kbin = BPT * tid + e;
-      ksize = nb + n[e];
-    }
-    if (p < 1.0 && n[e] > 0 && (nb == 0 || (double)mb < goal) && ((double)(mb + m[e]) >= goal)) {
-      // the first such bin: with a goal of 0 and less the first one of all
-      pbin = BPT * tid + e;
-      psize = nb + n[e];
-      pcount = n[e];
-      pabove = mb;
-    }
-    mb += m[e];
-    nb += n[e];
-  }
-  __syncthreads();
-  SampPlan plan{total, 0, kSampListAll, kSampBins - 2, k, 0};
-  if (!(A.u[r] > 0.f)) {
-    plan.mode = kSampDescend;
-  } else if (k > 0) {
-    plan.bin = kbin;
-    if (ksize > kSampList) plan.mode = kSampDescend;
-  } else if (p < 1.0 && pbin < kSampBins) {
-    plan.bin = pbin;
-    if (psize > kSampList) {
-      plan.mode = pcount > kSampList ? kSampDescend : kSampListBin;
-      plan.above = pabove;
-    }
-  } else if (all > kSampList) {  // everything is kept
-    plan.mode = kSampListBin;
-    plan.bin = kSampBins - 1;
-    plan.above = total;
-  }
-  if (c == 0 && tid == 0) A.plan[r] = plan;
-  if (plan.mode == kSampDescend) return;
-  const SampExp ex{table, (double)best, 1.4426950408889634074 / (double)temp, A.fbits};
-  auto list = [&](bool hit, float x, int i) __attribute__((always_inline)) {
-    const samp_u64 hits = __ballot(hit);
-    if (hits == 0) return;
-    unsigned at = 0;
-    const int first = __ffsll((unsigned long long)hits) - 1;
-    if (lane == first) at = atomicAdd(&A.listed[r], (unsigned)__popcll(hits));
-    at = __shfl(at, first, 64) + (unsigned)__popcll(hits & ((1ull << lane) - 1ull));
-    if (hit && at < kSampList) A.list[r * kSampList + at] = samp_entry(samp_key<DT>(x), i);
-  };
-  const int begin = min(c * A.chunk, A.n), end = min((c + 1) * A.chunk, A.n);
-  if (plan.mode == kSampListAll) {
-    samp_each<DT, kBinThreads>(row, begin, end, A.vec,
-                               [&](float x, int i) { list(x > -INFINITY && ex.bin(ex.log2w(x)) <= (int)plan.bin, x, i); });
-    return;
-  }
-  const double min_p = A.min_p ? (double)A.min_p[r] : 0.0;
-  for (int s = begin / A.seg + wave; s * A.seg < end; s += kBinThreads / 64) {
-    samp_u64 sum = 0;
-    for (int i0 = s * A.seg; i0 < min((s + 1) * A.seg, end); i0 += 64) {
-      const int i = i0 + lane;
-      const float x = i < end ? samp_value<DT>(row, i) : -INFINITY;
-      bool in_bin = false;
-      if (x > -INFINITY) {
-        const double y = ex.log2w(x);
-        const int b = ex.bin(y);
-        in_bin = b == (int)plan.bin && b < kSampBins - 1;
-        if (b < (int)plan.bin) {
-          const double w = ex.weight_of(y);
-          sum += w >= min_p ? ex.fix(w) : 0;
-        }
-      }
-      list(in_bin, x, i);
-    }
-    sum = samp_wave_sum(sum);
-    if (lane == 0) A.segsum[r * A.segs + s] = sum;
-  }
-}
-
 // Bitonic sort of size (a power of two, at most 2048) entries in LDS by 1024 threads, descending.
 __device__ __forceinline__ void samp_sort(samp_u64* v, int size) {
   for (int k = 2; k <= size; k <<= 1)
@@ -625,7 +498,13 @@ __device__ __forceinline__ void samp_sort(samp_u64* v, int size) {
 }
 
 struct SampList {
-  samp_u64 entry[kSampList], weight[kSampList], seg[kSampSegs];
+  samp_u64 entry[kSampList], weight[kSampList];
+};
+// What sample_draw goes by: the cut's bin, and whether everything down to it is listed or that bin alone.
+enum SampMode { kSampListAll = 0, kSampListBin = 1, kSampDescend = 2 };
+struct SampCut {
+  unsigned bin, size, count;  // tokens down to the bin, and in it
+  samp_u64 above;             // mass above it
 };
 
 template <int DT>
@@ -635,11 +514,12 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
     SampList li;
   } u_;
   __shared__ double table[64];
-  __shared__ samp_u64 part[kSampWaves];
-  __shared__ unsigned kept_count;
-  __shared__ int seg_at;
-  __shared__ samp_u64 seg_left;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = A.n;
+  __shared__ samp_u64 part[kSampWaves], chunk_mass[kSampMostChunks];
+  __shared__ unsigned npart[kSampWaves];
+  __shared__ unsigned listed_, kept_count;
+  __shared__ SampCut kcut, pcut, mcut, last;
+  __shared__ int first_at;
+  const int tid = threadIdx.x, lane = tid & 63, n = A.n;
   const int64_t r = blockIdx.x;
   const char* row = (const char*)A.logits + r * A.ld * (DT == TGM_F32 ? 4 : 2);
   const float temp = A.temperature[r], best = A.max[r];
@@ -654,64 +534,130 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
     });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
-    if (tid == 0) seg_at = n;
+    if (tid == 0) first_at = n;
     __syncthreads();
-    if (lane == 0) atomicMin(&seg_at, at);
+    if (lane == 0) atomicMin(&first_at, at);
     __syncthreads();
-    if (tid == 0) A.tokens[r] = seg_at;
+    if (tid == 0) A.tokens[r] = first_at;
     return;
   }
   samp_load_table(table);
-  if (tid == 0) kept_count = 0;
+  if (tid == 0) {
+    listed_ = kept_count = 0;
+    kcut.bin = pcut.bin = mcut.bin = last.bin = kSampBins;
+  }
+  if (tid < kSampMostChunks) chunk_mass[tid] = 0;
   const SampExp ex{table, (double)best, 1.4426950408889634074 / (double)temp, A.fbits};
-  const SampPlan plan = A.plan[r];
+  const double p = A.top_p ? (double)A.top_p[r] : 1.0, min_p = A.min_p ? (double)A.min_p[r] : 0.0;
+
+  // two bins a thread, all parts of the row
+  samp_u64 m[2] = {0, 0};
+  unsigned c[2] = {0, 0};
+  const int64_t o = r * A.chunks * kSampBins + 2 * tid;
+#pragma unroll 4
+  for (int i = 0; i < A.chunks; ++i)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      m[q] += A.mass[o + (int64_t)i * kSampBins + q];
+      c[q] += A.count[o + (int64_t)i * kSampBins + q];
+    }
+  samp_u64 total;
+  unsigned all;
+  samp_u64 mb = samp_scan<kSampThreads>(m[0] + m[1], part, total);
+  unsigned nb = samp_scan<kSampThreads>(c[0] + c[1], npart, all);
+  int k = A.top_k ? A.top_k[r] : 0;
+  if (k < 0 || k >= n || (unsigned)k >= all) k = 0;  // what is not counted weighs nothing
+  const double goal_p = p * (double)total;
+  // the bin of min_p: tokens above it weigh more, tokens below it less
+  const int mbin = min_p > 0.0 ? (min_p >= 1.0 ? 0 : ex.bin(log2(min_p))) : kSampBins - 2;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int b = 2 * tid + q;
+    const SampCut here{(unsigned)b, nb + c[q], c[q], mb};
+    if (k > 0 && nb < (unsigned)k && nb + c[q] >= (unsigned)k) kcut = here;
+    // the first bin with which the mass reaches the goal, with a goal of 0 and less the first one of all
+    if (p < 1.0 && c[q] > 0 && (nb == 0 || (double)mb < goal_p) && (double)(mb + m[q]) >= goal_p) pcut = here;
+    if (b == mbin) mcut = here;
+    mb += m[q];
+    nb += c[q];
+  }
   __syncthreads();
-  if (plan.mode == kSampDescend) {
+  SampCut cut = mcut;  // everything that min_p leaves
+  if (k > 0) {
+    if (p < 1.0 || kcut.bin < cut.bin) cut = kcut;  // top-p goes by the mass that top-k left
+  } else if (p < 1.0 && pcut.bin < cut.bin) {
+    cut = pcut;
+  }
+  const int mode = !(A.u[r] > 0.f) ? kSampDescend
+                                   : (cut.size <= kSampList ? kSampListAll
+                                                            : (k == 0 && cut.count <= kSampList ? kSampListBin : kSampDescend));
+  if (mode == kSampDescend) {
     sample_descend<DT>(A, u_.sh, row, r, ex);
     return;
   }
+
+  // The list.  Which tokens may belong to it is asked in 32 bits, with bounds half a bin too wide.
   SampList& li = u_.li;
-  const int listed = min((int)A.listed[r], kSampList);
+  const double step = 1.0 / (kSampPerBin * ex.rate);
+  const float lowest = (float)((double)best - ((double)cut.bin + 1.5) * step);
+  const float highest = mode == kSampListAll ? INFINITY : (float)((double)best - ((double)cut.bin - 0.5) * step);
+  const bool wide = !(step > (double)fabsf(best) * 0x1p-20);  // bins near the resolution of 32 bits: no bounds
+  samp_each<DT, kSampThreads>(row, 0, n, A.vec, [&](float x, int i) {
+    if (!(x > -INFINITY) || (!wide && (x < lowest || x > highest))) return;
+    const int b = ex.bin(ex.log2w(x));
+    if (b > (int)cut.bin || b >= kSampBins - 1 || (mode == kSampListBin && b != (int)cut.bin)) return;
+    const unsigned at = atomicAdd(&listed_, 1u);
+    if (at < kSampList) li.entry[at] = samp_entry(samp_key<DT>(x), i);
+  });
+  if (mode == kSampListBin)  // kept mass of each part of the vocabulary, but for the cut's bin
+    for (int i = 0; i < A.chunks; ++i) {
+      samp_u64 s = 0;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if (2 * tid + q < (int)cut.bin) s += A.mass[o + (int64_t)i * kSampBins + q];
+      s = samp_wave_sum(s);
+      if (lane == 0 && s) atomicAdd(&chunk_mass[i], s);
+    }
+  __syncthreads();
+  const int listed = min((int)listed_, kSampList);
   int size = 64;
   while (size < listed) size <<= 1;
-  for (int i = tid; i < size; i += kSampThreads) li.entry[i] = i < listed ? A.list[r * kSampList + i] : 0;
+  for (int i = listed + tid; i < size; i += kSampThreads) li.entry[i] = 0;
   samp_sort(li.entry, size);
   // weights in rank order (two ranks a thread), and what the cuts keep of them
-  const double p = A.top_p ? (double)A.top_p[r] : 1.0, min_p = A.min_p ? (double)A.min_p[r] : 0.0;
   samp_u64 e[2], w[2];
   double wd[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int i = 2 * tid + q;
     e[q] = i < size ? li.entry[i] : 0;
-    const bool in = i < listed && (plan.top_k == 0 || i < plan.top_k);
+    const bool in = i < listed && (k == 0 || i < k);
     wd[q] = in ? ex.weight(samp_unkey<DT>((unsigned)(e[q] >> 32))) : -1.0;
     w[q] = in ? ex.fix(wd[q]) : 0;
   }
   samp_u64 sum;
-  samp_u64 before = plan.above + samp_scan<kSampThreads>(w[0] + w[1], part, sum);
-  const double goal = p * (double)(plan.top_k > 0 ? sum : plan.total);
+  samp_u64 before = samp_scan<kSampThreads>(w[0] + w[1], part, sum) + (mode == kSampListBin ? cut.above : 0);
+  const double goal = p * (double)(k > 0 ? sum : total);
   unsigned mine = 0;
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int i = 2 * tid + q;
     // in the mode of a listed bin at least one token lies above it
-    const bool keep = wd[q] >= 0.0 && wd[q] >= min_p &&
-                      (!(p < 1.0) || (double)before < goal || (i == 0 && plan.mode == kSampListAll));
+    const bool keep = wd[q] >= 0.0 && wd[q] >= min_p && (!(p < 1.0) || (double)before < goal || (i == 0 && mode == kSampListAll));
     before += w[q];
     if (!keep) w[q] = 0;
     mine += keep;
     if (i < size) li.weight[i] = w[q];
     // next: the kept ones by index, so that the draw runs in the vocabulary's order
-    if (i < size && plan.mode == kSampListAll) li.entry[i] = keep ? (((e[q] & 0xFFFFFFFFull) << 32) | (unsigned)(i + 1)) : 0;
+    if (i < size && mode == kSampListAll) li.entry[i] = keep ? (((e[q] & 0xFFFFFFFFull) << 32) | (unsigned)(i + 1)) : 0;
   }
   const double u = (double)A.u[r];
-  auto target_of = [&](samp_u64 total) __attribute__((always_inline)) -> samp_u64 {
-    const double t = u * (double)total;
-    const samp_u64 target = t < (double)total ? (samp_u64)t : total;
-    return target >= total ? total - 1 : target;  // u of 1 and more: the last
+  auto target_of = [&](samp_u64 sum_) __attribute__((always_inline)) -> samp_u64 {
+    const double t = u * (double)sum_;
+    const samp_u64 target = t < (double)sum_ ? (samp_u64)t : sum_;
+    return target >= sum_ ? sum_ - 1 : target;  // u of 1 and more: the last
   };
-  if (plan.mode == kSampListAll) {
+  if (mode == kSampListAll) {
     samp_sort(li.entry, size);  // by ~index, descending: ascending indices first, dropped ones last
     samp_u64 x[2];
 #pragma unroll
@@ -720,13 +666,13 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
       e[q] = i < size ? li.entry[i] : 0;
       x[q] = e[q] ? li.weight[(unsigned)e[q] - 1] : 0;
     }
-    samp_u64 total;
-    samp_u64 at = samp_scan<kSampThreads>(x[0] + x[1], part, total);
-    if (total == 0) {  // min_p above 1
+    samp_u64 kept;
+    samp_u64 at = samp_scan<kSampThreads>(x[0] + x[1], part, kept);
+    if (kept == 0) {  // min_p above 1
       if (tid == 0) A.tokens[r] = 0;
       return;
     }
-    const samp_u64 target = target_of(total);
+    const samp_u64 target = target_of(kept);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       if (x[q] > 0 && at <= target && at + x[q] > target) A.tokens[r] = (int32_t)~(unsigned)(e[q] >> 32);
@@ -734,72 +680,64 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
     }
     return;
   }
-  // the segments' masses with the kept ones of the cut's bin
+  // the part of the vocabulary that the draw falls into
   if (mine) atomicAdd(&kept_count, mine);
-  li.seg[tid] = tid < A.segs ? A.segsum[r * A.segs + tid] : 0;
-  __syncthreads();
 #pragma unroll
   for (int q = 0; q < 2; ++q)
-    if (w[q]) atomicAdd(&li.seg[~(unsigned)e[q] / (unsigned)A.seg], w[q]);
+    if (w[q]) atomicAdd(&chunk_mass[~(unsigned)e[q] / (unsigned)A.chunk], w[q]);
   __syncthreads();
-  const samp_u64 cut = kept_count ? li.entry[kept_count - 1] : ~0ull;  // the last one kept of the bin
-  const samp_u64 own = li.seg[tid];
-  samp_u64 total;
-  const samp_u64 at = samp_scan<kSampThreads>(own, part, total);
-  if (total == 0) {
+  const samp_u64 lowest_kept = kept_count ? li.entry[kept_count - 1] : ~0ull;  // of the cut's bin
+  samp_u64 kept = 0;
+  for (int i = 0; i < A.chunks; ++i) kept += chunk_mass[i];
+  if (kept == 0) {
     if (tid == 0) A.tokens[r] = 0;
     return;
   }
-  const samp_u64 target = target_of(total);
-  if (at <= target && at + own > target) {
-    seg_at = tid;
-    seg_left = target - at;
-  }
-  __syncthreads();
-  if (wave > 0) return;
-  samp_u64 base = 0;
-  const int first = seg_at * A.seg, end = min(first + A.seg, n);
-  for (int i0 = first; i0 < end; i0 += 64) {
-    const int i = i0 + lane;
-    const float x = i < end ? samp_value<DT>(row, i) : -INFINITY;
-    samp_u64 s = 0;
-    if (x > -INFINITY) {
-      const double y = ex.log2w(x);
-      const int b = ex.bin(y);
-      const double wx = ex.weight_of(y);
-      if (wx >= min_p && (b < (int)plan.bin || (b == (int)plan.bin && samp_entry(samp_key<DT>(x), i) >= cut))) s = ex.fix(wx);
-    }
-    const samp_u64 one = s;
+  samp_u64 left = target_of(kept);
+  int ch = 0;
+  while (ch < A.chunks - 1 && left >= chunk_mass[ch]) left -= chunk_mass[ch++];
+  const int end = min((ch + 1) * A.chunk, n);
+  for (int first = ch * A.chunk; first < end; first += 8 * kSampThreads) {  // 8 neighbours a thread
+    samp_u64 x[8], s = 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const samp_u64 up = samp_shfl_up(s, o);
-      if (lane >= o) s += up;
+    for (int q = 0; q < 8; ++q) {
+      const int i = first + 8 * tid + q;
+      const float v = i < end ? samp_value<DT>(row, i) : -INFINITY;
+      x[q] = 0;
+      if (v > -INFINITY) {
+        const double y = ex.log2w(v);
+        const int b = ex.bin(y);
+        if (b < (int)cut.bin || (b == (int)cut.bin && samp_entry(samp_key<DT>(v), i) >= lowest_kept)) x[q] = ex.fix(ex.weight_of(y));
+      }
+      s += x[q];
     }
-    const samp_u64 hit = __ballot(one > 0 && base + s > seg_left);
-    if (hit) {
-      if (lane == __ffsll((unsigned long long)hit) - 1) A.tokens[r] = (int32_t)i;
+    samp_u64 tile;
+    samp_u64 at = samp_scan<kSampThreads>(s, part, tile);
+    if (left < tile) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        if (x[q] > 0 && at <= left && at + x[q] > left) A.tokens[r] = (int32_t)(first + 8 * tid + q);
+        at += x[q];
+      }
       return;
     }
-    const unsigned lo32 = __shfl((unsigned)s, 63, 64), hi32 = __shfl((unsigned)(s >> 32), 63, 64);
-    base += ((samp_u64)hi32 << 32) | lo32;
+    left -= tile;
   }
 }
 
 struct SampSizes {
-  int chunks, chunk, seg, segs;
-  int64_t mass, list, segsum, plan, count, listed, max, bytes;
+  int chunks, chunk;
+  int64_t mass, count, max, bytes;
 };
 
 static SampSizes samp_sizes(int64_t rows, int64_t vocab) {
   SampSizes z;
-  z.seg = vocab <= 256 * kSampSegs ? 256 : 1024;
-  z.segs = (int)((vocab + z.seg - 1) / z.seg);
   // two workgroups a CU, 2048 tokens each at least
   int64_t c = (512 + rows - 1) / rows;
   const int64_t most = (vocab + 2047) / 2048;
   c = c > most ? most : c;
   c = c > kSampMostChunks ? kSampMostChunks : c;
-  z.chunk = (int)((vocab + c * z.seg - 1) / (c * z.seg)) * z.seg;
+  z.chunk = (int)((vocab + c * 1024 - 1) / (c * 1024)) * 1024;
   z.chunks = (int)((vocab + z.chunk - 1) / z.chunk);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -808,11 +746,7 @@ static SampSizes samp_sizes(int64_t rows, int64_t vocab) {
     return o;
   };
   z.mass = take(rows * z.chunks * kSampBins * 8);
-  z.list = take(rows * kSampList * 8);
-  z.segsum = take(rows * z.segs * 8);
-  z.plan = take(rows * (int64_t)sizeof(SampPlan));
   z.count = take(rows * z.chunks * kSampBins * 4);
-  z.listed = take(rows * 4);
   z.max = take(rows * 4);
   z.bytes = at;
   return z;
@@ -820,21 +754,9 @@ static SampSizes samp_sizes(int64_t rows, int64_t vocab) {
 
 template <int DT>
 static void sample_launch(const SampleArgs& a, int64_t rows, hipStream_t st) {
-  for (int64_t r0 = 0; r0 < rows; r0 += 65535) {  // a grid's second dimension
-    SampleArgs b = a;
-    const int64_t n = rows - r0 < 65535 ? rows - r0 : 65535;
-    b.logits = (const char*)a.logits + r0 * a.ld * (DT == TGM_F32 ? 4 : 2);
-    b.u += r0, b.temperature += r0, b.tokens += r0;
-    if (b.top_k) b.top_k += r0;
-    if (b.top_p) b.top_p += r0;
-    if (b.min_p) b.min_p += r0;
-    b.mass += r0 * a.chunks * kSampBins, b.count += r0 * a.chunks * kSampBins, b.list += r0 * kSampList;
-    b.segsum += r0 * a.segs, b.plan += r0, b.listed += r0, b.max += r0;
-    const dim3 grid((unsigned)a.chunks, (unsigned)n);
-    hipLaunchKernelGGL(sample_bins<DT>, grid, dim3(kBinThreads), 0, st, b);
-    hipLaunchKernelGGL(sample_sift<DT>, grid, dim3(kBinThreads), 0, st, b);
-    hipLaunchKernelGGL(sample_draw<DT>, dim3((unsigned)n), dim3(kSampThreads), 0, st, b);
-  }
+  const unsigned eights = (unsigned)((rows + 7) / 8);
+  hipLaunchKernelGGL(sample_bins<DT>, dim3(8 * eights * (unsigned)a.chunks), dim3(kBinThreads), 0, st, a);
+  hipLaunchKernelGGL(sample_draw<DT>, dim3((unsigned)rows), dim3(kSampThreads), 0, st, a);
 }
 
 }  // namespace tgm
@@ -860,16 +782,14 @@ extern "C" int tgm_sample(const void* logits, int64_t dtype, int64_t rows, int64
   TGM_CHECK_ARG(workspace && workspace_bytes >= z.bytes && ((uintptr_t)workspace & 15) == 0, "workspace too small or misaligned");
   SampleArgs a;
   a.logits = logits, a.ld = ld, a.n = (int)vocab;
-  a.chunks = z.chunks, a.chunk = z.chunk, a.seg = z.seg, a.segs = z.segs;
+  a.chunks = z.chunks, a.chunk = z.chunk, a.rows = (int)rows;
   int lg = 0;
   while ((1ll << lg) < vocab) ++lg;
   a.fbits = 62 - lg > 50 ? 50 : 62 - lg;
   a.vec = ((uintptr_t)logits & 15) == 0 && (rows == 1 || (ld * dtype_size((int)dtype)) % 16 == 0);
   a.u = u, a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p, a.tokens = tokens;
   char* ws = (char*)workspace;
-  a.mass = (samp_u64*)(ws + z.mass), a.list = (samp_u64*)(ws + z.list), a.segsum = (samp_u64*)(ws + z.segsum);
-  a.plan = (SampPlan*)(ws + z.plan), a.count = (unsigned*)(ws + z.count), a.listed = (unsigned*)(ws + z.listed);
-  a.max = (float*)(ws + z.max);
+  a.mass = (samp_u64*)(ws + z.mass), a.count = (unsigned*)(ws + z.count), a.max = (float*)(ws + z.max);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == TGM_F32) sample_launch<TGM_F32>(a, rows, st);
   else if (dtype == TGM_F16) sample_launch<TGM_F16>(a, rows, st);
