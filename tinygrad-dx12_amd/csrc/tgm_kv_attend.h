@@ -52,7 +52,9 @@ __device__ __forceinline__ void at_split(float (&r)[8], at_bf16x8 (&t)[N]) {
     u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = bf16x2_bits(r[2 * i], r[2 * i + 1]);
+      unsigned pair = bf16x2_bits(r[2 * i], r[2 * i + 1]);
+      asm("" : "+v"(pair));  // else the low half is converted a second time for the difference
+      w[i] = pair;
       if (s + 1 < N) {
         r[2 * i] -= bits_f32(w[i] << 16);
         r[2 * i + 1] -= bits_f32(w[i] & 0xFFFF0000u);
@@ -129,5 +131,5 @@ void attend_many(const AttendLaunch& l, hipStream_t st);
 constexpr int attend_few_rows(int dt) { return dt == TGM_F32 ? 10 : 16; }
 constexpr int kFewBlock = 64, kFewWaves = 4;
 constexpr int kManyKeys = 64, kManyRows = 128;
-
+constexpr float kLazyLog2 = 8.f;
 }  // namespace tgm

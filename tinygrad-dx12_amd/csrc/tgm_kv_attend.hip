@@ -79,7 +79,8 @@ static AttendPlan attend_plan(const tgm_kv_cache* c, int64_t dt, int64_t heads, 
   const int64_t G = heads / c->kv_heads, rows = tokens * G, cap = cols * c->page_size;
   p.many = rows > attend_few_rows((int)dt);
   const int64_t own = cap > shared ? cap - shared : 0;
-  // enough workgroups for two rounds of 256 CUs with two of them each; a split of decode is at least one block a wave
+  // attend_many: as many workgroups as run at once, two a CU; attend_few: two rounds of three a CU, a split at least one
+  // block a wave
   if (shared > 0) {
     const int64_t tiles = (batch * rows + kManyRows - 1) / kManyRows * c->kv_heads;
     split_span(shared, (512 + tiles - 1) / tiles, kManyKeys, kMaxSlots / 2, p.pchunk, p.psplits);

@@ -171,7 +171,8 @@ __global__ void __launch_bounds__(256, 2) kv_attend_few(const AttendArgs A) {
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const int p = base + 16 * g + 4 * v + i;
-            if (p > last[ct] || p >= k_hi || !gok) S[ct][i][v] = -INFINITY;
+            const bool gone = (p > last[ct]) | (p >= k_hi) | !gok;
+            S[ct][i][v] = gone ? -INFINITY : S[ct][i][v];
           }
       }
       float bm = -INFINITY;
@@ -181,15 +182,18 @@ __global__ void __launch_bounds__(256, 2) kv_attend_few(const AttendArgs A) {
         for (int v = 0; v < 4; ++v) bm = fmaxf(bm, S[ct][i][v]);
       bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
       bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
-      const float mn = fmaxf(m[ct], bm * A.sl);
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      if (__any(mn != m[ct])) {
-        const float alpha = __builtin_amdgcn_exp2f(m[ct] - ref);
+      bm *= A.sl;
+      // the reference of the exponentials moves only when a maximum has outgrown it by 2^8: weights of up to 2^8 lose
+      // nothing in fp32 and bf16, and the output is rarely rescaled
+      if (__any(bm > m[ct] + kLazyLog2)) {
+        const float mn = fmaxf(m[ct], bm);
+        const float alpha = m[ct] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[ct] - mn);
         l[ct] *= alpha;
 #pragma unroll
         for (int d = 0; d < ND; ++d) O[ct][d] *= alpha;
+        m[ct] = mn;
       }
-      m[ct] = mn;
+      const float ref = m[ct] == -INFINITY ? 0.f : m[ct];
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         u32x4 words;

@@ -42,12 +42,9 @@ __global__ void __launch_bounds__(256, 2) kv_attend_many(const AttendArgs A, int
   if (!A.common) kend = min(kend, at_length(A, b) - A.T + (min(tile * kManyRows + kManyRows, nrows) - 1) / A.G + 1);
   const int k_lo = A.k0 + z * A.chunk, k_hi = min(k_lo + A.chunk, kend);
   const int nblocks = k_hi > k_lo ? (k_hi - k_lo + kManyKeys - 1) / kManyKeys : 0;
-  int wave_min = last, wave_max = last;
+  int wave_min = last;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    wave_min = min(wave_min, __shfl_xor(wave_min, o, 64));
-    wave_max = max(wave_max, __shfl_xor(wave_max, o, 64));
-  }
+  for (int o = 16; o > 0; o >>= 1) wave_min = min(wave_min, __shfl_xor(wave_min, o, 64));
 
   auto swz_k = [](int key) { return CH == 16 ? key & 15 : (key >> 1) & 7; };
   auto swz_v = [](int key) { return CH == 16 ? (key & 3) * 5 : (((key >> 1) & 1) << 2) | (key & 3); };
@@ -116,8 +113,8 @@ __global__ void __launch_bounds__(256, 2) kv_attend_many(const AttendArgs A, int
   for (int kb = 0; kb < nblocks; ++kb) {
     __syncthreads();  // block kb is staged; everybody is done with block kb - 1
     const int first = k_lo + kb * kManyKeys;
-    if (kb + 1 < nblocks) load(kb + 1, raw);
-    if (first <= wave_max) {  // uniform over the wave
+    load(kb + 1, raw);  // past the last block: positions that are not seen, staged and not used
+    {
       const unsigned char* st = lds + (kb & 1) * STAGE;
       f32x16 S[2] = {f32x16{}, f32x16{}};
 #pragma unroll
@@ -137,7 +134,8 @@ __global__ void __launch_bounds__(256, 2) kv_attend_many(const AttendArgs A, int
           for (int v = 0; v < 16; ++v) {
             const int p = first + kt * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
             const int ok = kt == 0 ? (v < 8 ? ok0 : ok1) : (v < 8 ? ok2 : ok3);
-            if (p > last || p >= k_hi || !ok) S[kt][v] = -INFINITY;
+            const bool gone = (p > last) | (p >= k_hi) | !ok;
+            S[kt][v] = gone ? -INFINITY : S[kt][v];
           }
       }
       float bm = -INFINITY;
@@ -145,18 +143,23 @@ __global__ void __launch_bounds__(256, 2) kv_attend_many(const AttendArgs A, int
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int v = 0; v < 16; ++v) bm = fmaxf(bm, S[kt][v]);
-      bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
-      const float mn = fmaxf(m, bm * A.sl);
-      const float ref = mn == -INFINITY ? 0.f : mn;
-      if (__any(mn != m)) {
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+      float other = bm;
+      swap32(bm, other);  // bm: the lower half's in both halves, other: the upper half's
+      bm = fmaxf(bm, other);
+      bm *= A.sl;
+      // The reference of the exponentials moves only when a maximum has outgrown it by 2^8: weights of up to 2^8 lose
+      // nothing in fp32 and bf16, and the output is rarely rescaled.
+      if (__any(bm > m + kLazyLog2)) {
+        const float mn = fmaxf(m, bm);
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
         l *= alpha;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
           for (int v = 0; v < 16; ++v) O[d][v] *= alpha;
+        m = mn;
       }
-      m = mn;
+      const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -178,7 +181,7 @@ __global__ void __launch_bounds__(256, 2) kv_attend_many(const AttendArgs A, int
           }
         }
     }
-    if (kb + 1 < nblocks) stage(kb + 1, raw);
+    stage(kb + 1, raw);
   }
   l += __shfl_xor(l, 32, 64);
   if (!rvalid) return;
