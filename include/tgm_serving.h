@@ -57,9 +57,8 @@ typedef struct tgm_rotary {
   int64_t layout;     /* tgm_rotary_layout */
 } tgm_rotary;
 
-/* A tensor [batch, tokens, heads, head_dim]. */
+/* The layout of a tensor [batch, tokens, heads, head_dim]; its address goes beside it. */
 typedef struct tgm_heads {
-  void* data;
   int64_t stride_b, stride_t, stride_h;
   int64_t heads;
   int64_t dtype;
@@ -67,20 +66,21 @@ typedef struct tgm_heads {
 
 /* out = x rotated, token t of sequence b at position start[b] + t.  Angles, sines and products
  * are computed in 64 bits and rounded once to 32 and once to the output's type.  out may be x. */
-int tgm_rotate(const tgm_rotary* rotary, const tgm_heads* x, const tgm_heads* out, const int32_t* start, int64_t batch,
-               int64_t tokens, int64_t head_dim, void* stream);
+int tgm_rotate(const tgm_rotary* rotary, const tgm_heads* x, const void* x_data, const tgm_heads* out, void* out_data,
+               const int32_t* start, int64_t batch, int64_t tokens, int64_t head_dim, void* stream);
 
 /* The cache write of new tokens: k (rotated by `rotary` unless that is NULL) and v are quantised
  * to the cache's formats at positions start[b] + t, in blocks of 32 values: the scale is
  * 2^(floor(log2 max|x|) - e), e the exponent of the format's largest value (8 for fp8_e4m3, 2 for
  * fp4_e2m1), at least 2^-127 and 2^0 for a block of zeros; codes round to the nearest, ties to
  * even, and saturate.  NaN is stored as 0; infinities as the largest finite value.
- * q (may be NULL) is rotated into q_out.  k_seen and v_seen (both or neither NULL) receive what
- * the cache now holds for the new tokens.  All of q, k and v have k's type. */
-int tgm_kv_append(const tgm_kv_cache* cache, const tgm_rotary* rotary, const tgm_heads* q, const tgm_heads* q_out,
-                  const tgm_heads* k, const tgm_heads* v, const tgm_heads* k_seen, const tgm_heads* v_seen,
-                  const int32_t* table, int64_t ld_table, int64_t table_cols, const int32_t* start, int64_t batch,
-                  int64_t tokens, void* stream);
+ * q (may be NULL) is rotated into q_out.  seen (may be NULL) is the layout of k_seen and v_seen,
+ * which receive what the cache now holds for the new tokens.  All of q, k and v have k's type. */
+int tgm_kv_append(const tgm_kv_cache* cache, const tgm_rotary* rotary, const tgm_heads* q, const void* q_data,
+                  const tgm_heads* q_out, void* q_out_data, const tgm_heads* k, const void* k_data, const tgm_heads* v,
+                  const void* v_data, const tgm_heads* seen, void* k_seen, void* v_seen, const int32_t* table,
+                  int64_t ld_table, int64_t table_cols, const int32_t* start, int64_t batch, int64_t tokens,
+                  void* stream);
 
 /* Positions first[b] .. first[b] + count - 1 of every sequence, [batch, count, kv_heads, head_dim]
  * contiguous of type dtype (rounded once from the exact value), 16-byte aligned. */
@@ -96,9 +96,9 @@ int tgm_kv_read(const tgm_kv_cache* cache, const int32_t* table, int64_t ld_tabl
  * workspace: tgm_kv_attend_workspace() bytes, 16-byte aligned. */
 int64_t tgm_kv_attend_workspace(const tgm_kv_cache* cache, int64_t q_dtype, int64_t heads, int64_t batch, int64_t tokens,
                                 int64_t table_cols, int64_t shared);
-int tgm_kv_attend(const tgm_kv_cache* cache, const tgm_heads* q, const int32_t* table, int64_t ld_table,
-                  int64_t table_cols, const int32_t* lengths, int64_t batch, int64_t tokens, int64_t shared, double scale,
-                  void* workspace, int64_t workspace_bytes, void* out, void* stream);
+int tgm_kv_attend(const tgm_kv_cache* cache, const tgm_heads* q, const void* q_data, const int32_t* table,
+                  int64_t ld_table, int64_t table_cols, const int32_t* lengths, int64_t batch, int64_t tokens,
+                  int64_t shared, double scale, void* workspace, int64_t workspace_bytes, void* out, void* stream);
 
 /* One token per row of logits [rows, vocab] (row stride ld) by inversion: with
  * w_i = exp((logit_i - max) / temperature) in 64 bits, the kept set is cut to the top_k largest

@@ -132,8 +132,8 @@ def c_cache(**kw):
     return bytes(Cache(**f))
 
 
-def c_heads(h=2, dtype=13, data=4096):
-    return struct.pack("Pqqqqq", data, h * 64, h * 64, 64, h, dtype)
+def c_heads(h=2, dtype=13):
+    return struct.pack("qqqqq", h * 64, h * 64, 64, h, dtype)
 
 
 @pytest.mark.parametrize("kw", [dict(kd=None), dict(kd=8), dict(pages=0), dict(kv_heads=0), dict(head_dim=80),
@@ -142,30 +142,33 @@ def test_c_entries_refuse_a_bad_cache(kw):
     """Every refusal comes before a launch: the addresses are never read."""
     x = c_heads()
     with pytest.raises(ValueError):
-        K.call("tgm_kv_append", c_cache(**kw), None, None, None, x, x, None, None, 4096, 2, 2, 4096, 1, 1, None)
+        K.call("tgm_kv_append", c_cache(**kw), None, None, None, None, None, x, 4096, x, 4096, None, None, None, 4096, 2, 2,
+               4096, 1, 1, None)
     with pytest.raises(ValueError):
         K.call("tgm_kv_read", c_cache(**kw), 4096, 2, 2, 4096, 1, 1, 4096, 4096, 13, None)
     with pytest.raises(ValueError):
-        K.call("tgm_kv_attend", c_cache(**kw), x, 4096, 2, 2, 4096, 1, 1, 0, 1.0, 4096, 1 << 30, 4096, None)
+        K.call("tgm_kv_attend", c_cache(**kw), x, 4096, 4096, 2, 2, 4096, 1, 1, 0, 1.0, 4096, 1 << 30, 4096, None)
 
 
 def test_c_entries_refuse_bad_calls():
     c, x = c_cache(), c_heads()
-    attend = dict(q=x, table=4096, ld=2, cols=2, lengths=4096, batch=1, tokens=1, shared=0, scale=1.0, ws=4096, wsb=1 << 30,
+    attend = dict(q=x, data=4096, table=4096, ld=2, cols=2, lengths=4096, batch=1, tokens=1, shared=0, scale=1.0, ws=4096, wsb=1 << 30,
                   out=4096)
-    for bad in (dict(q=None), dict(q=c_heads(3)), dict(q=c_heads(dtype=14)), dict(table=None), dict(ld=1), dict(cols=1 << 40),
+    for bad in (dict(q=None), dict(data=None), dict(q=c_heads(3)), dict(q=c_heads(dtype=14)), dict(table=None), dict(ld=1), dict(cols=1 << 40),
                 dict(lengths=None), dict(batch=-1), dict(tokens=-1), dict(shared=32), dict(shared=192), dict(scale=0.0),
                 dict(scale=math.nan), dict(out=None), dict(out=8), dict(cols=8, ld=8, wsb=16), dict(cols=8, ld=8, ws=None)):
         with pytest.raises(ValueError):
             K.call("tgm_kv_attend", c, *{**attend, **bad}.values(), None)
     rot = struct.pack("Pdqq", 4096, 1.0, 64, 0)
-    for args in [(None, x, x, 4096, 1, 1, 64), (struct.pack("Pdqq", 4096, 1.0, 66, 0), x, x, 4096, 1, 1, 64),
-                 (struct.pack("Pdqq", 4096, 1.0, 63, 0), x, x, 4096, 1, 1, 64),
-                 (struct.pack("Pdqq", 0, 1.0, 64, 0), x, x, 4096, 1, 1, 64),
-                 (struct.pack("Pdqq", 4096, 1.0, 64, 2), x, x, 4096, 1, 1, 64), (rot, x, c_heads(3), 4096, 1, 1, 64),
-                 (rot, x, c_heads(dtype=12), 4096, 1, 1, 64), (rot, x, x, None, 1, 1, 64), (rot, x, x, 4096, -1, 1, 64)]:
+    for r, a, b, start, batch in [(None, x, x, 4096, 1), (struct.pack("Pdqq", 4096, 1.0, 66, 0), x, x, 4096, 1),
+                                  (struct.pack("Pdqq", 4096, 1.0, 63, 0), x, x, 4096, 1),
+                                  (struct.pack("Pdqq", 0, 1.0, 64, 0), x, x, 4096, 1),
+                                  (struct.pack("Pdqq", 4096, 1.0, 64, 2), x, x, 4096, 1), (rot, x, c_heads(3), 4096, 1),
+                                  (rot, x, c_heads(dtype=12), 4096, 1), (rot, x, x, None, 1), (rot, x, x, 4096, -1)]:
         with pytest.raises(ValueError):
-            K.call("tgm_rotate", *args, None)
+            K.call("tgm_rotate", r, a, 4096, b, 4096, start, batch, 1, 64, None)
+    with pytest.raises(ValueError):
+        K.call("tgm_rotate", rot, x, None, x, 4096, 4096, 1, 1, 64, None)
     for args in [(4096, 14, 1, 8, 8), (4096, 13, -1, 8, 8), (4096, 13, 1, 0, 8), (4096, 13, 1, (1 << 20) + 1, 1 << 21),
                  (4096, 13, 2, 8, 7), (None, 13, 1, 8, 8)]:
         with pytest.raises(ValueError):
@@ -173,7 +176,7 @@ def test_c_entries_refuse_bad_calls():
 
 
 def test_nothing_to_do_is_no_error():
-    K.call("tgm_kv_attend", c_cache(), c_heads(), 4096, 2, 2, None, 0, 1, 0, 1.0, None, 0, None, None)
+    K.call("tgm_kv_attend", c_cache(), c_heads(), None, 4096, 2, 2, None, 0, 1, 0, 1.0, None, 0, None, None)
     K.call("tgm_kv_read", c_cache(), 4096, 2, 2, None, 1, 0, None, None, 13, None)
     K.call("tgm_sample", None, 13, 0, 8, 8, None, None, None, None, None, None, None, 0, None)
 

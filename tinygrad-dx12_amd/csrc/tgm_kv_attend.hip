@@ -134,9 +134,10 @@ extern "C" int64_t tgm_kv_attend_workspace(const tgm_kv_cache* cache, int64_t q_
   return attend_plan(cache, q_dtype, heads, batch, tokens, table_cols, shared).bytes;
 }
 
-extern "C" int tgm_kv_attend(const tgm_kv_cache* cache, const tgm_heads* q, const int32_t* table, int64_t ld_table,
-                             int64_t table_cols, const int32_t* lengths, int64_t batch, int64_t tokens, int64_t shared,
-                             double scale, void* workspace, int64_t workspace_bytes, void* out, void* stream) {
+extern "C" int tgm_kv_attend(const tgm_kv_cache* cache, const tgm_heads* q, const void* q_data, const int32_t* table,
+                             int64_t ld_table, int64_t table_cols, const int32_t* lengths, int64_t batch, int64_t tokens,
+                             int64_t shared, double scale, void* workspace, int64_t workspace_bytes, void* out,
+                             void* stream) {
   clear_error();
   AttendLaunch l{};
   AttendArgs& a = l.a;
@@ -149,13 +150,13 @@ extern "C" int tgm_kv_attend(const tgm_kv_cache* cache, const tgm_heads* q, cons
   TGM_CHECK_ARG(attend_sizes_ok(cache, q->heads, batch, tokens, table_cols, shared), "sizes out of range");
   TGM_CHECK_ARG(scale > 0 && scale < 1e30, "scale must be positive");
   if (batch == 0 || tokens == 0) return TGM_OK;
-  TGM_CHECK_ARG(q->data && lengths && out && ((uintptr_t)out & 15) == 0, "null or misaligned operand");
+  TGM_CHECK_ARG(q_data && lengths && out && ((uintptr_t)out & 15) == 0, "null or misaligned operand");
   const AttendPlan p = attend_plan(cache, q->dtype, q->heads, batch, tokens, table_cols, shared);
   TGM_CHECK_ARG(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 15) == 0),
                 "workspace too small or misaligned");
-  a.q = q->data, a.qb = q->stride_b, a.qt = q->stride_t, a.qh = q->stride_h;
+  a.q = q_data, a.qb = q->stride_b, a.qt = q->stride_t, a.qh = q->stride_h;
   const int64_t step = 16 / dtype_size((int)q->dtype);
-  a.qvec = ((uintptr_t)q->data & 15) == 0 && a.qb % step == 0 && a.qt % step == 0 && a.qh % step == 0;
+  a.qvec = ((uintptr_t)q_data & 15) == 0 && a.qb % step == 0 && a.qt % step == 0 && a.qh % step == 0;
   a.lengths = lengths;
   a.B = (int)batch, a.T = (int)tokens, a.H = (int)q->heads, a.HK = (int)cache->kv_heads, a.G = a.H / a.HK;
   a.sl = (float)(scale * 1.4426950408889634);

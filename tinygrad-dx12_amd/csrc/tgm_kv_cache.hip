@@ -180,23 +180,24 @@ static void launch_append(int mode, dim3 grid, hipStream_t st, const AppendArgs&
   else hipLaunchKernelGGL((kv_append<DT, HD, kRotPart>), grid, dim3(256), 0, st, a);
 }
 
-static AppendView append_view(const tgm_heads* t) {
+static AppendView append_view(const tgm_heads* t, const void* data) {
   if (!t) return AppendView{nullptr, 0, 0, 0, 0};
-  return AppendView{t->data, t->stride_b, t->stride_t, t->stride_h, heads_vec(t)};
+  return AppendView{(void*)data, t->stride_b, t->stride_t, t->stride_h, heads_vec(t, data)};
 }
 
 }  // namespace tgm
 
 using namespace tgm;
 
-extern "C" int tgm_kv_append(const tgm_kv_cache* cache, const tgm_rotary* rotary, const tgm_heads* q, const tgm_heads* q_out,
-                             const tgm_heads* k, const tgm_heads* v, const tgm_heads* k_seen, const tgm_heads* v_seen,
-                             const int32_t* table, int64_t ld_table, int64_t table_cols, const int32_t* start, int64_t batch,
-                             int64_t tokens, void* stream) {
+extern "C" int tgm_kv_append(const tgm_kv_cache* cache, const tgm_rotary* rotary, const tgm_heads* q, const void* q_data,
+                             const tgm_heads* q_out, void* q_out_data, const tgm_heads* k, const void* k_data,
+                             const tgm_heads* v, const void* v_data, const tgm_heads* seen, void* k_seen, void* v_seen,
+                             const int32_t* table, int64_t ld_table, int64_t table_cols, const int32_t* start,
+                             int64_t batch, int64_t tokens, void* stream) {
   clear_error();
   AppendArgs a;
   if (const int e = kv_check(cache, table, ld_table, table_cols, a.ks, a.vs, a.pg)) return e;
-  TGM_CHECK_ARG(k && v && (q != nullptr) == (q_out != nullptr) && (k_seen != nullptr) == (v_seen != nullptr), "null argument");
+  TGM_CHECK_ARG(k && v && (q != nullptr) == (q_out != nullptr), "null argument");
   if (rotary)
     if (const int e = rot_check(rotary, cache->head_dim)) return e;
   TGM_CHECK_ARG(batch >= 0 && tokens >= 0 && batch * tokens < (1ll << 30), "sizes out of range");
@@ -204,15 +205,14 @@ extern "C" int tgm_kv_append(const tgm_kv_cache* cache, const tgm_rotary* rotary
                 "q, k and v must be f32, f16 or bf16 and alike");
   TGM_CHECK_ARG(k->heads == cache->kv_heads && v->heads == cache->kv_heads, "k and v must have the cache's heads");
   TGM_CHECK_ARG(!q || (q->heads > 0 && q->heads <= 65535 && q_out->heads == q->heads), "invalid query heads");
-  TGM_CHECK_ARG(!k_seen || (heads_dtype_ok(k_seen->dtype) && v_seen->dtype == k_seen->dtype &&
-                            k_seen->heads == cache->kv_heads && v_seen->heads == cache->kv_heads),
+  TGM_CHECK_ARG(!seen || (heads_dtype_ok(seen->dtype) && seen->heads == cache->kv_heads),
                 "k_seen and v_seen must be f32, f16 or bf16 and have the cache's heads");
   if (batch == 0 || tokens == 0) return TGM_OK;
-  TGM_CHECK_ARG(k->data && v->data && start && (!q || (q->data && q_out->data)) && (!k_seen || (k_seen->data && v_seen->data)),
-                "null operand");
-  a.q = append_view(q), a.qo = append_view(q_out), a.k = append_view(k), a.v = append_view(v);
-  a.ko = append_view(k_seen), a.vo = append_view(v_seen);
-  a.H = q ? (int)q->heads : 0, a.HK = (int)cache->kv_heads, a.seen = k_seen ? (int)k_seen->dtype : -1;
+  TGM_CHECK_ARG(k_data && v_data && start && (!q || (q_data && q_out_data)) && (!seen || (k_seen && v_seen)), "null operand");
+  a.q = append_view(q, q_data), a.qo = append_view(q_out, q_out_data);
+  a.k = append_view(k, k_data), a.v = append_view(v, v_data);
+  a.ko = append_view(seen, k_seen), a.vo = append_view(seen, v_seen);
+  a.H = q ? (int)q->heads : 0, a.HK = (int)cache->kv_heads, a.seen = seen ? (int)seen->dtype : -1;
   a.kf = (int)cache->k_format, a.vf = (int)cache->v_format;
   a.rot = rotary ? RotArgs{rotary->freq, rotary->gain, (int)(rotary->rotary_dim / 2)} : RotArgs{nullptr, 1.0, 0};
   a.start = start, a.T = (int)tokens;

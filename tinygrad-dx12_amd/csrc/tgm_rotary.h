@@ -138,9 +138,9 @@ inline int rot_check(const tgm_rotary* r, int64_t head_dim) {
 
 inline bool heads_dtype_ok(int64_t dt) { return dt == TGM_F32 || dt == TGM_F16 || dt == TGM_BF16; }
 // 16-byte loads of 8 values (4 at a time in 32 bits) start at every head of every token.
-inline bool heads_vec(const tgm_heads* t) {
+inline bool heads_vec(const tgm_heads* t, const void* data) {
   const int64_t step = 16 / dtype_size((int)t->dtype);
-  return ((uintptr_t)t->data & 15) == 0 && t->stride_b % step == 0 && t->stride_t % step == 0 && t->stride_h % step == 0;
+  return ((uintptr_t)data & 15) == 0 && t->stride_b % step == 0 && t->stride_t % step == 0 && t->stride_h % step == 0;
 }
 
 }  // namespace tgm

@@ -89,8 +89,9 @@ static void launch_rotate(int mode, dim3 grid, hipStream_t st, const RotArgs& ro
 
 using namespace tgm;
 
-extern "C" int tgm_rotate(const tgm_rotary* rotary, const tgm_heads* x, const tgm_heads* out, const int32_t* start,
-                          int64_t batch, int64_t tokens, int64_t head_dim, void* stream) {
+extern "C" int tgm_rotate(const tgm_rotary* rotary, const tgm_heads* x, const void* x_data, const tgm_heads* out,
+                          void* out_data, const int32_t* start, int64_t batch, int64_t tokens, int64_t head_dim,
+                          void* stream) {
   clear_error();
   TGM_CHECK_ARG(rotary && x && out, "null argument");
   TGM_CHECK_ARG(batch >= 0 && tokens >= 0 && x->heads >= 0 && head_dim > 0, "negative size");
@@ -98,12 +99,12 @@ extern "C" int tgm_rotate(const tgm_rotary* rotary, const tgm_heads* x, const tg
   TGM_CHECK_ARG(heads_dtype_ok(x->dtype) && out->dtype == x->dtype && out->heads == x->heads,
                 "x and out must be f32, f16 or bf16 and alike");
   if (batch == 0 || tokens == 0 || x->heads == 0) return TGM_OK;
-  TGM_CHECK_ARG(x->data && out->data && start, "null operand");
+  TGM_CHECK_ARG(x_data && out_data && start, "null operand");
   TGM_CHECK_ARG(batch < (1 << 30) && tokens < (1 << 30) && x->heads < (1 << 24) && head_dim < (1 << 20) &&
                     batch * tokens < (1ll << 30), "sizes out of range");
   const RotArgs rot{rotary->freq, rotary->gain, (int)(rotary->rotary_dim / 2)};
-  const RotView vx{x->data, x->stride_b, x->stride_t, x->stride_h, heads_vec(x)};
-  const RotView vy{out->data, out->stride_b, out->stride_t, out->stride_h, heads_vec(out)};
+  const RotView vx{(void*)x_data, x->stride_b, x->stride_t, x->stride_h, heads_vec(x, x_data)};
+  const RotView vy{out_data, out->stride_b, out->stride_t, out->stride_h, heads_vec(out, out_data)};
   const hipStream_t st = (hipStream_t)stream;
   const int64_t ntok = batch * tokens;
   const int H = (int)x->heads, T = (int)tokens;

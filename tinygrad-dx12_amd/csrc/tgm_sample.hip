@@ -27,7 +27,9 @@ namespace tgm {
 
 constexpr int kSampThreads = 1024, kSampWaves = 16, kSampBins = 2048;
 typedef unsigned long long samp_u64;
+typedef unsigned samp_u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned samp_u32x4 __attribute__((ext_vector_type(4)));
+typedef samp_u64 samp_u64x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kSampList = 2048, kSampMostChunks = 16;
 constexpr double kSampPerBin = 40.0;  // bins per power of two of a weight: 2047 of them reach 2^-51
@@ -106,15 +108,21 @@ struct SampExp {
   const double* table;
   double max, rate;  // rate = log2(e) / temperature
   int fbits;
-  __device__ __forceinline__ double log2w(float x) const { return x == max ? 0.0 : ((double)x - max) * rate; }
+  bool infinite;     // the maximum is +inf: it weighs 1, all else 0
+  __device__ __forceinline__ SampExp(const double* t, float best, float temperature, int f)
+      : table(t), max(best), rate(1.4426950408889634074 / (double)temperature), fbits(f), infinite(best == INFINITY) {}
+  __device__ __forceinline__ double log2w(float x) const {
+    const double y = ((double)x - max) * rate;
+    return infinite ? (x == INFINITY ? 0.0 : -INFINITY) : y;
+  }
   // bins of 1 / 40 of a power of two, descending with x; kSampBins - 1 for weights that round to 0
   __device__ __forceinline__ int bin(double y) const {
     const double b = y * -kSampPerBin;
     return b < (double)(kSampBins - 1) ? (int)b : kSampBins - 1;
   }
-  __device__ __forceinline__ double weight(float x) const { return weight_of(log2w(x)); }
-  __device__ __forceinline__ double weight_of(double lw) const {
-    const double y = fmax(lw, -1100.0) * 64.0;
+  // 2^(lw + more), lw above -1100
+  __device__ __forceinline__ double power(double lw, int more) const {
+    const double y = lw * 64.0;
     const double k = __builtin_rint(y);
     const int ki = (int)k;
     const double r = (y - k) * (0.69314718055994530942 / 64.0);
@@ -124,12 +132,14 @@ struct SampExp {
     p = __builtin_fma(p, r, 0.5);
     p = __builtin_fma(p, r, 1.0);
     p = __builtin_fma(p, r, 1.0);
-    return __builtin_ldexp(p * table[ki & 63], ki >> 6);
+    return __builtin_ldexp(p * table[ki & 63], (ki >> 6) + more);
   }
+  __device__ __forceinline__ double weight(float x) const { return power(fmax(log2w(x), -1100.0), 0); }
   // w 2^F is at most 2^50: adding 2^52 rounds it to a whole number, which the sum's low 52 bits hold
-  __device__ __forceinline__ samp_u64 fix(double w) const {
-    const double s = __builtin_ldexp(w, fbits) + 0x1p52;
-    return __builtin_bit_cast(samp_u64, s) & 0xFFFFFFFFFFFFFull;
+  __device__ __forceinline__ samp_u64 fix(double w) const { return whole(__builtin_ldexp(w, fbits)); }
+  __device__ __forceinline__ samp_u64 fix_of(double lw) const { return whole(power(lw, fbits)); }  // the same
+  __device__ __forceinline__ samp_u64 whole(double w) const {
+    return __builtin_bit_cast(samp_u64, w + 0x1p52) & 0xFFFFFFFFFFFFFull;
   }
 };
 
@@ -434,14 +444,14 @@ __global__ void __launch_bounds__(kBinThreads) sample_bins(const SampleArgs A) {
   if (c == 0 && tid == 0) A.max[r] = best;
   const float temp = A.temperature[r];
   if (!(temp > 0.f) || !(best > -INFINITY)) return;
-  const SampExp ex{table, (double)best, 1.4426950408889634074 / (double)temp, A.fbits};
+  const SampExp ex(table, best, temp, A.fbits);
   samp_each<DT, kBinThreads>(row, min(c * A.chunk, A.n), min((c + 1) * A.chunk, A.n), A.vec, [&](float x, int) {
     if (!(x > -INFINITY)) return;
     const double y = ex.log2w(x);
     const int b = ex.bin(y);
     if (b == kSampBins - 1) return;
     atomicAdd(&count[b], 1u);
-    atomicAdd(&mass[b], ex.fix(ex.weight_of(y)));
+    atomicAdd(&mass[b], ex.fix_of(y));
   });
   __syncthreads();
   const int64_t o = (r * A.chunks + c) * kSampBins;
@@ -479,12 +489,27 @@ __device__ __forceinline__ T samp_scan(T v, T* part, T& total) {
 // A listed token: descending order of these is descending by value, ascending by index.
 __device__ __forceinline__ samp_u64 samp_entry(unsigned key, int i) { return ((samp_u64)key << 32) | (unsigned)~i; }
 
-// Bitonic sort of size (a power of two, at most 2048) entries in LDS by 1024 threads, descending.
-__device__ __forceinline__ void samp_sort(samp_u64* v, int size) {
+// Sorts size (a power of two from 64 to 2048) entries in LDS by 1024 threads, descending; entries differ but for zeros.
+// Up to 512 by counting the larger ones, several threads an entry (two barriers; 64 entries: about 0.3 us where the
+// network's 21 barriers take 2), beyond by a bitonic network.  `rank` holds `size` counters.
+__device__ __forceinline__ void samp_sort(samp_u64* v, unsigned* rank, int size) {
+  const int t = threadIdx.x;
+  if (size <= 512) {
+    const int i = t & (size - 1), share = size * size / kSampThreads, j0 = (t / size) * share;
+    if (t < size) rank[t] = 0;
+    __syncthreads();
+    const samp_u64 mine = v[i];
+    unsigned n = 0;
+    for (int j = j0; j < j0 + share; ++j) n += v[j] > mine || (v[j] == mine && j < i);
+    if (n) atomicAdd(&rank[i], n);
+    __syncthreads();
+    if (t < size) v[rank[t]] = mine;
+    __syncthreads();
+    return;
+  }
   for (int k = 2; k <= size; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
       __syncthreads();
-      const int t = threadIdx.x;
       if (t < size / 2) {
         const int a = 2 * t - (t & (j - 1)), b = a + j;
         const samp_u64 x = v[a], y = v[b];
@@ -499,6 +524,7 @@ __device__ __forceinline__ void samp_sort(samp_u64* v, int size) {
 
 struct SampList {
   samp_u64 entry[kSampList], weight[kSampList];
+  unsigned rank[512];
 };
 // What sample_draw goes by: the cut's bin, and whether everything down to it is listed or that bin alone.
 enum SampMode { kSampListAll = 0, kSampListBin = 1, kSampDescend = 2 };
@@ -547,20 +573,34 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
     kcut.bin = pcut.bin = mcut.bin = last.bin = kSampBins;
   }
   if (tid < kSampMostChunks) chunk_mass[tid] = 0;
-  const SampExp ex{table, (double)best, 1.4426950408889634074 / (double)temp, A.fbits};
+  const SampExp ex(table, best, temp, A.fbits);
   const double p = A.top_p ? (double)A.top_p[r] : 1.0, min_p = A.min_p ? (double)A.min_p[r] : 0.0;
 
   // two bins a thread, all parts of the row
   samp_u64 m[2] = {0, 0};
   unsigned c[2] = {0, 0};
   const int64_t o = r * A.chunks * kSampBins + 2 * tid;
-#pragma unroll 4
-  for (int i = 0; i < A.chunks; ++i)
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      m[q] += A.mass[o + (int64_t)i * kSampBins + q];
-      c[q] += A.count[o + (int64_t)i * kSampBins + q];
+  for (int i0 = 0; i0 < kSampMostChunks; i0 += 8) {  // eight parts' loads in flight
+    samp_u64x2 mi[8];
+    samp_u32x2 ci[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      mi[i] = samp_u64x2{0, 0};
+      ci[i] = samp_u32x2{0, 0};
+      if (i0 + i < A.chunks) {
+        mi[i] = *(const samp_u64x2*)(A.mass + o + (int64_t)(i0 + i) * kSampBins);
+        ci[i] = *(const samp_u32x2*)(A.count + o + (int64_t)(i0 + i) * kSampBins);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        m[q] += mi[i][q];
+        c[q] += ci[i][q];
+      }
+  }
   samp_u64 total;
   unsigned all;
   samp_u64 mb = samp_scan<kSampThreads>(m[0] + m[1], part, total);
@@ -609,21 +649,19 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
     const unsigned at = atomicAdd(&listed_, 1u);
     if (at < kSampList) li.entry[at] = samp_entry(samp_key<DT>(x), i);
   });
-  if (mode == kSampListBin)  // kept mass of each part of the vocabulary, but for the cut's bin
+  if (mode == kSampListBin) {  // kept mass of each part of the vocabulary, but for the cut's bin
     for (int i = 0; i < A.chunks; ++i) {
-      samp_u64 s = 0;
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-        if (2 * tid + q < (int)cut.bin) s += A.mass[o + (int64_t)i * kSampBins + q];
-      s = samp_wave_sum(s);
+      const samp_u64x2 mi = *(const samp_u64x2*)(A.mass + o + (int64_t)i * kSampBins);
+      const samp_u64 s = samp_wave_sum((2 * tid < (int)cut.bin ? mi[0] : 0) + (2 * tid + 1 < (int)cut.bin ? mi[1] : 0));
       if (lane == 0 && s) atomicAdd(&chunk_mass[i], s);
     }
+  }
   __syncthreads();
   const int listed = min((int)listed_, kSampList);
   int size = 64;
   while (size < listed) size <<= 1;
   for (int i = listed + tid; i < size; i += kSampThreads) li.entry[i] = 0;
-  samp_sort(li.entry, size);
+  samp_sort(li.entry, li.rank, size);
   // weights in rank order (two ranks a thread), and what the cuts keep of them
   samp_u64 e[2], w[2];
   double wd[2];
@@ -658,7 +696,7 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
     return target >= sum_ ? sum_ - 1 : target;  // u of 1 and more: the last
   };
   if (mode == kSampListAll) {
-    samp_sort(li.entry, size);  // by ~index, descending: ascending indices first, dropped ones last
+    samp_sort(li.entry, li.rank, size);  // by ~index, descending: ascending indices first, dropped ones last
     samp_u64 x[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -699,15 +737,27 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   const int end = min((ch + 1) * A.chunk, n);
   for (int first = ch * A.chunk; first < end; first += 8 * kSampThreads) {  // 8 neighbours a thread
     samp_u64 x[8], s = 0;
+    float v[8];
+    const int i0 = first + 8 * tid;
+    if (A.vec && i0 + 8 <= end) {
+      constexpr int W = DT == TGM_F32 ? 2 : 1, V = 8 / W;
+#pragma unroll
+      for (int h = 0; h < W; ++h) {
+        const samp_u32x4 word = ((const samp_u32x4*)row)[i0 / V + h];
+#pragma unroll
+        for (int q = 0; q < V; ++q) v[h * V + q] = samp_value<DT>(&word, q);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = i0 + q < end ? samp_value<DT>(row, i0 + q) : -INFINITY;
+    }
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const int i = first + 8 * tid + q;
-      const float v = i < end ? samp_value<DT>(row, i) : -INFINITY;
       x[q] = 0;
-      if (v > -INFINITY) {
-        const double y = ex.log2w(v);
+      if (v[q] > -INFINITY) {
+        const double y = ex.log2w(v[q]);
         const int b = ex.bin(y);
-        if (b < (int)cut.bin || (b == (int)cut.bin && samp_entry(samp_key<DT>(v), i) >= lowest_kept)) x[q] = ex.fix(ex.weight_of(y));
+        if (b < (int)cut.bin || (b == (int)cut.bin && samp_entry(samp_key<DT>(v[q]), i0 + q) >= lowest_kept)) x[q] = ex.fix_of(y);
       }
       s += x[q];
     }
@@ -716,7 +766,7 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
     if (left < tile) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        if (x[q] > 0 && at <= left && at + x[q] > left) A.tokens[r] = (int32_t)(first + 8 * tid + q);
+        if (x[q] > 0 && at <= left && at + x[q] > left) A.tokens[r] = i0 + q;
         at += x[q];
       }
       return;

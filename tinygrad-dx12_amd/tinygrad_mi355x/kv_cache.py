@@ -22,7 +22,7 @@ from typing import NamedTuple
 
 import torch
 
-from tinygrad_mi355x.rotary import _DT, Rotary, check_heads, check_index, heads_arg
+from tinygrad_mi355x.rotary import _DT, _HEADS, Plans, Rotary, check_heads, check_index, heads_arg
 from tinygrad_mi355x.runtime import kernels as K
 
 FORMATS = {"fp8_e4m3": (0, 8), "fp4_e2m1": (1, 4)}  # enum tgm_kv_format, bits of a code
@@ -65,7 +65,7 @@ class PackedKVCache:
                                 self.v_scales.data_ptr(), pages, kv_heads, head_dim, page_size, FORMATS[k_format][0],
                                 FORMATS[v_format][0])
         self._scale = 1.0 / math.sqrt(head_dim)
-        self._workspace_of: dict[tuple, int] = {}
+        self._plans = Plans()
 
     def nbytes(self) -> int:
         return sum(t.numel() for t in (self.k_data, self.k_scales, self.v_data, self.v_scales))
@@ -78,8 +78,9 @@ class PackedKVCache:
         if table.device != self.device:
             raise ValueError(f"the page table is on {table.device}, the cache on {self.device}")
 
-    def _table_args(self, table: torch.Tensor) -> tuple[int, int, int]:
-        return table.data_ptr(), max(table.stride(0), table.shape[1]), table.shape[1]
+    @staticmethod
+    def _table_args(table: torch.Tensor) -> tuple[int, int]:
+        return max(table.stride(0), table.shape[1]), table.shape[1]
 
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor, *,
                rotary: Rotary | None = None, q: torch.Tensor | None = None,
@@ -90,10 +91,30 @@ class PackedKVCache:
         into a new tensor.  With ``seen`` the new keys and values come back in that type as the cache holds them.
         Positions outside the table, or whose entry names no page, are not stored.
         """
+        sig = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), table.shape,
+               table.stride(), table.dtype, table.get_device(), start.shape, start.stride(), start.dtype,
+               start.get_device(), rotary, seen) + (() if q is None else (q.shape, q.stride(), q.dtype, q.get_device()))
+        plan = self._plans.get(sig)
+        if plan is None:
+            plan = self._append_plan(sig, k, v, table, start, rotary, q, seen)
+        rot_arg, q_arg, qo_arg, k_arg, v_arg, seen_arg, ld, cols, batch, tokens, index = plan
+        q_out = k_out = v_out = None
+        q_ptr = qo_ptr = ko_ptr = vo_ptr = None
+        if q is not None:
+            q_out = q.new_empty(q.shape)
+            q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
+        if seen is not None:
+            k_out, v_out = k.new_empty(k.shape, dtype=seen), k.new_empty(k.shape, dtype=seen)
+            ko_ptr, vo_ptr = k_out.data_ptr(), v_out.data_ptr()
+        K.call("tgm_kv_append", self._arg, rot_arg, q_arg, q_ptr, qo_arg, qo_ptr, k_arg, k.data_ptr(), v_arg, v.data_ptr(),
+               seen_arg, ko_ptr, vo_ptr, table.data_ptr(), ld, cols, start.data_ptr(), batch, tokens, K.stream_on(index))
+        return Appended(q_out, k_out, v_out)
+
+    def _append_plan(self, sig, k, v, table, start, rotary, q, seen) -> tuple:
         check_heads(k, "k")
         check_heads(v, "v")
-        batch, tokens = k.shape[0], k.shape[1]
-        if k.shape[2] != self.kv_heads or k.shape[3] != self.head_dim or v.shape != k.shape:
+        batch, tokens, hk, hd = k.shape
+        if hk != self.kv_heads or hd != self.head_dim or v.shape != k.shape:
             raise ValueError(f"k and v must be [batch, tokens, {self.kv_heads}, {self.head_dim}], got {tuple(k.shape)} "
                              f"and {tuple(v.shape)}")
         if v.dtype is not k.dtype or k.device != self.device or v.device != self.device:
@@ -104,26 +125,19 @@ class PackedKVCache:
             rotary.check(k, self.head_dim)
         if q is not None:
             check_heads(q, "q")
-            if q.shape[:2] != k.shape[:2] or q.shape[3] != self.head_dim or q.dtype is not k.dtype or q.device != k.device:
+            if q.shape[:2] != k.shape[:2] or q.shape[2] < 1 or q.shape[3] != hd or q.dtype is not k.dtype or q.device != k.device:
                 raise ValueError("q must be [batch, tokens, heads, head_dim] beside k, of its type")
         if seen is not None and seen not in _DT:
             raise ValueError(f"seen must be float32, float16 or bfloat16, got {seen}")
         K.require_device(k)
-        q_out = k_out = v_out = None
-        q_arg = qo_arg = ko_arg = vo_arg = None
-        if q is not None:
-            if q.shape[2]:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-                q_arg, qo_arg = heads_arg(q), heads_arg(q_out)
-            else:
-                q_out = q
-        if seen is not None:
-            k_out = torch.empty(k.shape, dtype=seen, device=k.device)
-            v_out = torch.empty(k.shape, dtype=seen, device=k.device)
-            ko_arg, vo_arg = heads_arg(k_out), heads_arg(v_out)
-        K.call("tgm_kv_append", self._arg, None if rotary is None else rotary.arg, q_arg, qo_arg, heads_arg(k),
-               heads_arg(v), ko_arg, vo_arg, *self._table_args(table), start.data_ptr(), batch, tokens, K.stream_of(k))
-        return Appended(q_out, k_out, v_out)
+
+        def fresh(heads: int, dtype: torch.dtype) -> bytes:
+            return _HEADS(tokens * heads * hd, heads * hd, hd, heads, _DT[dtype])
+
+        ld, cols = self._table_args(table)
+        return self._plans.keep(sig, (None if rotary is None else rotary.arg, None if q is None else heads_arg(q),
+                                      None if q is None else fresh(q.shape[2], q.dtype), heads_arg(k), heads_arg(v),
+                                      None if seen is None else fresh(hk, seen), ld, cols, batch, tokens, k.get_device()))
 
     def read(self, table: torch.Tensor, first: torch.Tensor, count: int,
              dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
@@ -140,7 +154,7 @@ class PackedKVCache:
         K.require_device(self.k_data)
         shape = (batch, count, self.kv_heads, self.head_dim)
         k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
-        K.call("tgm_kv_read", self._arg, *self._table_args(table), first.data_ptr(), batch, count, k.data_ptr(),
+        K.call("tgm_kv_read", self._arg, table.data_ptr(), *self._table_args(table), first.data_ptr(), batch, count, k.data_ptr(),
                v.data_ptr(), _DT[dtype], K.stream_of(table))
         return k, v
 
@@ -155,6 +169,27 @@ class PackedKVCache:
         ``shared`` positions (a multiple of page_size) from the front are common to the batch: they lie in the pages
         that row 0 of the table names, and are read once for all sequences.
         """
+        scale = self._scale if scale is None else float(scale)
+        if not 0 < scale < 1e30:
+            raise ValueError(f"scale must be positive, got {scale}")
+        if out is not None and (out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device
+                                or not out.is_contiguous()):
+            raise ValueError("out must be like q, and contiguous")
+        sig = (q.shape, q.stride(), q.dtype, q.get_device(), table.shape, table.stride(), table.dtype, table.get_device(),
+               lengths.shape, lengths.stride(), lengths.dtype, lengths.get_device(), shared)
+        plan = self._plans.get(sig)
+        if plan is None:
+            plan = self._attend_plan(sig, q, table, lengths, shared)
+        q_arg, ld, cols, batch, tokens, need, index = plan
+        if out is None:
+            out = q.new_empty(q.shape)
+        # the workspace is of the caching allocator, so that calls on several streams never share one
+        workspace = q.new_empty(need, dtype=torch.uint8).data_ptr() if need else None
+        K.call("tgm_kv_attend", self._arg, q_arg, q.data_ptr(), table.data_ptr(), ld, cols, lengths.data_ptr(), batch, tokens,
+               shared, scale, workspace, need, out.data_ptr(), K.stream_on(index))
+        return out
+
+    def _attend_plan(self, sig, q, table, lengths, shared) -> tuple:
         check_heads(q, "q")
         batch, tokens, heads, head_dim = q.shape
         if head_dim != self.head_dim or heads < 1 or heads % self.kv_heads:
@@ -166,22 +201,7 @@ class PackedKVCache:
         check_index(lengths, "lengths", batch, q)
         if shared < 0 or shared % self.page_size or shared > table.shape[1] * self.page_size:
             raise ValueError(f"shared must be a multiple of {self.page_size} within the page table, got {shared}")
-        scale = self._scale if scale is None else float(scale)
-        if not 0 < scale < 1e30:
-            raise ValueError(f"scale must be positive, got {scale}")
-        if out is not None and (out.shape != q.shape or out.dtype is not q.dtype or out.device != q.device
-                                or not out.is_contiguous()):
-            raise ValueError("out must be like q, and contiguous")
         K.require_device(q)
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dt, cols = _DT[q.dtype], table.shape[1]
-        key = (dt, heads, batch, tokens, cols, shared)
-        need = self._workspace_of.get(key)
-        if need is None:
-            need = self._workspace_of[key] = K.load_library().tgm_kv_attend_workspace(self._arg, *key)
-        # of the caching allocator, so that calls on several streams never share one
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        K.call("tgm_kv_attend", self._arg, heads_arg(q), *self._table_args(table), lengths.data_ptr(), batch, tokens,
-               shared, scale, K.ptr(workspace), need, out.data_ptr(), K.stream_of(q))
-        return out
+        ld, cols = self._table_args(table)
+        need = K.load_library().tgm_kv_attend_workspace(self._arg, _DT[q.dtype], heads, batch, tokens, cols, shared)
+        return self._plans.keep(sig, (heads_arg(q), ld, cols, batch, tokens, need, q.get_device()))

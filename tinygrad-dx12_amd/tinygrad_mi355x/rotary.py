@@ -19,13 +19,24 @@ from tinygrad_mi355x.runtime import kernels as K
 LAYOUTS = {"half": 0, "interleaved": 1}
 FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 _DT = {dt: K.dtype_id(dt) for dt in FLOATS}
-_HEADS = struct.Struct("Pqqqqq").pack
+_HEADS = struct.Struct("qqqqq").pack
 
 
 def heads_arg(t: torch.Tensor) -> bytes:
     """struct tgm_heads of a tensor [batch, tokens, heads, head_dim]."""
     sb, st, sh, _ = t.stride()
-    return _HEADS(t.data_ptr(), sb, st, sh, t.shape[2], _DT[t.dtype])
+    return _HEADS(sb, st, sh, t.shape[2], _DT[t.dtype])
+
+
+class Plans(dict):
+    """What calls of one signature (shapes, strides, types, devices) have in common: checked once, then looked up, since
+    the checks of a call on a few tokens take longer than its kernel.  Bounded: a program has few signatures."""
+
+    def keep(self, key, plan):
+        if len(self) >= 512:
+            self.clear()
+        self[key] = plan
+        return plan
 
 
 def check_heads(t: torch.Tensor, name: str) -> None:
@@ -109,6 +120,7 @@ class Rotary:
         self.head_dim, self.rotary_dim, self.base, self.layout = head_dim, rotary_dim, base, layout
         freq, self.gain = frequencies(rotary_dim, base, scaling)
         self.freq = freq.to(device)
+        self._plans = Plans()
         self.arg = struct.pack("Pdqq", self.freq.data_ptr(), self.gain, rotary_dim, LAYOUTS[layout])  # struct tgm_rotary
 
     def check(self, x: torch.Tensor, head_dim: int) -> None:
@@ -122,17 +134,28 @@ class Rotary:
 
         ``start``: int32 [batch].  ``out`` may be x itself.  Angles, sines and products are computed in 64 bits.
         """
-        check_heads(x, "x")
-        batch, tokens, _, head_dim = x.shape
-        self.check(x, head_dim)
-        check_index(start, "start", batch, x)
+        sig = (x.shape, x.stride(), x.dtype, x.get_device(), start.shape, start.stride(), start.dtype, start.get_device())
+        plan = self._plans.get(sig)
+        if plan is None:
+            plan = self._plan(sig, x, start)
+        x_arg, out_arg, shape, batch, tokens, index = plan
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out = x.new_empty(shape)
         else:
             check_heads(out, "out")
-            if out.shape != x.shape or out.dtype is not x.dtype or out.device != x.device:
+            if out.shape != shape or out.dtype is not x.dtype or out.device != x.device:
                 raise ValueError("out must be like x")
-        K.require_device(x)
-        K.call("tgm_rotate", self.arg, heads_arg(x), heads_arg(out), start.data_ptr(), batch, tokens, head_dim,
-               K.stream_of(x))
+            out_arg = heads_arg(out)
+        K.call("tgm_rotate", self.arg, x_arg, x.data_ptr(), out_arg, out.data_ptr(), start.data_ptr(), batch, tokens,
+               self.head_dim, K.stream_on(index))
         return out
+
+    def _plan(self, sig, x: torch.Tensor, start: torch.Tensor) -> tuple:
+        check_heads(x, "x")
+        batch, tokens, heads, head_dim = x.shape
+        self.check(x, head_dim)
+        check_index(start, "start", batch, x)
+        K.require_device(x)
+        row = heads * head_dim
+        out_arg = _HEADS(tokens * row, row, head_dim, heads, _DT[x.dtype])
+        return self._plans.keep(sig, (heads_arg(x), out_arg, x.shape, batch, tokens, x.get_device()))

@@ -52,5 +52,12 @@ def stream_of(t: torch.Tensor) -> int:
     return _raw_stream(index)
 
 
+def stream_on(index: int) -> int:
+    """The current stream of device ``index``."""
+    if _raw_stream is None:
+        return torch.cuda.current_stream(index).cuda_stream
+    return _raw_stream(index)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()

@@ -89,10 +89,10 @@ SIGNATURES = {
     "tgm_dec_gemv_bf16": (_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P),
     "tgm_dec_argmax": (_P, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P),
     # serving operators (include/tgm_serving.h)
-    "tgm_rotate": (_P, _P, _P, _P, _I64, _I64, _I64, _P),
-    "tgm_kv_append": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P),
+    "tgm_rotate": (_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P),
+    "tgm_kv_append": (_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P),
     "tgm_kv_read": (_P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _INT, _P),
-    "tgm_kv_attend": (_P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, ctypes.c_double, _P, _I64, _P, _P),
+    "tgm_kv_attend": (_P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, ctypes.c_double, _P, _I64, _P, _P),
     "tgm_sample": (_P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P),
 }
 EXPORTS = ("tgm_abi_version", "tgm_last_error", "tgm_dec_attention_workspace", "tgm_gemm_w_split_workspace",

@@ -8,21 +8,11 @@ from __future__ import annotations
 
 import torch
 
-from tinygrad_mi355x.rotary import _DT
+from tinygrad_mi355x.rotary import _DT, Plans
 from tinygrad_mi355x.runtime import kernels as K
 
 MAX_VOCAB = 1 << 20
-_workspace_of: dict[tuple, int] = {}
-
-
-def _per_row(value, name: str, rows: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    if isinstance(value, torch.Tensor):
-        if value.dtype is not dtype or value.dim() != 1 or value.shape[0] != rows or not value.is_contiguous():
-            raise ValueError(f"{name} must be a number or contiguous {dtype} [{rows}], got {value.dtype} {tuple(value.shape)}")
-        if value.device != device:
-            raise ValueError(f"{name} is on {value.device}, not on {device}")
-        return value
-    return torch.full((rows,), value, dtype=dtype, device=device)
+_plans = Plans()
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor | float = 1.0,
@@ -38,6 +28,38 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
 
     Each parameter is one number, or a contiguous tensor with one per row (float32; top_k int32).
     """
+    if out is not None and logits.dim():
+        _per_row(out, "out", logits.shape[0], torch.int32, logits.device)
+    sig = (logits.shape, logits.stride(), logits.dtype, logits.get_device(), _signature(u), _signature(temperature),
+           _signature(top_k), _signature(top_p), _signature(min_p))
+    plan = _plans.get(sig)
+    if plan is None:
+        plan = _plan(sig, logits, u, temperature, top_k, top_p, min_p)
+    dt, rows, vocab, ld, need, index, numbers = plan
+    if numbers:  # given as plain numbers
+        temperature = _filled(temperature, rows, torch.float32, logits.device)
+        top_k = _filled(top_k, rows, torch.int32, logits.device)
+        top_p = _filled(top_p, rows, torch.float32, logits.device)
+        min_p = _filled(min_p, rows, torch.float32, logits.device)
+    if out is None:
+        out = logits.new_empty(rows, dtype=torch.int32)
+    # the workspace is of the caching allocator, so that calls on several streams never share one
+    workspace = logits.new_empty(need, dtype=torch.uint8).data_ptr() if need else None
+    K.call("tgm_sample", logits.data_ptr(), dt, rows, vocab, ld, u.data_ptr(), temperature.data_ptr(),
+           None if top_k is None else top_k.data_ptr(), None if top_p is None else top_p.data_ptr(),
+           None if min_p is None else min_p.data_ptr(), out.data_ptr(), workspace, need, K.stream_on(index))
+    return out
+
+
+def _signature(t):
+    return (t.shape, t.stride(), t.dtype, t.get_device()) if isinstance(t, torch.Tensor) else type(t)
+
+
+def _filled(value, rows: int, dtype: torch.dtype, device: torch.device):
+    return value if value is None or isinstance(value, torch.Tensor) else torch.full((rows,), value, dtype=dtype, device=device)
+
+
+def _plan(sig, logits, u, temperature, top_k, top_p, min_p) -> tuple:
     if logits.dim() != 2 or logits.dtype not in _DT:
         raise ValueError(f"logits must be float32, float16 or bfloat16 [rows, vocab], got {logits.dtype} "
                          f"{tuple(logits.shape)}")
@@ -46,27 +68,28 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
         raise ValueError(f"the vocabulary must hold 1 to {MAX_VOCAB} tokens, got {vocab}")
     if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
         raise ValueError("rows of logits must be contiguous and apart")
-    device = logits.device
-    u = _per_row(u, "u", rows, torch.float32, device)
-    temperature = _per_row(temperature, "temperature", rows, torch.float32, device)
-    if top_k is not None:
-        top_k = _per_row(top_k, "top_k", rows, torch.int32, device)
-    if top_p is not None:
-        top_p = _per_row(top_p, "top_p", rows, torch.float32, device)
-    if min_p is not None:
-        min_p = _per_row(min_p, "min_p", rows, torch.float32, device)
-    if out is not None:
-        _per_row(out, "out", rows, torch.int32, device)
+    if not isinstance(u, torch.Tensor):
+        raise ValueError("u must be a tensor: one random number per row")
+    numbers = False
+    for value, name, dtype in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
+                               (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                               (min_p, "min_p", torch.float32)):
+        if isinstance(value, torch.Tensor):
+            _per_row(value, name, rows, dtype, logits.device)
+        elif value is not None:
+            if not isinstance(value, (int, float)) or name == "top_k" and not isinstance(value, int):
+                raise ValueError(f"{name} must be a number or a tensor, got {value!r}")
+            numbers = True
+        elif name == "temperature":
+            raise ValueError("temperature must be a number or a tensor")
     K.require_device(logits)
-    if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device=device)
     dt = _DT[logits.dtype]
-    key = (rows, vocab, dt)
-    need = _workspace_of.get(key)
-    if need is None:
-        need = _workspace_of[key] = K.load_library().tgm_sample_workspace(*key)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    K.call("tgm_sample", logits.data_ptr(), dt, rows, vocab, max(logits.stride(0), vocab), u.data_ptr(),
-           temperature.data_ptr(), K.ptr(top_k), K.ptr(top_p), K.ptr(min_p), out.data_ptr(), K.ptr(workspace), need,
-           K.stream_of(logits))
-    return out
+    need = K.load_library().tgm_sample_workspace(rows, vocab, dt)
+    return _plans.keep(sig, (dt, rows, vocab, max(logits.stride(0), vocab), need, logits.get_device(), numbers))
+
+
+def _per_row(t: torch.Tensor, name: str, rows: int, dtype: torch.dtype, device: torch.device) -> None:
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
+        raise ValueError(f"{name} must be a number or contiguous {dtype} [{rows}], got {t.dtype} {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
