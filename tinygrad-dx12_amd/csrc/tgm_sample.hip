@@ -25,13 +25,14 @@
 
 namespace tgm {
 
+constexpr int kCutThreads = 256;  // of sample_draw, 8 bins each
 constexpr int kSampThreads = 1024, kSampWaves = 16, kSampBins = 2048;
 typedef unsigned long long samp_u64;
 typedef unsigned samp_u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned samp_u32x4 __attribute__((ext_vector_type(4)));
 typedef samp_u64 samp_u64x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kSampList = 2048, kSampMostChunks = 16;
+constexpr int kSampList = 2048, kSampQueue = 2 * kSampList, kSampMostChunks = 16;
 constexpr double kSampPerBin = 40.0;  // bins per power of two of a weight: 2047 of them reach 2^-51
 
 struct SampleArgs {
@@ -108,13 +109,10 @@ struct SampExp {
   const double* table;
   double max, rate;  // rate = log2(e) / temperature
   int fbits;
-  bool infinite;     // the maximum is +inf: it weighs 1, all else 0
   __device__ __forceinline__ SampExp(const double* t, float best, float temperature, int f)
-      : table(t), max(best), rate(1.4426950408889634074 / (double)temperature), fbits(f), infinite(best == INFINITY) {}
-  __device__ __forceinline__ double log2w(float x) const {
-    const double y = ((double)x - max) * rate;
-    return infinite ? (x == INFINITY ? 0.0 : -INFINITY) : y;
-  }
+      : table(t), max(best), rate(1.4426950408889634074 / (double)temperature), fbits(f) {}
+  // the minimum turns inf - inf, a maximum of +inf itself, into 0
+  __device__ __forceinline__ double log2w(float x) const { return fmin(((double)x - max) * rate, 0.0); }
   // bins of 1 / 40 of a power of two, descending with x; kSampBins - 1 for weights that round to 0
   __device__ __forceinline__ int bin(double y) const {
     const double b = y * -kSampPerBin;
@@ -161,18 +159,28 @@ __device__ __forceinline__ void samp_each(const void* row, int first, int last, 
   for (int i = done + threadIdx.x; i < last; i += THREADS) f(samp_value<DT>(row, i), i);
 }
 
-__device__ __forceinline__ samp_u64 samp_shfl_up(samp_u64 v, int d) {
-  const unsigned lo = __shfl_up((unsigned)v, d, 64), hi = __shfl_up((unsigned)(v >> 32), d, 64);
+// Inclusive prefix sum over the wave by DPP moves alone: shifts within rows of 16, then the rows' totals.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ samp_u64 samp_dpp(samp_u64 v) {
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xF, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xF, false);
   return ((samp_u64)hi << 32) | lo;
 }
-__device__ __forceinline__ samp_u64 samp_wave_sum(samp_u64 v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const unsigned lo = __shfl_xor((unsigned)v, o, 64), hi = __shfl_xor((unsigned)(v >> 32), o, 64);
-    v += ((samp_u64)hi << 32) | lo;
-  }
+__device__ __forceinline__ samp_u64 samp_wave_scan(samp_u64 v) {
+  v += samp_dpp<0x111, 0xF>(v);  // row_shr:1
+  v += samp_dpp<0x112, 0xF>(v);
+  v += samp_dpp<0x114, 0xF>(v);
+  v += samp_dpp<0x118, 0xF>(v);
+  v += samp_dpp<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  v += samp_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
   return v;
 }
+__device__ __forceinline__ samp_u64 samp_lane(samp_u64 v, int lane) {
+  const unsigned lo = __builtin_amdgcn_readlane((int)(unsigned)v, lane);
+  const unsigned hi = __builtin_amdgcn_readlane((int)(unsigned)(v >> 32), lane);
+  return ((samp_u64)hi << 32) | lo;
+}
+__device__ __forceinline__ samp_u64 samp_wave_sum(samp_u64 v) { return samp_lane(samp_wave_scan(v), 63); }
 
 struct SampShared {
   samp_u64 mass[kSampBins];
@@ -200,17 +208,8 @@ __device__ __forceinline__ void samp_find(SampShared& sh, int bins, bool by_mass
       m[e] = sh.mass[b];
     }
   }
-  unsigned pc = c[0] + c[1];
-  samp_u64 pm = m[0] + m[1];
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned uc = __shfl_up(pc, o, 64);
-    const samp_u64 um = samp_shfl_up(pm, o);
-    if (lane >= o) {
-      pc += uc;
-      pm += um;
-    }
-  }
+  unsigned pc = (unsigned)samp_wave_scan(c[0] + c[1]);
+  samp_u64 pm = samp_wave_scan(m[0] + m[1]);
   if (lane == 63) {
     sh.wave_count[wave] = pc;
     sh.wave_mass[wave] = pm;
@@ -386,20 +385,14 @@ __device__ void sample_descend(const SampleArgs& A, SampShared& sh, const void* 
     const int64_t end = min((int64_t)n, lo + seg / kSampWaves);
     for (int64_t i0 = lo; i0 < end; i0 += 64) {
       const int64_t i = i0 + lane;
-      samp_u64 s = i < end ? kept(samp_value<DT>(row, i), i) : 0;
-      const samp_u64 own = s;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const samp_u64 up = samp_shfl_up(s, o);
-        if (lane >= o) s += up;
-      }
+      const samp_u64 own = i < end ? kept(samp_value<DT>(row, i), i) : 0;
+      const samp_u64 s = samp_wave_scan(own);
       const samp_u64 hit = __ballot(base + s > target && own > 0);
       if (hit) {
         if (lane == __ffsll((unsigned long long)hit) - 1) A.tokens[r] = (int32_t)i;
         break;
       }
-      const unsigned lo32 = __shfl((unsigned)s, 63, 64), hi32 = __shfl((unsigned)(s >> 32), 63, 64);
-      base += ((samp_u64)hi32 << 32) | lo32;
+      base += samp_lane(s, 63);
     }
   }
 }
@@ -461,35 +454,24 @@ __global__ void __launch_bounds__(kBinThreads) sample_bins(const SampleArgs A) {
   }
 }
 
-// Exclusive prefix of v over the workgroup, and its total.
-template <int THREADS, typename T>
-__device__ __forceinline__ T samp_scan(T v, T* part, T& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    T up;
-    if constexpr (sizeof(T) == 8) up = samp_shfl_up(s, o);
-    else up = __shfl_up(s, o, 64);
-    if (lane >= o) s += up;
-  }
+// Exclusive prefix of v over the workgroup's first WAVES waves (the others pass 0), and its total.
+template <int WAVES>
+__device__ __forceinline__ samp_u64 samp_scan(samp_u64 v, samp_u64* part, samp_u64& total) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const samp_u64 s = samp_wave_scan(v);
   __syncthreads();  // the last scan's partials have been read
-  if (lane == 63) part[wave] = s;
+  if (lane == 63 && wave < WAVES) part[wave] = s;
   __syncthreads();
-  T before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    before += w < wave ? part[w] : 0;
-    total += part[w];
-  }
+  const samp_u64 p = samp_wave_scan(lane < WAVES ? part[lane] : 0);
+  total = samp_lane(p, 63);
+  const samp_u64 before = wave > 0 ? samp_lane(p, wave - 1) : 0;  // wave is uniform
   return before + s - v;
 }
 
 // A listed token: descending order of these is descending by value, ascending by index.
 __device__ __forceinline__ samp_u64 samp_entry(unsigned key, int i) { return ((samp_u64)key << 32) | (unsigned)~i; }
 
-// Sorts size (a power of two from 64 to 2048) entries in LDS by 1024 threads, descending; entries differ but for zeros.
+// Sorts size (a power of two from 64 to 2048) entries in LDS by 1024 threads, descending; no two entries are alike.
 // Up to 512 by counting the larger ones, several threads an entry (two barriers; 64 entries: about 0.3 us where the
 // network's 21 barriers take 2), beyond by a bitonic network.  `rank` holds `size` counters.
 __device__ __forceinline__ void samp_sort(samp_u64* v, unsigned* rank, int size) {
@@ -500,7 +482,8 @@ __device__ __forceinline__ void samp_sort(samp_u64* v, unsigned* rank, int size)
     __syncthreads();
     const samp_u64 mine = v[i];
     unsigned n = 0;
-    for (int j = j0; j < j0 + share; ++j) n += v[j] > mine || (v[j] == mine && j < i);
+#pragma unroll 4
+    for (int j = j0; j < j0 + share; ++j) n += v[j] > mine;
     if (n) atomicAdd(&rank[i], n);
     __syncthreads();
     if (t < size) v[rank[t]] = mine;
@@ -538,14 +521,17 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   __shared__ union {
     SampShared sh;
     SampList li;
+    struct {
+      samp_u64 mass[kSampBins];
+      unsigned count[kSampBins];
+    } bins;
   } u_;
   __shared__ double table[64];
   __shared__ samp_u64 part[kSampWaves], chunk_mass[kSampMostChunks];
-  __shared__ unsigned npart[kSampWaves];
-  __shared__ unsigned listed_, kept_count;
+  __shared__ unsigned listed_, queued_, kept_count;
   __shared__ SampCut kcut, pcut, mcut, last;
   __shared__ int first_at;
-  const int tid = threadIdx.x, lane = tid & 63, n = A.n;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = A.n;
   const int64_t r = blockIdx.x;
   const char* row = (const char*)A.logits + r * A.ld * (DT == TGM_F32 ? 4 : 2);
   const float temp = A.temperature[r], best = A.max[r];
@@ -569,57 +555,77 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   }
   samp_load_table(table);
   if (tid == 0) {
-    listed_ = kept_count = 0;
+    listed_ = queued_ = kept_count = 0;
     kcut.bin = pcut.bin = mcut.bin = last.bin = kSampBins;
   }
   if (tid < kSampMostChunks) chunk_mass[tid] = 0;
   const SampExp ex(table, best, temp, A.fbits);
   const double p = A.top_p ? (double)A.top_p[r] : 1.0, min_p = A.min_p ? (double)A.min_p[r] : 0.0;
 
-  // two bins a thread, all parts of the row
-  samp_u64 m[2] = {0, 0};
-  unsigned c[2] = {0, 0};
-  const int64_t o = r * A.chunks * kSampBins + 2 * tid;
+  // all parts of the row, two bins a thread
+  {
+    samp_u64 m[2] = {0, 0};
+    unsigned c[2] = {0, 0};
+    const int64_t o = r * A.chunks * kSampBins + 2 * tid;
 #pragma unroll
-  for (int i0 = 0; i0 < kSampMostChunks; i0 += 8) {  // eight parts' loads in flight
-    samp_u64x2 mi[8];
-    samp_u32x2 ci[8];
+    for (int i0 = 0; i0 < kSampMostChunks; i0 += 8) {  // eight parts' loads in flight
+      samp_u64x2 mi[8];
+      samp_u32x2 ci[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      mi[i] = samp_u64x2{0, 0};
-      ci[i] = samp_u32x2{0, 0};
-      if (i0 + i < A.chunks) {
-        mi[i] = *(const samp_u64x2*)(A.mass + o + (int64_t)(i0 + i) * kSampBins);
-        ci[i] = *(const samp_u32x2*)(A.count + o + (int64_t)(i0 + i) * kSampBins);
+      for (int i = 0; i < 8; ++i) {
+        mi[i] = samp_u64x2{0, 0};
+        ci[i] = samp_u32x2{0, 0};
+        if (i0 + i < A.chunks) {
+          mi[i] = *(const samp_u64x2*)(A.mass + o + (int64_t)(i0 + i) * kSampBins);
+          ci[i] = *(const samp_u32x2*)(A.count + o + (int64_t)(i0 + i) * kSampBins);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          m[q] += mi[i][q];
+          c[q] += ci[i][q];
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        m[q] += mi[i][q];
-        c[q] += ci[i][q];
-      }
+    for (int q = 0; q < 2; ++q) {
+      u_.bins.mass[2 * tid + q] = m[q];
+      u_.bins.count[2 * tid + q] = c[q];
+    }
   }
-  samp_u64 total;
-  unsigned all;
-  samp_u64 mb = samp_scan<kSampThreads>(m[0] + m[1], part, total);
-  unsigned nb = samp_scan<kSampThreads>(c[0] + c[1], npart, all);
-  int k = A.top_k ? A.top_k[r] : 0;
-  if (k < 0 || k >= n || (unsigned)k >= all) k = 0;  // what is not counted weighs nothing
-  const double goal_p = p * (double)total;
-  // the bin of min_p: tokens above it weigh more, tokens below it less
-  const int mbin = min_p > 0.0 ? (min_p >= 1.0 ? 0 : ex.bin(log2(min_p))) : kSampBins - 2;
+  __syncthreads();
+  // prefixes and cuts: four waves with eight bins a thread (sixteen waves spend more on the scan than on its terms)
+  samp_u64 m[8] = {}, msum = 0;
+  unsigned c[8] = {}, csum = 0;
+  if (tid < kCutThreads)
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int b = 2 * tid + q;
-    const SampCut here{(unsigned)b, nb + c[q], c[q], mb};
-    if (k > 0 && nb < (unsigned)k && nb + c[q] >= (unsigned)k) kcut = here;
-    // the first bin with which the mass reaches the goal, with a goal of 0 and less the first one of all
-    if (p < 1.0 && c[q] > 0 && (nb == 0 || (double)mb < goal_p) && (double)(mb + m[q]) >= goal_p) pcut = here;
-    if (b == mbin) mcut = here;
-    mb += m[q];
-    nb += c[q];
+    for (int q = 0; q < 8; ++q) {
+      m[q] = u_.bins.mass[8 * tid + q];
+      c[q] = u_.bins.count[8 * tid + q];
+      msum += m[q];
+      csum += c[q];
+    }
+  samp_u64 total, all;
+  samp_u64 mb = samp_scan<kCutThreads / 64>(msum, part, total);
+  unsigned nb = (unsigned)samp_scan<kCutThreads / 64>(csum, part, all);
+  int k = A.top_k ? A.top_k[r] : 0;
+  if (k < 0 || k >= n || (unsigned)k >= (unsigned)all) k = 0;  // what is not counted weighs nothing
+  const double goal_p = p * (double)total;
+  if (tid < kCutThreads) {
+    // the bin of min_p: tokens above it weigh more, tokens below it less
+    const int mbin = min_p > 0.0 ? (min_p >= 1.0 ? 0 : ex.bin(log2(min_p))) : kSampBins - 2;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int b = 8 * tid + q;
+      const SampCut here{(unsigned)b, nb + c[q], c[q], mb};
+      if (k > 0 && nb < (unsigned)k && nb + c[q] >= (unsigned)k) kcut = here;
+      // the first bin with which the mass reaches the goal, with a goal of 0 and less the first one of all
+      if (p < 1.0 && c[q] > 0 && (nb == 0 || (double)mb < goal_p) && (double)(mb + m[q]) >= goal_p) pcut = here;
+      if (b == mbin) mcut = here;
+      mb += m[q];
+      nb += c[q];
+    }
   }
   __syncthreads();
   SampCut cut = mcut;  // everything that min_p leaves
@@ -639,28 +645,57 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   // The list.  Which tokens may belong to it is asked in 32 bits, with bounds half a bin too wide.
   SampList& li = u_.li;
   const double step = 1.0 / (kSampPerBin * ex.rate);
-  const float lowest = (float)((double)best - ((double)cut.bin + 1.5) * step);
-  const float highest = mode == kSampListAll ? INFINITY : (float)((double)best - ((double)cut.bin - 0.5) * step);
-  const bool wide = !(step > (double)fabsf(best) * 0x1p-20);  // bins near the resolution of 32 bits: no bounds
-  samp_each<DT, kSampThreads>(row, 0, n, A.vec, [&](float x, int i) {
-    if (!(x > -INFINITY) || (!wide && (x < lowest || x > highest))) return;
+  const bool narrow = step > (double)fabsf(best) * 0x1p-20 && best < INFINITY;  // else bins near 32 bits' resolution
+  const double low = (double)best - ((double)cut.bin + 1.5) * step;
+  const double high = mode == kSampListAll ? (double)best : (double)best - ((double)cut.bin - 0.5) * step;
+  const float middle = narrow ? (float)(0.5 * (low + high)) : 0.f, reach = narrow ? (float)(0.5 * (high - low) + step) : INFINITY;
+  __syncthreads();  // the bins have been read
+  auto consider = [&](float x, int i) __attribute__((always_inline)) {
+    if (!(fabsf(x - middle) <= reach)) return;  // NaN too
     const int b = ex.bin(ex.log2w(x));
     if (b > (int)cut.bin || b >= kSampBins - 1 || (mode == kSampListBin && b != (int)cut.bin)) return;
     const unsigned at = atomicAdd(&listed_, 1u);
     if (at < kSampList) li.entry[at] = samp_entry(samp_key<DT>(x), i);
-  });
-  if (mode == kSampListBin) {  // kept mass of each part of the vocabulary, but for the cut's bin
-    for (int i = 0; i < A.chunks; ++i) {
-      const samp_u64x2 mi = *(const samp_u64x2*)(A.mass + o + (int64_t)i * kSampBins);
-      const samp_u64 s = samp_wave_sum((2 * tid < (int)cut.bin ? mi[0] : 0) + (2 * tid + 1 < (int)cut.bin ? mi[1] : 0));
-      if (lane == 0 && s) atomicAdd(&chunk_mass[i], s);
+  };
+  // Whole 16-byte vectors first: the few that may hold such a token are queued, and looked into by as many threads
+  // afterwards (a test and a branch for each token of the row cost three times as much).
+  constexpr int V = DT == TGM_F32 ? 4 : 8;
+  const int nv = A.vec ? n / V : 0;
+  unsigned* queue = (unsigned*)li.weight;
+#pragma unroll 4
+  for (int i = tid; i < nv; i += kSampThreads) {
+    const samp_u32x4 word = ((const samp_u32x4*)row)[i];
+    float d = INFINITY;  // the smallest distance; NaN does not count
+#pragma unroll
+    for (int q = 0; q < V; ++q) d = fminf(d, fabsf(load_f32(&word, DT, q) - middle));
+    if (d <= reach) {
+      const unsigned at = atomicAdd(&queued_, 1u);
+      if (at < kSampQueue) queue[at] = (unsigned)i;
     }
+  }
+  __syncthreads();
+  const int queued = (int)queued_;
+  if (queued <= kSampQueue) {
+    for (int j = tid; j < queued * V; j += kSampThreads) {
+      const int i = (int)queue[j / V] * V + j % V;
+      consider(samp_value<DT>(row, i), i);
+    }
+  } else {
+    for (int i = tid; i < nv * V; i += kSampThreads) consider(samp_value<DT>(row, i), i);
+  }
+  for (int i = nv * V + tid; i < n; i += kSampThreads) consider(samp_value<DT>(row, i), i);
+  if (mode == kSampListBin && wave < A.chunks) {  // kept mass of each part of the vocabulary, but for the cut's bin
+    const samp_u64* part_mass = A.mass + (r * A.chunks + wave) * kSampBins;
+    samp_u64 s = 0;
+    for (int b = lane; b < (int)cut.bin; b += 64) s += part_mass[b];
+    s = samp_wave_sum(s);
+    if (lane == 0) chunk_mass[wave] = s;
   }
   __syncthreads();
   const int listed = min((int)listed_, kSampList);
   int size = 64;
   while (size < listed) size <<= 1;
-  for (int i = listed + tid; i < size; i += kSampThreads) li.entry[i] = 0;
+  for (int i = listed + tid; i < size; i += kSampThreads) li.entry[i] = (samp_u64)(i + 1);  // below every token's
   samp_sort(li.entry, li.rank, size);
   // weights in rank order (two ranks a thread), and what the cuts keep of them
   samp_u64 e[2], w[2];
@@ -674,7 +709,7 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
     w[q] = in ? ex.fix(wd[q]) : 0;
   }
   samp_u64 sum;
-  samp_u64 before = samp_scan<kSampThreads>(w[0] + w[1], part, sum) + (mode == kSampListBin ? cut.above : 0);
+  samp_u64 before = samp_scan<kSampWaves>(w[0] + w[1], part, sum) + (mode == kSampListBin ? cut.above : 0);
   const double goal = p * (double)(k > 0 ? sum : total);
   unsigned mine = 0;
 #pragma unroll
@@ -687,7 +722,7 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
     mine += keep;
     if (i < size) li.weight[i] = w[q];
     // next: the kept ones by index, so that the draw runs in the vocabulary's order
-    if (i < size && mode == kSampListAll) li.entry[i] = keep ? (((e[q] & 0xFFFFFFFFull) << 32) | (unsigned)(i + 1)) : 0;
+    if (i < size && mode == kSampListAll) li.entry[i] = keep ? (((e[q] & 0xFFFFFFFFull) << 32) | (unsigned)(i + 1)) : (samp_u64)(i + 1);
   }
   const double u = (double)A.u[r];
   auto target_of = [&](samp_u64 sum_) __attribute__((always_inline)) -> samp_u64 {
@@ -702,10 +737,10 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
     for (int q = 0; q < 2; ++q) {
       const int i = 2 * tid + q;
       e[q] = i < size ? li.entry[i] : 0;
-      x[q] = e[q] ? li.weight[(unsigned)e[q] - 1] : 0;
+      x[q] = e[q] >> 32 ? li.weight[(unsigned)e[q] - 1] : 0;
     }
     samp_u64 kept;
-    samp_u64 at = samp_scan<kSampThreads>(x[0] + x[1], part, kept);
+    samp_u64 at = samp_scan<kSampWaves>(x[0] + x[1], part, kept);
     if (kept == 0) {  // min_p above 1
       if (tid == 0) A.tokens[r] = 0;
       return;
@@ -762,7 +797,7 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
       s += x[q];
     }
     samp_u64 tile;
-    samp_u64 at = samp_scan<kSampThreads>(s, part, tile);
+    samp_u64 at = samp_scan<kSampWaves>(s, part, tile);
     if (left < tile) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
@@ -782,9 +817,9 @@ struct SampSizes {
 
 static SampSizes samp_sizes(int64_t rows, int64_t vocab) {
   SampSizes z;
-  // two workgroups a CU, 2048 tokens each at least
+  // two workgroups a CU, 4096 tokens each at least: every part adds 24 KB to what sample_draw reads
   int64_t c = (512 + rows - 1) / rows;
-  const int64_t most = (vocab + 2047) / 2048;
+  const int64_t most = (vocab + 4095) / 4096;
   c = c > most ? most : c;
   c = c > kSampMostChunks ? kSampMostChunks : c;
   z.chunk = (int)((vocab + c * 1024 - 1) / (c * 1024)) * 1024;
