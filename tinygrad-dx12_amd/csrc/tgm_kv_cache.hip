@@ -11,6 +11,7 @@ struct AppendView {
 };
 struct AppendArgs {
   AppendView q, qo, k, v, ko, vo;
+  int vec;  // all of q, k and v take 16-byte loads
   int H, HK, seen;  // seen: dtype of ko and vo, or -1
   KvStore ks, vs;
   int kf, vf;
@@ -103,21 +104,33 @@ __global__ void __launch_bounds__(256) kv_append(const AppendArgs A) {
   const int part = (int)(w - token * A.parts);
   const int b = (int)(token / A.T), t = (int)(token - (int64_t)b * A.T);
   const int chunk = lane % LPH, sub = lane / LPH;
+  const int heads = A.H + 2 * A.HK;
+  // heads of this lane: the next one's values are under way while one is rotated and stored
+  const int64_t qi = b * A.q.sb + t * A.q.st, ki = b * A.k.sb + t * A.k.st, vi = b * A.v.sb + t * A.v.st;
+  auto fetch = [&](int h, const void*& x, int64_t& at, float (&u)[8], float (&v)[8]) __attribute__((always_inline)) {
+    const bool is_q = h < A.H, is_k = h < A.H + A.HK;
+    x = is_q ? A.q.p : (is_k ? A.k.p : A.v.p);
+    at = is_q ? qi + h * A.q.sh : (is_k ? ki + (h - A.H) * A.k.sh : vi + (h - A.H - A.HK) * A.v.sh);
+    const bool vec = A.vec;  // of all three: uniform
+    kv_load8<DT>(x, at + 8 * chunk, vec, u);
+    kv_load8<DT>(x, at + HD / 2 + 8 * chunk, vec, v);
+  };
+  const void *x, *x2;
+  int64_t at, at2;
+  float u[8], v[8], u2[8], v2[8];
+  int h = part * HPI + sub;
+  if (h < heads) fetch(h, x, at, u, v);
   const int pos = A.start[b] + t;
   const int page = kv_page(A.pg, A.pg.table + b * A.pg.ld, pos), slot = pos & A.pg.mask;
   RotLane<HD, MODE> turn;
   if constexpr (MODE != kRotNone) rot_angles(A.rot, pos, lane, angles[wave]);
   if constexpr (MODE == kRotHalf || MODE == kRotInterleaved) turn.load(A.rot, angles[wave], chunk);
-  const int heads = A.H + 2 * A.HK;
-  for (int h = part * HPI + sub; h < heads; h += A.parts * HPI) {
+  for (; h < heads; h += A.parts * HPI) {
+    const int next = h + A.parts * HPI;
+    if (next < heads) fetch(next, x2, at2, u2, v2);
     const int which = h < A.H ? 0 : (h < A.H + A.HK ? 1 : 2);
-    const AppendView& x = which == 0 ? A.q : (which == 1 ? A.k : A.v);
     const int hh = which == 0 ? h : (which == 1 ? h - A.H : h - A.H - A.HK);
-    const int64_t at = b * x.sb + t * x.st + hh * x.sh;
-    float u[8], v[8];
-    kv_load8<DT>(x.p, at + 8 * chunk, x.vec, u);
-    kv_load8<DT>(x.p, at + HD / 2 + 8 * chunk, x.vec, v);
-    if (which < 2) rot_apply<DT, HD, MODE>(A.rot, turn, angles[wave], chunk, x.p, at, u, v);
+    if (which < 2) rot_apply<DT, HD, MODE>(A.rot, turn, angles[wave], chunk, x, at, u, v);
     if (which == 0) {
       const int64_t to = b * A.qo.sb + t * A.qo.st + hh * A.qo.sh;
       kv_store8<DT>(A.qo.p, to + 8 * chunk, A.qo.vec, u);
@@ -129,6 +142,12 @@ __global__ void __launch_bounds__(256) kv_append(const AppendArgs A) {
       const int64_t to = b * o.sb + t * o.st + hh * o.sh;
       kv_put8(fmt, st, A.pg, HD, A.HK, page, slot, hh, 8 * chunk, u, o, to, A.seen);
       kv_put8(fmt, st, A.pg, HD, A.HK, page, slot, hh, HD / 2 + 8 * chunk, v, o, to, A.seen);
+    }
+    x = x2, at = at2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      u[e] = u2[e];
+      v[e] = v2[e];
     }
   }
 }
@@ -215,6 +234,7 @@ extern "C" int tgm_kv_append(const tgm_kv_cache* cache, const tgm_rotary* rotary
   a.H = q ? (int)q->heads : 0, a.HK = (int)cache->kv_heads, a.seen = seen ? (int)seen->dtype : -1;
   a.kf = (int)cache->k_format, a.vf = (int)cache->v_format;
   a.rot = rotary ? RotArgs{rotary->freq, rotary->gain, (int)(rotary->rotary_dim / 2)} : RotArgs{nullptr, 1.0, 0};
+  a.vec = (!q || a.q.vec) && a.k.vec && a.v.vec;
   a.start = start, a.T = (int)tokens;
   const int64_t ntok = batch * tokens;
   const int groups = ((a.H + 2 * a.HK) * (int)(cache->head_dim / 16) + 63) / 64;
