@@ -31,7 +31,8 @@ struct AttendArgs {
   int k0, kcap;        // positions k0 .. kcap - 1 are this launch's
   int chunk;           // positions per split
   int slot0, slots;    // this launch's first partial of a row, and partials per row (1: the output itself)
-  int common;          // every sequence's rows against row 0's pages
+  int common;          // attend_many: every sequence's rows against row 0's pages
+  int prefix;          // attend_few: positions below it lie in row 0's pages
   float sl;            // scale * log2(e)
   float* part;         // [row][slot][HD] sums, then [row][slot][2] maximum (log2 units) and sum of weights
   void* out;

@@ -54,11 +54,13 @@ __global__ void __launch_bounds__(256) attend_merge(const AttendArgs A, int pslo
   }
 }
 
+constexpr int64_t kAlonePairs = 196608;  // (sequence, shared position, kv head) triples that are read without sharing
 constexpr int kMaxSlots = 64;  // splits of a row: a lane each in attend_merge
 
 struct AttendPlan {
   bool many;           // a sequence's own positions by attend_many
   int chunk, splits;   // of a sequence's own positions
+  int prefix;          // positions that the batch shares, read once for all; below it but for these: own
   int pchunk, psplits; // of the common prefix
   int64_t bytes;
 };
@@ -78,19 +80,23 @@ static AttendPlan attend_plan(const tgm_kv_cache* c, int64_t dt, int64_t heads, 
   AttendPlan p{};
   const int64_t G = heads / c->kv_heads, rows = tokens * G, cap = cols * c->page_size;
   p.many = rows > attend_few_rows((int)dt);
-  const int64_t own = cap > shared ? cap - shared : 0;
-  // attend_many: as many workgroups as run at once, two a CU; attend_few: two rounds of three a CU, a split at least one
-  // block a wave
-  if (shared > 0) {
+  // A prefix that a few rows read is not worth the two launches: each sequence reads it by itself, through row 0's
+  // pages and out of the caches (8 sequences of 2300 positions, 2048 of them shared: 16 us so, 23 in common).
+  p.prefix = shared > 0 && (p.many || batch * shared * c->kv_heads > kAlonePairs) ? (int)shared : 0;
+  const int64_t own = cap > p.prefix ? cap - p.prefix : 0;
+  // attend_many: as many workgroups as run at once, two a CU
+  if (p.prefix > 0) {
     const int64_t tiles = (batch * rows + kManyRows - 1) / kManyRows * c->kv_heads;
     split_span(shared, (512 + tiles - 1) / tiles, kManyKeys, kMaxSlots / 2, p.pchunk, p.psplits);
   }
-  const int64_t most = kMaxSlots - p.psplits;
+  const int64_t most = kMaxSlots - p.psplits, heads_of_all = c->kv_heads * batch;
   if (p.many) {
-    const int64_t tiles = (rows + kManyRows - 1) / kManyRows * c->kv_heads * batch;
+    const int64_t tiles = (rows + kManyRows - 1) / kManyRows * heads_of_all;
     split_span(own, 512 / tiles, kManyKeys, most, p.chunk, p.splits);
   } else {
-    split_span(own, (1536 + c->kv_heads * batch - 1) / (c->kv_heads * batch), kFewWaves * kFewBlock, most, p.chunk, p.splits);
+    // six rounds of two workgroups a CU, a split at least one block a wave: fewer leave CUs idle at the end of ragged
+    // batches (16 sequences of up to 32700 positions: 155 us with half as many, 141 so, 145 with twice as many)
+    split_span(own, (3072 + heads_of_all - 1) / heads_of_all, kFewWaves * kFewBlock, most, p.chunk, p.splits);
   }
   const int slots = p.splits + p.psplits;
   p.bytes = slots == 1 ? 0 : batch * tokens * heads * slots * (c->head_dim + 2) * 4;
@@ -103,11 +109,11 @@ static void attend_go(const AttendPlan& p, AttendLaunch l, int shared, int cap, 
   a.slots = p.splits + p.psplits;
   if (p.psplits) {
     AttendLaunch c = l;
-    c.a.k0 = 0, c.a.kcap = shared, c.a.chunk = p.pchunk, c.a.slot0 = 0, c.a.common = 1;
+    c.a.k0 = 0, c.a.kcap = p.prefix, c.a.chunk = p.pchunk, c.a.slot0 = 0, c.a.common = 1;
     c.splits = p.psplits;
     attend_many<DT>(c, st);
   }
-  a.k0 = shared, a.kcap = cap, a.chunk = p.chunk, a.slot0 = p.psplits, a.common = 0;
+  a.k0 = p.prefix, a.kcap = cap, a.chunk = p.chunk, a.slot0 = p.psplits, a.common = 0, a.prefix = shared;
   l.splits = p.splits;
   if (p.many) attend_many<DT>(l, st);
   else attend_few<DT>(l, st);

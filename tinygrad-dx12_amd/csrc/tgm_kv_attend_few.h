@@ -42,6 +42,39 @@ __global__ void __launch_bounds__(256, 2) kv_attend_few(const AttendArgs A) {
   const int k_lo = A.k0 + z * A.chunk, k_hi = min(k_lo + A.chunk, kend);
   if (k_lo >= kend && A.slots > 1) return;  // attend_merge knows
 
+  const int32_t* trow = A.pg.table + b * A.pg.ld;
+  // positions below A.prefix lie in row 0's pages
+  auto page_of = [&](int pos) __attribute__((always_inline)) { return kv_page(A.pg, pos < A.prefix ? A.pg.table : trow, pos); };
+  struct Raw {
+    unsigned k[4][KL / 4], v[KPL][VL / 4], ksc, vsc[KPL / 4];
+    bool kok, vok;
+  };
+  auto load = [&](int base, Raw& r) __attribute__((always_inline)) {
+    const int kp = base + 4 * c, kpage = page_of(kp);
+    r.kok = kpage >= 0;
+    const int64_t kph = (int64_t)(kpage < 0 ? 0 : kpage) * A.HK + j;
+    const int kslot = kp & A.pg.mask;
+    const uint8_t* kd = A.ks.data + ((kph << A.pg.shift) + kslot) * KROW + g * KL;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at_load<KL>(kd + i * KROW, r.k[i]);
+    r.ksc = *(const unsigned*)(A.ks.scales + ((kph * (HD / kKvBlock) + g * (HD / 4) / kKvBlock) << A.pg.shift) + kslot);
+    const int vp = base + KPL * (lane / LPR), vpage = page_of(vp), ch = lane % LPR;
+    r.vok = vpage >= 0;
+    const int64_t vph = (int64_t)(vpage < 0 ? 0 : vpage) * A.HK + j;
+    const int vslot = vp & A.pg.mask;
+    const uint8_t* vd = A.vs.data + ((vph << A.pg.shift) + vslot) * VROW + ch * VL;
+#pragma unroll
+    for (int i = 0; i < KPL; ++i) at_load<VL>(vd + i * VROW, r.v[i]);
+    const uint8_t* vs = A.vs.scales + ((vph * (HD / kKvBlock) + ch / 2) << A.pg.shift) + vslot;
+#pragma unroll
+    for (int i = 0; i < KPL / 4; ++i) r.vsc[i] = *(const unsigned*)(vs + 4 * i);
+  };
+
+  const int step = kFewWaves * kFewBlock;
+  Raw cur;
+  int base = k_lo + wave * kFewBlock;
+  if (base < k_hi) load(base, cur);  // under way while q is staged
+
   // q's operands, in lane order
   for (int f = wave; f < CT * STEPS; f += kFewWaves) {
     const int ct = f / STEPS, i = f % STEPS;
@@ -63,32 +96,6 @@ __global__ void __launch_bounds__(256, 2) kv_attend_few(const AttendArgs A) {
   }
   least = len - A.T;  // row 0's
   __syncthreads();
-
-  const int32_t* trow = A.pg.table + b * A.pg.ld;
-  struct Raw {
-    unsigned k[4][KL / 4], v[KPL][VL / 4], ksc, vsc[KPL / 4];
-    bool kok, vok;
-  };
-  auto load = [&](int base, Raw& r) __attribute__((always_inline)) {
-    const int kp = base + 4 * c, kpage = kv_page(A.pg, trow, kp);
-    r.kok = kpage >= 0;
-    const int64_t kph = (int64_t)(kpage < 0 ? 0 : kpage) * A.HK + j;
-    const int kslot = kp & A.pg.mask;
-    const uint8_t* kd = A.ks.data + ((kph << A.pg.shift) + kslot) * KROW + g * KL;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) at_load<KL>(kd + i * KROW, r.k[i]);
-    r.ksc = *(const unsigned*)(A.ks.scales + ((kph * (HD / kKvBlock) + g * (HD / 4) / kKvBlock) << A.pg.shift) + kslot);
-    const int vp = base + KPL * (lane / LPR), vpage = kv_page(A.pg, trow, vp), ch = lane % LPR;
-    r.vok = vpage >= 0;
-    const int64_t vph = (int64_t)(vpage < 0 ? 0 : vpage) * A.HK + j;
-    const int vslot = vp & A.pg.mask;
-    const uint8_t* vd = A.vs.data + ((vph << A.pg.shift) + vslot) * VROW + ch * VL;
-#pragma unroll
-    for (int i = 0; i < KPL; ++i) at_load<VL>(vd + i * VROW, r.v[i]);
-    const uint8_t* vs = A.vs.scales + ((vph * (HD / kKvBlock) + ch / 2) << A.pg.shift) + vslot;
-#pragma unroll
-    for (int i = 0; i < KPL / 4; ++i) r.vsc[i] = *(const unsigned*)(vs + 4 * i);
-  };
 
   f32x4 O[CT][ND];
   float m[CT], l[CT];
@@ -113,10 +120,6 @@ __global__ void __launch_bounds__(256, 2) kv_attend_few(const AttendArgs A) {
     for (int d = 0; d < ND; ++d)
       vread[e][d] = (unsigned)(row * HD * 2 + (((2 * d + ((i16 & 3) >> 1)) ^ swz(row)) * 16) + (i16 & 1) * 8);
   }
-  const int step = kFewWaves * kFewBlock;
-  Raw cur;
-  int base = k_lo + wave * kFewBlock;
-  if (base < k_hi) load(base, cur);
 #pragma unroll 1
   for (; base < k_hi; base += step) {
     Raw nxt = cur;
