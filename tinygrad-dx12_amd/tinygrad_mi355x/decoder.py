@@ -281,7 +281,7 @@ class Decoder:
     def _down(self, rows: int, L: LayerWeights, stream: int) -> int:
         """The down projection of ``act``: into ``delta``, or as K-slice parts (returns their count)."""
         cfg = self.cfg
-        if self.down_slices > 1 and 5 <= rows <= GEMV_MAX_ROWS:
+        if self.down_slices > 1 and 5 <= rows <= self.batch:  # delta_parts holds `batch` rows a slice
             w = L.w_down
             K.call("tgm_dec_gemv_parts", w.data.data_ptr(), K.FORMAT_IDS[w.format], cfg.hidden, cfg.ffn, K.ptr(w.scales),
                    K.dtype_id(w.scales.dtype) if w.scales is not None else -1, w.block_size, self.act.data_ptr(), BF16,
