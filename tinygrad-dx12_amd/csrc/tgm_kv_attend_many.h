@@ -114,73 +114,74 @@ __global__ void __launch_bounds__(256, 2) kv_attend_many(const AttendArgs A, int
     __syncthreads();  // block kb is staged; everybody is done with block kb - 1
     const int first = k_lo + kb * kManyKeys;
     load(kb + 1, raw);  // past the last block: positions that are not seen, staged and not used
-    {
-      const unsigned char* st = lds + (kb & 1) * STAGE;
-      f32x16 S[2] = {f32x16{}, f32x16{}};
+    const unsigned char* st = lds + (kb & 1) * STAGE;
+    f32x16 S[2] = {f32x16{}, f32x16{}};
 #pragma unroll
-      for (int s = 0; s < NJ; ++s)
+    for (int s = 0; s < NJ; ++s)
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          const at_bf16x8 a = *(const at_bf16x8*)(st + (kt * 32 + l32) * ROW + (((2 * s + half) ^ swz_k(l32)) * 16));
+      for (int kt = 0; kt < 2; ++kt) {
+        const at_bf16x8 a = *(const at_bf16x8*)(st + (kt * 32 + l32) * ROW + (((2 * s + half) ^ swz_k(l32)) * 16));
 #pragma unroll
-          for (int q = 0; q < NQ; ++q) S[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qt[s][q], S[kt], 0, 0, 0);
-        }
-      const int* okg = okgroup[kb & 1];
-      const int ok0 = okg[0], ok1 = okg[1], ok2 = okg[2], ok3 = okg[3];
-      if (first + kManyKeys - 1 > wave_min || first + kManyKeys > k_hi || !(ok0 & ok1 & ok2 & ok3)) {  // uniform
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const int p = first + kt * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
-            const int ok = kt == 0 ? (v < 8 ? ok0 : ok1) : (v < 8 ? ok2 : ok3);
-            const bool gone = (p > last) | (p >= k_hi) | !ok;
-            S[kt][v] = gone ? -INFINITY : S[kt][v];
-          }
+        for (int q = 0; q < NQ; ++q) S[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qt[s][q], S[kt], 0, 0, 0);
       }
-      float bm = -INFINITY;
+    const int* okg = okgroup[kb & 1];
+    const int ok0 = okg[0], ok1 = okg[1], ok2 = okg[2], ok3 = okg[3];
+    if (first + kManyKeys - 1 > wave_min || first + kManyKeys > k_hi || !(ok0 & ok1 & ok2 & ok3)) {  // uniform
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) bm = fmaxf(bm, S[kt][v]);
-      float other = bm;
-      swap32(bm, other);  // bm: the lower half's in both halves, other: the upper half's
-      bm = fmaxf(bm, other);
-      bm *= A.sl;
-      // The reference of the exponentials moves only when a maximum has outgrown it by 2^8: weights of up to 2^8 lose
-      // nothing in fp32 and bf16, and the output is rarely rescaled.
-      if (__any(bm > m + kLazyLog2)) {
-        const float mn = fmaxf(m, bm);
-        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-        l *= alpha;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) O[d][v] *= alpha;
-        m = mn;
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float x[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][8 * u + i], A.sl, -ref));
-            l += x[i];
-          }
-          at_bf16x8 pb[NP];
-          at_split<NP>(x, pb);
-#pragma unroll
-          for (int d = 0; d < ND; ++d) {  // keys 16 u + 4 h .. + 4 of tile kt, then the ones 8 on
-            const unsigned char* row = st + voff[d] + (kt * 32 + u * 16) * ROW;
-            const at_bf16x8 a = at_tr_pair(row, row + 8 * ROW);
-#pragma unroll
-            for (int q = 0; q < NP; ++q) O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, pb[q], O[d], 0, 0, 0);
-          }
+        for (int v = 0; v < 16; ++v) {
+          const int p = first + kt * 32 + 8 * (v >> 2) + 4 * half + (v & 3);
+          const int ok = kt == 0 ? (v < 8 ? ok0 : ok1) : (v < 8 ? ok2 : ok3);
+          const bool gone = (p > last) | (p >= k_hi) | !ok;
+          S[kt][v] = gone ? -INFINITY : S[kt][v];
         }
     }
+    float b4[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      b4[i] = S[i >> 1][8 * (i & 1)];
+#pragma unroll
+      for (int v = 1; v < 8; ++v) b4[i] = fmaxf(b4[i], S[i >> 1][8 * (i & 1) + v]);
+    }
+    float bm = fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
+    float other = bm;
+    swap32(bm, other);  // bm: the lower half's in both halves, other: the upper half's
+    bm = fmaxf(bm, other);
+    bm *= A.sl;
+    // The reference of the exponentials moves only when a maximum has outgrown it by 2^8: weights of up to 2^8 lose
+    // nothing in fp32 and bf16, and the output is rarely rescaled.
+    if (__any(bm > m + kLazyLog2)) {
+      const float mn = fmaxf(m, bm);
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) O[d][v] *= alpha;
+      m = mn;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][8 * u + i], A.sl, -ref));
+        }
+        l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        at_bf16x8 pb[NP];
+        at_split<NP>(x, pb);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {  // keys 16 u + 4 h .. + 4 of tile kt, then the ones 8 on
+          const unsigned char* row = st + voff[d] + (kt * 32 + u * 16) * ROW;
+          const at_bf16x8 a = at_tr_pair(row, row + 8 * ROW);
+#pragma unroll
+          for (int q = 0; q < NP; ++q) O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, pb[q], O[d], 0, 0, 0);
+        }
+      }
     stage(kb + 1, raw);
   }
   l += __shfl_xor(l, 32, 64);

@@ -210,9 +210,7 @@ class Decoder:
         self.gu = torch.empty((rows, 2 * cfg.ffn), **f32)
         self.act = torch.empty((rows, cfg.ffn), dtype=torch.bfloat16, device=dev)
         self.logits = torch.empty((batch, cfg.vocab), **f32)
-        cache = (cfg.layers, batch, cfg.kv_heads, max_seq, cfg.head_dim)
-        self.k_cache = torch.zeros(cache, dtype=torch.bfloat16, device=dev)
-        self.v_cache = torch.zeros(cache, dtype=torch.bfloat16, device=dev)
+        self._allocate_cache()
         # decode attention: one pass or position splits (ONE_PASS_SHORT_LEN)
         self.position_splits = min(max(1, math.ceil(max_seq / 64)), 32)
         cus = torch.cuda.get_device_properties(dev).multi_processor_count
@@ -266,6 +264,12 @@ class Decoder:
         self.layer_trace: list[dict[str, torch.Tensor | None]] | None = None
 
     # ---------------------------------------------------------------- building blocks
+    def _allocate_cache(self) -> None:
+        cfg = self.cfg
+        cache = (cfg.layers, self.batch, cfg.kv_heads, self.max_seq, cfg.head_dim)
+        self.k_cache = torch.zeros(cache, dtype=torch.bfloat16, device=self.device)
+        self.v_cache = torch.zeros(cache, dtype=torch.bfloat16, device=self.device)
+
     def _add_norm(self, rows: int, parts: int, first: bool, weight: torch.Tensor, out: torch.Tensor, odt: int,
                   stream: int) -> None:
         """h += delta (or the ``parts`` down-projection parts; nothing before the first layer),
@@ -306,26 +310,7 @@ class Decoder:
             else:
                 self._add_norm(rows, parts, li == 0, L.attn_norm, self.xn16, F16, stream)
                 _packed_product(self.xn16, rows, d, L.wqkv, self.qkv, cfg.qkv_rows, stream)
-            kc, vc = self.k_cache[li], self.v_cache[li]
-            fused = seq_rows == 1 and self.fuse_rope  # one new token per sequence: RoPE + cache store in attention
-            if seq_rows > 1 and self.prompt_attention == "fused":
-                K.call("tgm_dec_rope_kv", self.qkv.data_ptr(), rows, seq_rows, cfg.heads, cfg.kv_heads, cfg.head_dim,
-                       self.pos.data_ptr(), cfg.rope_base, kc.data_ptr(), vc.data_ptr(), self.max_seq, None, None,
-                       None, 0, 1, stream)
-                K.call("tgm_dec_prefill_attention", self.qkv.data_ptr(), rows, seq_rows, cfg.heads, cfg.kv_heads,
-                       cfg.head_dim, self.pos.data_ptr(), kc.data_ptr(), vc.data_ptr(), self.max_seq,
-                       self.attn.data_ptr(), F16, stream)
-            elif seq_rows > 1 and self.prompt_attention == "gemm":
-                self._prefill_attention(rows, seq_rows, kc, vc, stream)
-            else:
-                if not fused:
-                    K.call("tgm_dec_rope_kv", self.qkv.data_ptr(), rows, seq_rows, cfg.heads, cfg.kv_heads,
-                           cfg.head_dim, self.pos.data_ptr(), cfg.rope_base, kc.data_ptr(), vc.data_ptr(),
-                           self.max_seq, None, None, None, 0, 1, stream)
-                K.call("tgm_dec_attention", self.qkv.data_ptr(), rows, seq_rows, cfg.heads, cfg.kv_heads,
-                       cfg.head_dim, self.pos.data_ptr(), kc.data_ptr(), vc.data_ptr(), self.max_seq,
-                       cfg.rope_base if fused else 0.0, splits, self.workspace.data_ptr() if splits > 1 else None,
-                       self.workspace_bytes if splits > 1 else 0, self.attn.data_ptr(), F16, stream)
+            self._attention(li, rows, seq_rows, splits, stream)
             _packed_product(self.attn, rows, cfg.heads * cfg.head_dim, L.wo, self.delta, d, stream)
             if fuse_norm:  # h_alt + delta -> h, RMSNorm and the gate|up projection with SwiGLU
                 w = L.w_gate_up
@@ -354,6 +339,30 @@ class Decoder:
             parts = self._down(rows, L, stream)
             self._trace(rows, parts=parts)
         self._add_norm(rows, parts, False, self.w.final_norm, self.xnb, BF16, stream)
+
+    def _attention(self, li: int, rows: int, seq_rows: int, splits: int, stream: int) -> None:
+        """Layer ``li``'s attention: rotary positions, the cache write, and ``attn`` from ``qkv`` and the cache."""
+        cfg = self.cfg
+        kc, vc = self.k_cache[li], self.v_cache[li]
+        fused = seq_rows == 1 and self.fuse_rope  # one new token per sequence: RoPE + cache store in attention
+        if seq_rows > 1 and self.prompt_attention == "fused":
+            K.call("tgm_dec_rope_kv", self.qkv.data_ptr(), rows, seq_rows, cfg.heads, cfg.kv_heads, cfg.head_dim,
+                   self.pos.data_ptr(), cfg.rope_base, kc.data_ptr(), vc.data_ptr(), self.max_seq, None, None,
+                   None, 0, 1, stream)
+            K.call("tgm_dec_prefill_attention", self.qkv.data_ptr(), rows, seq_rows, cfg.heads, cfg.kv_heads,
+                   cfg.head_dim, self.pos.data_ptr(), kc.data_ptr(), vc.data_ptr(), self.max_seq,
+                   self.attn.data_ptr(), F16, stream)
+        elif seq_rows > 1 and self.prompt_attention == "gemm":
+            self._prefill_attention(rows, seq_rows, kc, vc, stream)
+        else:
+            if not fused:
+                K.call("tgm_dec_rope_kv", self.qkv.data_ptr(), rows, seq_rows, cfg.heads, cfg.kv_heads,
+                       cfg.head_dim, self.pos.data_ptr(), cfg.rope_base, kc.data_ptr(), vc.data_ptr(),
+                       self.max_seq, None, None, None, 0, 1, stream)
+            K.call("tgm_dec_attention", self.qkv.data_ptr(), rows, seq_rows, cfg.heads, cfg.kv_heads,
+                   cfg.head_dim, self.pos.data_ptr(), kc.data_ptr(), vc.data_ptr(), self.max_seq,
+                   cfg.rope_base if fused else 0.0, splits, self.workspace.data_ptr() if splits > 1 else None,
+                   self.workspace_bytes if splits > 1 else 0, self.attn.data_ptr(), F16, stream)
 
     def _trace(self, rows: int, fused_norm: bool = False, parts: int = 0) -> None:
         if self.layer_trace is not None:
