@@ -87,7 +87,7 @@ static AttendPlan attend_plan(const tgm_kv_cache* c, int64_t dt, int64_t heads, 
   // attend_many: as many workgroups as run at once, two a CU
   if (p.prefix > 0) {
     const int64_t tiles = (batch * rows + kManyRows - 1) / kManyRows * c->kv_heads;
-    split_span(shared, (512 + tiles - 1) / tiles, kManyKeys, kMaxSlots / 2, p.pchunk, p.psplits);
+    split_span(shared, (512 + tiles - 1) / tiles, kManyKeys, kMaxSlots - 16, p.pchunk, p.psplits);
   }
   const int64_t most = kMaxSlots - p.psplits, heads_of_all = c->kv_heads * batch;
   if (p.many) {

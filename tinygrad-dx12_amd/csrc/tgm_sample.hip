@@ -81,10 +81,15 @@ struct SampKey {
   __device__ static constexpr int width(int level) { return DT == TGM_F32 ? (level == 2 ? 10 : 11) : 8; }
 };
 
+template <int DT>
+__device__ __forceinline__ float samp_load(const void* row, int64_t i) {
+  if constexpr (DT == TGM_F16) return (float)((const _Float16*)row)[i];
+  else return load_f32(row, DT, i);
+}
 // A logit and its key: ascending with the value, equal for equal values (-0 is +0).
 template <int DT>
 __device__ __forceinline__ float samp_value(const void* row, int64_t i) {
-  return load_f32(row, DT, i) + 0.0f;
+  return samp_load<DT>(row, i) + 0.0f;
 }
 template <int DT>
 __device__ __forceinline__ unsigned samp_key(float x) {
@@ -148,7 +153,7 @@ __device__ __forceinline__ void samp_each(const void* row, int first, int last, 
   int done = first;
   if (vec) {
     const int v1 = last / V;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = first / V + threadIdx.x; i < v1; i += THREADS) {
       const samp_u32x4 w = ((const samp_u32x4*)row)[i];
 #pragma unroll
@@ -472,8 +477,8 @@ __device__ __forceinline__ samp_u64 samp_scan(samp_u64 v, samp_u64* part, samp_u
 __device__ __forceinline__ samp_u64 samp_entry(unsigned key, int i) { return ((samp_u64)key << 32) | (unsigned)~i; }
 
 // Sorts size (a power of two from 64 to 2048) entries in LDS by 1024 threads, descending; no two entries are alike.
-// Up to 512 by counting the larger ones, several threads an entry (two barriers; 64 entries: about 0.3 us where the
-// network's 21 barriers take 2), beyond by a bitonic network.  `rank` holds `size` counters.
+// Up to 512 by counting the larger ones, several threads an entry (three barriers; 64 entries: about 0.3 us where a
+// network of 21 steps takes 2), beyond by a bitonic network whose steps within 128 entries need no barrier.  `rank` holds `size` counters.
 __device__ __forceinline__ void samp_sort(samp_u64* v, unsigned* rank, int size) {
   const int t = threadIdx.x;
   if (size <= 512) {
@@ -490,9 +495,17 @@ __device__ __forceinline__ void samp_sort(samp_u64* v, unsigned* rank, int size)
     __syncthreads();
     return;
   }
+  bool across = true;  // whether the last step, or what came before, went across waves
   for (int k = 2; k <= size; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
+      // with j below 128 a wave's 64 pairs stay within 128 entries of its own
+      if (across || j >= 128) __syncthreads();
+      else {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      }
+      across = j >= 128;
       if (t < size / 2) {
         const int a = 2 * t - (t & (j - 1)), b = a + j;
         const samp_u64 x = v[a], y = v[b];
@@ -634,9 +647,12 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   } else if (p < 1.0 && pcut.bin < cut.bin) {
     cut = pcut;
   }
-  const int mode = !(A.u[r] > 0.f) ? kSampDescend
-                                   : (cut.size <= kSampList ? kSampListAll
-                                                            : (k == 0 && cut.count <= kSampList ? kSampListBin : kSampDescend));
+  // up to 512 tokens are sorted faster than a part of the vocabulary is weighed, more of them slower
+  int mode = kSampDescend;
+  if (A.u[r] > 0.f) {
+    if (cut.size <= (k > 0 ? kSampList : 512)) mode = kSampListAll;
+    else if (k == 0 && cut.count <= kSampList) mode = kSampListBin;
+  }
   if (mode == kSampDescend) {
     sample_descend<DT>(A, u_.sh, row, r, ex);
     return;
@@ -662,12 +678,12 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   constexpr int V = DT == TGM_F32 ? 4 : 8;
   const int nv = A.vec ? n / V : 0;
   unsigned* queue = (unsigned*)li.weight;
-#pragma unroll 4
+#pragma unroll 8
   for (int i = tid; i < nv; i += kSampThreads) {
     const samp_u32x4 word = ((const samp_u32x4*)row)[i];
     float d = INFINITY;  // the smallest distance; NaN does not count
 #pragma unroll
-    for (int q = 0; q < V; ++q) d = fminf(d, fabsf(load_f32(&word, DT, q) - middle));
+    for (int q = 0; q < V; ++q) d = fminf(d, fabsf(samp_load<DT>(&word, q) - middle));
     if (d <= reach) {
       const unsigned at = atomicAdd(&queued_, 1u);
       if (at < kSampQueue) queue[at] = (unsigned)i;
