@@ -306,9 +306,12 @@ def test_attend_over_many_splits(dev, dtype, tokens):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("batch,tokens,shared,hk,group", [(3, 1, 64, 2, 4), (5, 2, 640, 1, 7), (40, 1, 320, 1, 4), (2, 9, 192, 2, 2)])
+@pytest.mark.parametrize("batch,tokens,shared,hk,group", [(3, 1, 64, 2, 4), (5, 2, 640, 1, 7), (40, 1, 320, 1, 4), (2, 9, 192, 2, 2),
+                                                             (52, 1, 1024, 4, 4), (52, 2, 1024, 4, 4)])
 def test_attend_shared_prefix(dev, dtype, batch, tokens, shared, hk, group):
-    """The prefix once for all gives what each sequence's own attention gives; some sequences end inside it."""
+    """The prefix once for all gives what each sequence's own attention gives; some sequences end inside it.  The last two
+    are large enough to be read in common by few rows each, in one launch with the sequences' own positions (8 rows of 16
+    bits) and in one of its own."""
     print(f"shared {dtype} {batch} {tokens} {shared} {hk}x{group}", flush=True)
     page, hd = 64, 128
     cols = shared // page + 3

@@ -127,9 +127,12 @@ template <int DT>
 void attend_few(const AttendLaunch& l, hipStream_t st);
 template <int DT>
 void attend_many(const AttendLaunch& l, hipStream_t st);
+template <int DT>
+void attend_both(const AttendLaunch& prefix, const AttendLaunch& own, hipStream_t st);  // rows of one tile of attend_few
 
 // Rows (tokens x heads of a group) that attend_few takes.
-constexpr int attend_few_rows(int dt) { return dt == TGM_F32 ? 10 : 16; }
+constexpr int attend_few_tile(int dt) { return dt == TGM_F32 ? 5 : 8; }  // rows of one column tile
+constexpr int attend_few_rows(int dt) { return 2 * attend_few_tile(dt); }
 constexpr int kFewBlock = 64, kFewWaves = 4;
 constexpr int kManyKeys = 64, kManyRows = 128;
 constexpr float kLazyLog2 = 8.f;

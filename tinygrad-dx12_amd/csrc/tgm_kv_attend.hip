@@ -107,16 +107,18 @@ template <int DT>
 static void attend_go(const AttendPlan& p, AttendLaunch l, int shared, int cap, hipStream_t st) {
   AttendArgs& a = l.a;
   a.slots = p.splits + p.psplits;
-  if (p.psplits) {
-    AttendLaunch c = l;
-    c.a.k0 = 0, c.a.kcap = p.prefix, c.a.chunk = p.pchunk, c.a.slot0 = 0, c.a.common = 1;
-    c.splits = p.psplits;
-    attend_many<DT>(c, st);
-  }
+  AttendLaunch c = l;
+  c.a.k0 = 0, c.a.kcap = p.prefix, c.a.chunk = p.pchunk, c.a.slot0 = 0, c.a.common = 1;
+  c.splits = p.psplits;
   a.k0 = p.prefix, a.kcap = cap, a.chunk = p.chunk, a.slot0 = p.psplits, a.common = 0, a.prefix = shared;
   l.splits = p.splits;
-  if (p.many) attend_many<DT>(l, st);
-  else attend_few<DT>(l, st);
+  if (p.psplits && a.T * a.G <= attend_few_tile(DT)) {
+    attend_both<DT>(c, l, st);
+  } else {
+    if (p.psplits) attend_many<DT>(c, st);
+    if (p.many) attend_many<DT>(l, st);
+    else attend_few<DT>(l, st);
+  }
   if (a.slots > 1) {
     const dim3 grid((unsigned)(((int64_t)a.B * a.T * a.H + 3) / 4));
     if (l.hd == 64) hipLaunchKernelGGL((attend_merge<DT, 64>), grid, dim3(256), 0, st, a, p.psplits);

@@ -20,22 +20,31 @@
 
 namespace tgm {
 
+// Sizes of the workgroup's LDS: q's operands, each wave's staged values (or its part of the output), each wave's maxima
+// and sums.
+template <int DT, int HD, int CT>
+struct FewLds {
+  static constexpr int VALUES = 32 * HD * 2, PART = 16 * (HD + 4) * 4;
+  static constexpr int WAVE = VALUES > PART ? VALUES : PART;
+  static constexpr int Q = CT * (HD / 32) * AttendTerms<DT>::Q * 1024;
+  static constexpr int BYTES = Q + kFewWaves * WAVE + 2 * kFewWaves * 16 * CT * 4;
+};
+
+// Split z of kv head j of sequence b.
 template <int DT, int KB, int VB, int HD, int CT>
-__global__ void __launch_bounds__(256, 2) kv_attend_few(const AttendArgs A) {
+__device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds, int z, int j, int b) {
   constexpr int NQ = AttendTerms<DT>::Q, NP = AttendTerms<DT>::P, RP = 16 / NP;
   constexpr int STEPS = HD / 32, ND = HD / 16;
   constexpr int KROW = HD * KB / 8, VROW = HD * VB / 8;
   constexpr int KL = KROW / 4, VL = VROW * 16 / HD;  // bytes a lane loads of a key and of a value row
   constexpr int LPR = HD / 16, KPL = 64 * LPR / 64;  // lanes per value row; value rows per lane and block
-  constexpr int VLDS = 32 * HD * 2;
-  constexpr int RED = 16 * (HD + 4) * 4;
-  constexpr int WLDS = VLDS > RED ? VLDS : RED;
-  __shared__ __attribute__((aligned(16))) unsigned char qlds[CT * STEPS * NQ * 1024];
-  __shared__ __attribute__((aligned(16))) unsigned char wlds[kFewWaves * WLDS];
-  __shared__ float sm[kFewWaves][16 * CT], ss[kFewWaves][16 * CT];
+  constexpr int WLDS = FewLds<DT, HD, CT>::WAVE;
+  unsigned char* qlds = lds;
+  unsigned char* wlds = lds + FewLds<DT, HD, CT>::Q;
+  float(*sm)[16 * CT] = (float(*)[16 * CT])(wlds + kFewWaves * WLDS);
+  float(*ss)[16 * CT] = sm + kFewWaves;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int z = blockIdx.x, j = blockIdx.y, b = blockIdx.z;
   const int rows = A.T * A.G;
   const int len = at_length(A, b);
   const int kend = min(len, A.kcap);
@@ -299,6 +308,12 @@ __global__ void __launch_bounds__(256, 2) kv_attend_few(const AttendArgs A) {
     }
     __syncthreads();
   }
+}
+
+template <int DT, int KB, int VB, int HD, int CT>
+__global__ void __launch_bounds__(256, 2) kv_attend_few(const AttendArgs A) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[FewLds<DT, HD, CT>::BYTES];
+  few_body<DT, KB, VB, HD, CT>(A, lds, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 template <int DT, int KB, int VB, int HD>

@@ -17,24 +17,30 @@
 
 namespace tgm {
 
+// LDS: two stages of keys and values, and whether the pages of a stage's four groups of 16 positions exist.
+template <int HD>
+struct ManyLds {
+  static constexpr int STAGES = 4 * kManyKeys * HD * 2, BYTES = STAGES + 2 * 4 * 4;
+};
+
+// Workgroup `at` of the row tiles and splits of kv head j; sequence b where the positions are not common.
 template <int DT, int KB, int VB, int HD>
-__global__ void __launch_bounds__(256, 2) kv_attend_many(const AttendArgs A, int tiles) {
+__device__ __forceinline__ void many_body(const AttendArgs& A, unsigned char* lds, int tiles, int at, int j, int seq) {
   constexpr int NQ = AttendTerms<DT>::Q, NP = AttendTerms<DT>::P;
   constexpr int NJ = HD / 16, ND = HD / 32;
   constexpr int ROW = HD * 2, CH = ROW / 16;
   constexpr int BLOCK = kManyKeys * ROW, STAGE = 2 * BLOCK;
   constexpr int KROW = HD * KB / 8, VROW = HD * VB / 8, KL = KROW / 4, VL = VROW / 4;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * STAGE];
-  __shared__ int okgroup[2][4];  // whether the pages of a block's four groups of 16 positions exist
+  int(*okgroup)[4] = (int(*)[4])(lds + ManyLds<HD>::STAGES);
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int z = blockIdx.x / tiles, tile = tiles - 1 - (int)(blockIdx.x % tiles);  // the longest rows first
-  const int j = blockIdx.y, TG = A.T * A.G;
+  const int z = at / tiles, tile = tiles - 1 - at % tiles;  // the longest rows first
+  const int TG = A.T * A.G;
   const int nrows = A.common ? A.B * TG : TG;
   const int r0 = tile * kManyRows + wave * 32;
   const int r = min(r0 + l32, nrows - 1);
   const bool rvalid = r0 + l32 < nrows;
-  const int b = A.common ? r / TG : (int)blockIdx.z;
+  const int b = A.common ? r / TG : seq;
   const int rt = r - (A.common ? b * TG : 0), t = rt / A.G, h = j * A.G + rt % A.G;
   const int last = min(at_length(A, b), A.kcap + A.T) - A.T + t;  // the last position this row sees
   // positions any row of the workgroup sees
@@ -211,6 +217,12 @@ __global__ void __launch_bounds__(256, 2) kv_attend_many(const AttendArgs A, int
       ml[1] = l;
     }
   }
+}
+
+template <int DT, int KB, int VB, int HD>
+__global__ void __launch_bounds__(256, 2) kv_attend_many(const AttendArgs A, int tiles) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[ManyLds<HD>::BYTES];
+  many_body<DT, KB, VB, HD>(A, lds, tiles, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 template <int DT, int KB, int VB, int HD>
