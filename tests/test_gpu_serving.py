@@ -371,6 +371,19 @@ def test_attend_views_scale_and_out(dev):
     assert torch.equal(c.attend(q, wide[:, :5], lengths), c.attend(q, wide[:, :5].contiguous(), lengths))
 
 
+def test_empty_calls(dev):
+    c, rot = make_cache(dev, 4, 2, 64, 64, "fp8_e4m3", "fp8_e4m3", seed=1), Rotary(64, device=dev)
+    none, table = i32(dev, []), torch.zeros((0, 2), dtype=torch.int32, device=dev)
+    x, y = torch.zeros((0, 3, 2, 64), device=dev), torch.zeros((2, 0, 2, 64), device=dev)
+    start, rows = i32(dev, [0, 0]), i32(dev, [[0, 1], [2, 3]])
+    assert rot.rotate(x, none).shape == x.shape and rot.rotate(y, start).shape == y.shape
+    assert c.append(x, x, table, none, rotary=rot, q=x, seen=F32).k.shape == x.shape
+    assert c.append(y, y, rows, start, rotary=rot, q=y, seen=F32).q.shape == y.shape
+    assert c.attend(x, table, none).shape == x.shape and c.attend(y, rows, start).shape == y.shape
+    assert c.read(table, none, 5)[0].shape == (0, 5, 2, 64)
+    assert sample(torch.zeros((0, 9), device=dev), torch.zeros(0, device=dev)).shape == (0,)
+
+
 def test_large_scores_and_flat_ones(dev):
     """One position takes all the weight; and all weigh the same."""
     for factor in (60.0, 0.0):
@@ -468,6 +481,29 @@ def test_sample_draws_with_the_right_frequencies(dev):
     freq = np.bincount(got.cpu().numpy(), minlength=n) / draws
     want = torch.softmax(row.double(), 0).numpy()
     assert np.abs(freq - want).max() <= 1.0 / draws + 1e-6  # evenly spaced u: each interval holds its share to one draw
+
+
+def test_sample_long_lists_and_many_rows(dev):
+    """Lists of every length class, cuts among more equal logits than a list holds, u = 0, and more rows than a slab."""
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(3, 40000, generator=g)
+    x[1] = torch.randint(0, 5, (40000,), generator=g).float()
+    x[2] = 1.0
+    for k, p in ((300, 1.0), (600, 0.9), (1500, 0.99), (2048, 1.0), (5000, 0.97), (0, 0.02), (0, 0.1), (0, 0.6), (39999, 0.5)):
+        print(f"sample lists {k} {p}", flush=True)
+        for u in (torch.rand(3, generator=g), torch.zeros(3)):
+            check_sample(dev, x, u, 1.0, k, p, 0.0)
+    rows = 2048 * 2 + 77
+    logits = torch.randn(rows, 130, generator=g)
+    check_sample(dev, logits, torch.rand(rows, generator=g), 0.8, 20, 0.9, 0.01)
+
+
+def test_a_whole_vocabulary_of_2_to_the_20(dev):
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(2, 1 << 20, generator=g) * 2
+    for dtype in (F32, BF16):
+        for k, p, t in ((0, 0.9, 1.0), (50, 0.95, 0.7), (0, 1.0, 1.0), (4000, 1.0, 1.0)):
+            check_sample(dev, x.to(dtype), torch.rand(2, generator=g), t, k, p, 0.0)
 
 
 # ----------------------------------------------------------------------------- streams and graphs

@@ -38,7 +38,7 @@ constexpr double kSampPerBin = 40.0;  // bins per power of two of a weight: 2047
 struct SampleArgs {
   const void* logits;
   int64_t ld;
-  int n, fbits, vec;
+  int n, fbits;
   int chunks, chunk;  // workgroups of a row in sample_bins, tokens of each
   int rows;
   const float* u;
@@ -146,22 +146,31 @@ struct SampExp {
   }
 };
 
-// f(value, index) over tokens first .. last - 1 of a row, in no order (first a multiple of 8).
+// The first token of a row whose address is a multiple of 16.
+template <int DT>
+__device__ __forceinline__ int samp_aligned(const void* row) {
+  return (int)((16u - ((unsigned)(uintptr_t)row & 15u)) & 15u) / (DT == TGM_F32 ? 4 : 2);
+}
+
+// f(value, index) over tokens first .. last - 1 of a row, in no order: whole 16-byte vectors where they are aligned, the
+// few tokens before and behind one by one.
 template <int DT, int THREADS, typename F>
-__device__ __forceinline__ void samp_each(const void* row, int first, int last, int vec, F f) {
+__device__ __forceinline__ void samp_each(const void* row, int first, int last, F f) {
   constexpr int V = DT == TGM_F32 ? 4 : 8;
-  int done = first;
-  if (vec) {
-    const int v1 = last / V;
+  const int al = samp_aligned<DT>(row);
+  const int begin = first <= al ? al : first + (V - 1) - (first - al + V - 1) % V;  // first + 0 .. V - 1
+  const int vectors = last > begin ? (last - begin) / V : 0;
+  const samp_u32x4* v = (const samp_u32x4*)((const char*)row + (int64_t)begin * (16 / V));
 #pragma unroll 8
-    for (int i = first / V + threadIdx.x; i < v1; i += THREADS) {
-      const samp_u32x4 w = ((const samp_u32x4*)row)[i];
+  for (int i = threadIdx.x; i < vectors; i += THREADS) {
+    const samp_u32x4 w = v[i];
 #pragma unroll
-      for (int e = 0; e < V; ++e) f(samp_value<DT>(&w, e), i * V + e);
-    }
-    if (v1 * V > done) done = v1 * V;
+    for (int e = 0; e < V; ++e) f(samp_value<DT>(&w, e), begin + i * V + e);
   }
-  for (int i = done + threadIdx.x; i < last; i += THREADS) f(samp_value<DT>(row, i), i);
+  const int head = min(begin, last) - first;  // under V
+  if ((int)threadIdx.x < head) f(samp_value<DT>(row, first + threadIdx.x), first + (int)threadIdx.x);
+  const int tail = begin + vectors * V + (int)threadIdx.x;
+  if (tail < last && begin < last) f(samp_value<DT>(row, tail), tail);
 }
 
 // Inclusive prefix sum over the wave by DPP moves alone: shifts within rows of 16, then the rows' totals.
@@ -264,7 +273,7 @@ __device__ void sample_descend(const SampleArgs& A, SampShared& sh, const void* 
         sh.count[i] = 0;
       }
       __syncthreads();
-      samp_each<DT, kSampThreads>(row, 0, n, A.vec, [&](float x, int) {
+      samp_each<DT, kSampThreads>(row, 0, n, [&](float x, int) {
         if (!(x > -INFINITY)) return;
         const unsigned k = samp_key<DT>(x);
         if (level > 0 && (k >> (sft + width)) != prefix) return;
@@ -404,9 +413,9 @@ __device__ void sample_descend(const SampleArgs& A, SampShared& sh, const void* 
 
 // The row's largest logit (-inf: none), in every thread.
 template <int DT, int THREADS>
-__device__ __forceinline__ float samp_max(const void* row, int n, int vec, float* part) {
+__device__ __forceinline__ float samp_max(const void* row, int n, float* part) {
   float best = -INFINITY;
-  samp_each<DT, THREADS>(row, 0, n, vec, [&](float x, int) { best = fmaxf(best, x); });  // NaN: the other operand
+  samp_each<DT, THREADS>(row, 0, n, [&](float x, int) { best = fmaxf(best, x); });  // NaN: the other operand
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor(best, o, 64));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = best;
@@ -438,12 +447,12 @@ __global__ void __launch_bounds__(kBinThreads) sample_bins(const SampleArgs A) {
     mass[i] = 0;
     count[i] = 0;
   }
-  const float best = samp_max<DT, kBinThreads>(row, A.n, A.vec, part);
+  const float best = samp_max<DT, kBinThreads>(row, A.n, part);
   if (c == 0 && tid == 0) A.max[r] = best;
   const float temp = A.temperature[r];
   if (!(temp > 0.f) || !(best > -INFINITY)) return;
   const SampExp ex(table, best, temp, A.fbits);
-  samp_each<DT, kBinThreads>(row, min(c * A.chunk, A.n), min((c + 1) * A.chunk, A.n), A.vec, [&](float x, int) {
+  samp_each<DT, kBinThreads>(row, min(c * A.chunk, A.n), min((c + 1) * A.chunk, A.n), [&](float x, int) {
     if (!(x > -INFINITY)) return;
     const double y = ex.log2w(x);
     const int b = ex.bin(y);
@@ -554,7 +563,7 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   }
   if (!(temp > 0.f)) {  // the first maximum
     int at = n;
-    samp_each<DT, kSampThreads>(row, 0, n, A.vec, [&](float x, int i) {
+    samp_each<DT, kSampThreads>(row, 0, n, [&](float x, int i) {
       if (x == best && i < at) at = i;
     });
 #pragma unroll
@@ -676,11 +685,12 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   // Whole 16-byte vectors first: the few that may hold such a token are queued, and looked into by as many threads
   // afterwards (a test and a branch for each token of the row cost three times as much).
   constexpr int V = DT == TGM_F32 ? 4 : 8;
-  const int nv = A.vec ? n / V : 0;
+  const int al = min(samp_aligned<DT>(row), n), nv = (n - al) / V;
+  const samp_u32x4* vectors = (const samp_u32x4*)(row + (int64_t)al * (16 / V));
   unsigned* queue = (unsigned*)li.weight;
 #pragma unroll 8
   for (int i = tid; i < nv; i += kSampThreads) {
-    const samp_u32x4 word = ((const samp_u32x4*)row)[i];
+    const samp_u32x4 word = vectors[i];
     float d = INFINITY;  // the smallest distance; NaN does not count
 #pragma unroll
     for (int q = 0; q < V; ++q) d = fminf(d, fabsf(samp_load<DT>(&word, q) - middle));
@@ -693,13 +703,14 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   const int queued = (int)queued_;
   if (queued <= kSampQueue) {
     for (int j = tid; j < queued * V; j += kSampThreads) {
-      const int i = (int)queue[j / V] * V + j % V;
+      const int i = al + (int)queue[j / V] * V + j % V;
       consider(samp_value<DT>(row, i), i);
     }
   } else {
-    for (int i = tid; i < nv * V; i += kSampThreads) consider(samp_value<DT>(row, i), i);
+    for (int i = tid; i < nv * V; i += kSampThreads) consider(samp_value<DT>(row, al + i), al + i);
   }
-  for (int i = nv * V + tid; i < n; i += kSampThreads) consider(samp_value<DT>(row, i), i);
+  if (tid < al) consider(samp_value<DT>(row, tid), tid);
+  if (al + nv * V + tid < n) consider(samp_value<DT>(row, al + nv * V + tid), al + nv * V + tid);
   if (mode == kSampListBin && wave < A.chunks) {  // kept mass of each part of the vocabulary, but for the cut's bin
     const samp_u64* part_mass = A.mass + (r * A.chunks + wave) * kSampBins;
     samp_u64 s = 0;
@@ -786,21 +797,23 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   int ch = 0;
   while (ch < A.chunks - 1 && left >= chunk_mass[ch]) left -= chunk_mass[ch++];
   const int end = min((ch + 1) * A.chunk, n);
-  for (int first = ch * A.chunk; first < end; first += 8 * kSampThreads) {  // 8 neighbours a thread
+  const int begin = ch * A.chunk;
+  // 8 neighbours a thread, from an aligned token at or before the part's first
+  for (int first = begin - ((begin - al) & 7); first < end; first += 8 * kSampThreads) {
     samp_u64 x[8], s = 0;
     float v[8];
     const int i0 = first + 8 * tid;
-    if (A.vec && i0 + 8 <= end) {
-      constexpr int W = DT == TGM_F32 ? 2 : 1, V = 8 / W;
+    if (i0 >= begin && i0 + 8 <= end) {
+      constexpr int W = 8 / V;
 #pragma unroll
       for (int h = 0; h < W; ++h) {
-        const samp_u32x4 word = ((const samp_u32x4*)row)[i0 / V + h];
+        const samp_u32x4 word = *(const samp_u32x4*)(row + (int64_t)(i0 + h * V) * (16 / V));
 #pragma unroll
         for (int q = 0; q < V; ++q) v[h * V + q] = samp_value<DT>(&word, q);
       }
     } else {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = i0 + q < end ? samp_value<DT>(row, i0 + q) : -INFINITY;
+      for (int q = 0; q < 8; ++q) v[q] = i0 + q >= begin && i0 + q < end ? samp_value<DT>(row, i0 + q) : -INFINITY;
     }
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -831,8 +844,12 @@ struct SampSizes {
   int64_t mass, count, max, bytes;
 };
 
+// Rows go in slabs, one after the other over one workspace (24 KB a part of a row).
+constexpr int64_t kSampSlab = 2048;
+
 static SampSizes samp_sizes(int64_t rows, int64_t vocab) {
   SampSizes z;
+  if (rows > kSampSlab) rows = kSampSlab;
   // two workgroups a CU, 4096 tokens each at least: every part adds 24 KB to what sample_draw reads
   int64_t c = (512 + rows - 1) / rows;
   const int64_t most = (vocab + 4095) / 4096;
@@ -855,9 +872,18 @@ static SampSizes samp_sizes(int64_t rows, int64_t vocab) {
 
 template <int DT>
 static void sample_launch(const SampleArgs& a, int64_t rows, hipStream_t st) {
-  const unsigned eights = (unsigned)((rows + 7) / 8);
-  hipLaunchKernelGGL(sample_bins<DT>, dim3(8 * eights * (unsigned)a.chunks), dim3(kBinThreads), 0, st, a);
-  hipLaunchKernelGGL(sample_draw<DT>, dim3((unsigned)rows), dim3(kSampThreads), 0, st, a);
+  for (int64_t r0 = 0; r0 < rows; r0 += kSampSlab) {
+    SampleArgs b = a;
+    b.rows = (int)(rows - r0 < kSampSlab ? rows - r0 : kSampSlab);
+    b.logits = (const char*)a.logits + r0 * a.ld * (DT == TGM_F32 ? 4 : 2);
+    b.u += r0, b.temperature += r0, b.tokens += r0;
+    if (b.top_k) b.top_k += r0;
+    if (b.top_p) b.top_p += r0;
+    if (b.min_p) b.min_p += r0;
+    const unsigned eights = (unsigned)((b.rows + 7) / 8);
+    hipLaunchKernelGGL(sample_bins<DT>, dim3(8 * eights * (unsigned)b.chunks), dim3(kBinThreads), 0, st, b);
+    hipLaunchKernelGGL(sample_draw<DT>, dim3((unsigned)b.rows), dim3(kSampThreads), 0, st, b);
+  }
 }
 
 }  // namespace tgm
@@ -883,11 +909,10 @@ extern "C" int tgm_sample(const void* logits, int64_t dtype, int64_t rows, int64
   TGM_CHECK_ARG(workspace && workspace_bytes >= z.bytes && ((uintptr_t)workspace & 15) == 0, "workspace too small or misaligned");
   SampleArgs a;
   a.logits = logits, a.ld = ld, a.n = (int)vocab;
-  a.chunks = z.chunks, a.chunk = z.chunk, a.rows = (int)rows;
+  a.chunks = z.chunks, a.chunk = z.chunk, a.rows = 0;
   int lg = 0;
   while ((1ll << lg) < vocab) ++lg;
   a.fbits = 62 - lg > 50 ? 50 : 62 - lg;
-  a.vec = ((uintptr_t)logits & 15) == 0 && (rows == 1 || (ld * dtype_size((int)dtype)) % 16 == 0);
   a.u = u, a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p, a.tokens = tokens;
   char* ws = (char*)workspace;
   a.mass = (samp_u64*)(ws + z.mass), a.count = (unsigned*)(ws + z.count), a.max = (float*)(ws + z.max);

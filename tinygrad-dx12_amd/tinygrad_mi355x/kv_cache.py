@@ -12,6 +12,9 @@ past what a sequence uses may hold anything (the kernels check every page number
 * ``read`` gives positions back in a floating type;
 * ``attend`` is grouped-query attention of the newest tokens over everything cached, a few tokens (decode) or a chunk
   of a prompt, with or without a prefix that the whole batch shares.
+
+Results and workspaces come from torch's caching allocator: to replay calls as a graph, capture them with
+``torch.cuda.graph``, which keeps their memory in a pool of its own.
 """
 
 from __future__ import annotations
@@ -106,8 +109,10 @@ class PackedKVCache:
         if seen is not None:
             k_out, v_out = k.new_empty(k.shape, dtype=seen), k.new_empty(k.shape, dtype=seen)
             ko_ptr, vo_ptr = k_out.data_ptr(), v_out.data_ptr()
-        K.call("tgm_kv_append", self._arg, rot_arg, q_arg, q_ptr, qo_arg, qo_ptr, k_arg, k.data_ptr(), v_arg, v.data_ptr(),
-               seen_arg, ko_ptr, vo_ptr, table.data_ptr(), ld, cols, start.data_ptr(), batch, tokens, K.stream_on(index))
+        if batch and tokens:
+            K.call("tgm_kv_append", self._arg, rot_arg, q_arg, q_ptr, qo_arg, qo_ptr, k_arg, k.data_ptr(), v_arg,
+                   v.data_ptr(), seen_arg, ko_ptr, vo_ptr, table.data_ptr(), ld, cols, start.data_ptr(), batch, tokens,
+                   K.stream_on(index))
         return Appended(q_out, k_out, v_out)
 
     def _append_plan(self, sig, k, v, table, start, rotary, q, seen) -> tuple:
@@ -154,6 +159,8 @@ class PackedKVCache:
         K.require_device(self.k_data)
         shape = (batch, count, self.kv_heads, self.head_dim)
         k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        if not batch or not count:
+            return k, v
         K.call("tgm_kv_read", self._arg, table.data_ptr(), *self._table_args(table), first.data_ptr(), batch, count, k.data_ptr(),
                v.data_ptr(), _DT[dtype], K.stream_of(table))
         return k, v
@@ -185,8 +192,9 @@ class PackedKVCache:
             out = q.new_empty(q.shape)
         # the workspace is of the caching allocator, so that calls on several streams never share one
         workspace = q.new_empty(need, dtype=torch.uint8).data_ptr() if need else None
-        K.call("tgm_kv_attend", self._arg, q_arg, q.data_ptr(), table.data_ptr(), ld, cols, lengths.data_ptr(), batch, tokens,
-               shared, scale, workspace, need, out.data_ptr(), K.stream_on(index))
+        if batch and tokens:
+            K.call("tgm_kv_attend", self._arg, q_arg, q.data_ptr(), table.data_ptr(), ld, cols, lengths.data_ptr(), batch,
+                   tokens, shared, scale, workspace, need, out.data_ptr(), K.stream_on(index))
         return out
 
     def _attend_plan(self, sig, q, table, lengths, shared) -> tuple:

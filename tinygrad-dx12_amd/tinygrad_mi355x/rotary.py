@@ -146,8 +146,9 @@ class Rotary:
             if out.shape != shape or out.dtype is not x.dtype or out.device != x.device:
                 raise ValueError("out must be like x")
             out_arg = heads_arg(out)
-        K.call("tgm_rotate", self.arg, x_arg, x.data_ptr(), out_arg, out.data_ptr(), start.data_ptr(), batch, tokens,
-               self.head_dim, K.stream_on(index))
+        if batch and tokens:
+            K.call("tgm_rotate", self.arg, x_arg, x.data_ptr(), out_arg, out.data_ptr(), start.data_ptr(), batch, tokens,
+                   self.head_dim, K.stream_on(index))
         return out
 
     def _plan(self, sig, x: torch.Tensor, start: torch.Tensor) -> tuple:
