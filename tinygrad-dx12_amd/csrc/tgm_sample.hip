@@ -486,11 +486,12 @@ __device__ __forceinline__ samp_u64 samp_scan(samp_u64 v, samp_u64* part, samp_u
 __device__ __forceinline__ samp_u64 samp_entry(unsigned key, int i) { return ((samp_u64)key << 32) | (unsigned)~i; }
 
 // Sorts size (a power of two from 64 to 2048) entries in LDS by 1024 threads, descending; no two entries are alike.
-// Up to 512 by counting the larger ones, several threads an entry (three barriers; 64 entries: about 0.3 us where a
-// network of 21 steps takes 2), beyond by a bitonic network whose steps within 128 entries need no barrier.  `rank` holds `size` counters.
+// Up to 256 by counting the larger ones, several threads an entry, three barriers in all (64 entries take about 0.3 us
+// where a network of 21 steps takes 2; 512 take 8, and by the network 4), beyond by a bitonic network whose steps within
+// 128 entries need no barrier.  `rank` holds 256 counters.
 __device__ __forceinline__ void samp_sort(samp_u64* v, unsigned* rank, int size) {
   const int t = threadIdx.x;
-  if (size <= 512) {
+  if (size <= 256) {
     const int i = t & (size - 1), share = size * size / kSampThreads, j0 = (t / size) * share;
     if (t < size) rank[t] = 0;
     __syncthreads();
@@ -529,7 +530,7 @@ __device__ __forceinline__ void samp_sort(samp_u64* v, unsigned* rank, int size)
 
 struct SampList {
   samp_u64 entry[kSampList], weight[kSampList];
-  unsigned rank[512];
+  unsigned rank[256];
 };
 // What sample_draw goes by: the cut's bin, and whether everything down to it is listed or that bin alone.
 enum SampMode { kSampListAll = 0, kSampListBin = 1, kSampDescend = 2 };
