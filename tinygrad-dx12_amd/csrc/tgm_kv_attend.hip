@@ -3,6 +3,8 @@
 
 namespace tgm {
 
+// Bound by the partial sums' bytes: 8.8 us for 16384 rows of four splits (34 MB, out of the caches).
+//
 // One wave per row: weights of its splits (lane s: slot s), then their weighted sum, four dims a lane and the wave's
 // halves (quarters for 64 dims) on slots of their own, several loads in flight.  Slots of the common prefix (below
 // `pslots`) are always written, those of a sequence's own positions as far as it reaches.
@@ -80,9 +82,12 @@ static AttendPlan attend_plan(const tgm_kv_cache* c, int64_t dt, int64_t heads, 
   AttendPlan p{};
   const int64_t G = heads / c->kv_heads, rows = tokens * G, cap = cols * c->page_size;
   p.many = rows > attend_few_rows((int)dt);
-  // A prefix that a few rows read is not worth the two launches: each sequence reads it by itself, through row 0's
-  // pages and out of the caches (8 sequences of 2300 positions, 2048 of them shared: 16 us so, 23 in common).
-  p.prefix = shared > 0 && (p.many || batch * shared * c->kv_heads > kAlonePairs) ? (int)shared : 0;
+  // A prefix that a few rows read goes with each sequence, through row 0's pages and out of the caches: the products over
+  // 128 rows at a time, most of them empty, take longer.  In common and so, us, fp8: 8 sequences on 2048 positions of 8
+  // heads 17 and 17 (bf16), 16 of them 19 and 23, 32 of them 21 and 34; f32, whose rows split into three terms, 16 of them
+  // 26 and 25, 32 of them 29 and 38.
+  const int64_t alone = dt == TGM_F32 ? 2 * kAlonePairs : kAlonePairs;
+  p.prefix = shared > 0 && (p.many || batch * shared * c->kv_heads > alone) ? (int)shared : 0;
   const int64_t own = cap > p.prefix ? cap - p.prefix : 0;
   // attend_many: as many workgroups as run at once, two a CU
   if (p.prefix > 0) {
@@ -96,7 +101,7 @@ static AttendPlan attend_plan(const tgm_kv_cache* c, int64_t dt, int64_t heads, 
   } else {
     // six rounds of two workgroups a CU, a split at least one block a wave: fewer leave CUs idle at the end of ragged
     // batches (16 sequences of up to 32700 positions: 155 us with half as many, 141 so, 145 with twice as many)
-    split_span(own, (3072 + heads_of_all - 1) / heads_of_all, kFewWaves * kFewBlock, most, p.chunk, p.splits);
+    split_span(own, (6 * 512 + heads_of_all - 1) / heads_of_all, kFewWaves * kFewBlock, most, p.chunk, p.splits);
   }
   const int slots = p.splits + p.psplits;
   p.bytes = slots == 1 ? 0 : batch * tokens * heads * slots * (c->head_dim + 2) * 4;

