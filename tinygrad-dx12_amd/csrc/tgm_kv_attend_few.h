@@ -15,10 +15,12 @@
 // column c in lane group g are then keys 16 g + 4 v + i, and the products with V take the keys with i = 0, 1 and then
 // those with i = 2, 3: V goes through LDS in these two halves.
 //
-// Bound by memory: 16 sequences of up to 32700 positions, 32 query and 8 kv heads of 128, fp8 (640 MB) take 136 us, 4.7
-// TB/s (140 with the join; a copy reaches 5.1), the vector instructions busy for a quarter of it and the matrix pipe for
-// 6 %.  Each wave keeps the next block of 64 positions (16 KB) under way in registers, which is what limits it to two
-// waves per SIMD.  Short ones are a chain of latencies: 1000 positions of one sequence take 8 us, and the join 3.
+// Bound by memory: 16 sequences of up to 32700 positions, 32 query and 8 kv heads of 128, fp8 (640 MB) take 129 us with
+// the join, 4.95 TB/s (a copy reaches 5.1), the vector instructions busy for a quarter of it and the matrix pipe for 6 %.
+// What keeps the memory busy is waves: three per SIMD that load a block of 64 positions (16 KB) and compute it beat two
+// that hold the next block in registers (140), and four, which spill (220).  f32 queries stay at two (16 x 16000 positions:
+// 118 us, at three, spilling, 122).  Short ones are a chain of latencies: 1000 positions of one sequence take 8 us, and
+// the join 3.
 #pragma once
 
 #include "tgm_kv_attend.h"
@@ -44,7 +46,6 @@ __device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds
   constexpr int KL = KROW / 4, VL = VROW * 16 / HD;  // bytes a lane loads of a key and of a value row
   constexpr int LPR = HD / 16, KPL = 64 * LPR / 64;  // lanes per value row; value rows per lane and block
   constexpr int WLDS = FewLds<DT, HD, CT>::WAVE;
-  constexpr bool AHEAD = CT == 1;  // the next block's loads under way: two column tiles have no registers for it
   unsigned char* qlds = lds;
   unsigned char* wlds = lds + FewLds<DT, HD, CT>::Q;
   float(*sm)[16 * CT] = (float(*)[16 * CT])(wlds + kFewWaves * WLDS);
@@ -84,11 +85,6 @@ __device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds
 #pragma unroll
     for (int i = 0; i < KPL / 4; ++i) r.vsc[i] = *(const unsigned*)(vs + 4 * i);
   };
-
-  const int step = kFewWaves * kFewBlock;
-  Raw cur;
-  int base = k_lo + wave * kFewBlock;
-  if (AHEAD && base < k_hi) load(base, cur);  // under way while q is staged
 
   // q's operands, in lane order
   for (int f = wave; f < CT * STEPS; f += kFewWaves) {
@@ -136,10 +132,9 @@ __device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds
       vread[e][d] = (unsigned)(row * HD * 2 + (((2 * d + ((i16 & 3) >> 1)) ^ swz(row)) * 16) + (i16 & 1) * 8);
   }
 #pragma unroll 1
-  for (; base < k_hi; base += step) {
-    Raw nxt;
-    if (!AHEAD) load(base, cur);
-    else if (base + step < k_hi) load(base + step, nxt);
+  for (int base = k_lo + wave * kFewBlock; base < k_hi; base += kFewWaves * kFewBlock) {
+    Raw cur;
+    load(base, cur);
     const unsigned long long kok = __ballot(cur.kok);
     const bool whole = base + kFewBlock <= k_hi && __all(cur.kok);  // every position exists (uniform)
     if (!whole) {
@@ -260,7 +255,6 @@ __device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
-    if (AHEAD) cur = nxt;
   }
 
   // the four waves' parts of each row, summed in their order
@@ -318,7 +312,7 @@ __device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds
 }
 
 template <int DT, int KB, int VB, int HD, int CT>
-__global__ void __launch_bounds__(256, 2) kv_attend_few(const AttendArgs A) {
+__global__ void __launch_bounds__(256, CT == 1 && DT != TGM_F32 ? 3 : 2) kv_attend_few(const AttendArgs A) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[FewLds<DT, HD, CT>::BYTES];
   few_body<DT, KB, VB, HD, CT>(A, lds, blockIdx.x, blockIdx.y, blockIdx.z);
 }
