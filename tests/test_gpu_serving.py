@@ -307,11 +307,12 @@ def test_attend_over_many_splits(dev, dtype, tokens):
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("batch,tokens,shared,hk,group", [(3, 1, 64, 2, 4), (5, 2, 640, 1, 7), (40, 1, 320, 1, 4), (2, 9, 192, 2, 2),
-                                                             (52, 1, 1024, 4, 4), (52, 2, 1024, 4, 4)])
+                                                             (52, 2, 1024, 4, 4), (100, 1, 1024, 4, 2),
+                                                             (100, 3, 1024, 4, 2)])
 def test_attend_shared_prefix(dev, dtype, batch, tokens, shared, hk, group):
-    """The prefix once for all gives what each sequence's own attention gives; some sequences end inside it.  The last two
-    are large enough to be read in common by few rows each, in one launch with the sequences' own positions (8 rows of 16
-    bits) and in one of its own."""
+    """The prefix once for all gives what each sequence's own attention gives; some sequences end inside it.  The last
+    three are large enough to be read in common by few rows each (the last two for f32 too), in one launch with the
+    sequences' own positions (up to 8 rows, f32 5) and in one of its own."""
     print(f"shared {dtype} {batch} {tokens} {shared} {hk}x{group}", flush=True)
     page, hd = 64, 128
     cols = shared // page + 3
