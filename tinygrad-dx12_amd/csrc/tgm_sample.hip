@@ -748,8 +748,9 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int i = 2 * tid + q;
-    // in the mode of a listed bin at least one token lies above it
-    const bool keep = wd[q] >= 0.0 && wd[q] >= min_p && (!(p < 1.0) || (double)before < goal || (i == 0 && mode == kSampListAll));
+    // the first token of all stays whatever top-p asks for; a bin that is listed alone may be the first one
+    const bool keep = wd[q] >= 0.0 && wd[q] >= min_p &&
+                      (!(p < 1.0) || (double)before < goal || (i == 0 && (mode == kSampListAll || cut.size == cut.count)));
     before += w[q];
     if (!keep) w[q] = 0;
     mine += keep;
