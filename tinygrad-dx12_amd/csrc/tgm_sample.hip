@@ -676,9 +676,10 @@ __global__ void __launch_bounds__(kSampThreads) sample_draw(const SampleArgs A) 
   // The list.  Which tokens may belong to it is asked in 32 bits, with bounds half a bin too wide.
   SampList& li = u_.li;
   const double step = 1.0 / (kSampPerBin * ex.rate);
-  const bool narrow = step > (double)fabsf(best) * 0x1p-20 && best < INFINITY;  // else bins near 32 bits' resolution
   const double low = (double)best - ((double)cut.bin + 1.5) * step;
   const double high = mode == kSampListAll ? (double)best : (double)best - ((double)cut.bin - 0.5) * step;
+  // else bins near 32 bits' resolution, or bounds beyond their range (an infinite temperature: an infinite step)
+  const bool narrow = step > (double)fabsf(best) * 0x1p-20 && fabs((double)best) < 0x1p120 && fabs(low) < 0x1p120 && fabs(high) < 0x1p120;
   const float middle = narrow ? (float)(0.5 * (low + high)) : 0.f, reach = narrow ? (float)(0.5 * (high - low) + step) : INFINITY;
   __syncthreads();  // the bins have been read
   auto consider = [&](float x, int i) __attribute__((always_inline)) {
