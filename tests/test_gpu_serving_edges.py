@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_serving import BF16, F32, check_sample
+from test_gpu_serving import BF16, F16, F32, check_sample, i32, make_cache, make_table, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,40 @@ def test_sample_at_huge_temperatures(dev, n, temperature):
         for top_k, top_p, min_p in ((0, 0.9, 0.0), (0, 1.0, 0.5), (n // 2, 0.8, 0.0), (0, 1.0, 0.0)):
             for u in (torch.rand(3, generator=g), torch.zeros(3)):
                 check_sample(dev, x, u, temperature, top_k, top_p, min_p)
+
+
+# ----------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens,n,shared", [(1, 40, 0), (1, 2000, 0), (3, 2000, 0), (40, 50, 0), (40, 2000, 0), (40, 2000, 1024),
+                                             (1, 1100, 1024), (3, 1100, 1024)])
+def test_attend_shows_what_is_not_finite(dev, dtype, tokens, n, shared):
+    """A query row with a NaN or an infinity, and one whose score at one position is beyond 32 bits, are NaN, in one split
+    and in several; a score of -infinity weighs nothing; the other rows are what they were, and a token that sees nothing
+    still gives zeros.
+
+    The other rows may be rescaled at other blocks than before: both results hold the tolerance of test_gpu_serving.py, with
+    |v| and |k| up to 448 2^-7."""
+    print(f"not finite {dtype} tokens {tokens} positions {n} shared {shared}", flush=True)
+    batch, heads, hd = (104 if tokens < 40 and shared else 3), 12, 128
+    own = -(-n // 64) - shared // 64
+    c = make_cache(dev, shared // 64 + batch * own, 4, hd, 64, "fp8_e4m3", "fp8_e4m3", seed=50)
+    table = make_table(dev, batch, shared // 64 + own, shared // 64 + batch * own, 51, shared // 64)
+    lengths = i32(dev, [n, 0] + [n] * (batch - 2))
+    p = (n - tokens) // 2  # the first block of a key that sequence 0 sees: 448 2^118 in dim 7, zeros beside it
+    page = int(table[0, p // 64])
+    c.k_data[page, :, p % 64, :32] = 0
+    c.k_data[page, :, p % 64, 7], c.k_scales[page, :, 0, p % 64] = 0x7E, 245
+    q = randn(dev, 52, batch, tokens, heads, hd, dtype=dtype)
+    q[..., 7] = 0
+    want = c.attend(q, table, lengths, shared=shared)
+    assert torch.isfinite(want).all() and not want[1].any()
+    q[0, -1, 0, 5], q[0, -1, 1], q[0, -1, 2, 7], q[0, -1, 3, 7] = math.nan, math.inf, 1000.0, -1000.0
+    q[1, :, 4] = math.nan  # sees nothing
+    got = c.attend(q, table, lengths, shared=shared)
+    assert torch.isnan(got[0, -1, :3]).all()
+    assert torch.isfinite(got[0, -1, 3:]).all() and torch.isfinite(got[0, :-1]).all() and not got[1].any()
+    size = 3.5 * float(q[2:].abs().float().sum(-1).max()) / math.sqrt(hd)
+    tol = 2 * 3.5 * (2 * ((hd + 6) * 2.0 ** -24 * size + 2.0 ** -22) + 2.0 ** -17 + 2.0 ** -18) + want.double().abs() * torch.finfo(dtype).eps
+    off = (got.double() - want.double()).abs() - tol
+    assert float(off[0, -1, 4:].max()) <= 0 and float(off[2:].max()) <= 0
+    assert tokens == 1 or float(off[0, :-1].max()) <= 0

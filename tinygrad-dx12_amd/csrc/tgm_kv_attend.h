@@ -8,6 +8,10 @@
 // f32 3), each probability into 2 terms (16 bits; the output keeps 8 or 11) or, for f32 output, 3 (24 bits).  Products
 // of bf16 values are exact in fp32, sums, maxima and the softmax's sum are fp32; the output is rounded once.
 //
+// What is not finite shows: a row with a NaN among its scores, or with one of +infinity, is NaN (its sum of weights is, in
+// every split that holds such a score).  Zeros are for rows whose weights are all zero: no position is seen, or every
+// score is -infinity.
+//
 // A masked position's value codes are replaced by zeros before they meet a probability of zero, so that whatever lies
 // in memory that was never written (NaN codes among it) does not reach the sums.
 #pragma once

@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(256) attend_merge(const AttendArgs A, int pslo
   float M = m;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  const float w = l > 0.f ? __builtin_amdgcn_exp2f(m - M) : 0.f;
+  const float w = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - M);
   float sum = l * w;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(256) attend_merge(const AttendArgs A, int pslo
       const int s = s0 + u * N + sub;  // 63 at most where s0 < n <= 64
       ws[u] = __shfl(w, s, 64);        // 0 past the last one, and where a slot's sums were not written
       x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (ws[u] > 0.f) x[u] = *(const f32x4*)(p + s * HD);
+      if (ws[u] != 0.f) x[u] = *(const f32x4*)(p + s * HD);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) acc += x[u] * ws[u];
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(256) attend_merge(const AttendArgs A, int pslo
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o, 64);
   if (sub == 0) {
-    const float inv = sum > 0.f ? 1.0f / sum : 0.f;
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // NaN in any split: NaN
 #pragma unroll
     for (int e = 0; e < 4; ++e) at_store<DT>(A.out, row * HD + d + e, acc[e] * inv);
   }

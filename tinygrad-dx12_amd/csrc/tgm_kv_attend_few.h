@@ -296,7 +296,7 @@ __device__ __forceinline__ void few_body(const AttendArgs& A, unsigned char* lds
         }
         const int64_t row = ((int64_t)b * A.T + r / A.G) * A.H + j * A.G + r % A.G;
         if (A.slots == 1) {
-          at_store<DT>(A.out, row * HD + d, L > 0.f ? o / L : 0.f);
+          at_store<DT>(A.out, row * HD + d, L == 0.f ? 0.f : o / L);
         } else {
           A.part[(row * A.slots + A.slot0 + z) * HD + d] = o;
           if (d == 0) {

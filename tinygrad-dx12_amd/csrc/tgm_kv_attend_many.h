@@ -201,17 +201,17 @@ __device__ __forceinline__ void many_body(const AttendArgs& A, unsigned char* ld
   if (!rvalid) return;
   const int64_t row = ((int64_t)b * A.T + t) * A.H + h;
   if (A.slots == 1) {
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const float inv = 1.0f / l;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) at_store<DT>(A.out, row * HD + d * 32 + 8 * g + 4 * half + i, l > 0.f ? O[d][4 * g + i] * inv : 0.f);
+        for (int i = 0; i < 4; ++i) at_store<DT>(A.out, row * HD + d * 32 + 8 * g + 4 * half + i, l == 0.f ? 0.f : O[d][4 * g + i] * inv);
   } else {
     const int slot = A.slot0 + z;
     float* o = A.part + (row * A.slots + slot) * HD;
-    if (l > 0.f) {
+    if (l != 0.f) {
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll

@@ -170,8 +170,8 @@ class PackedKVCache:
         """Attention of the newest tokens: q [batch, tokens, heads, head_dim] (rotated), out alike.
 
         ``lengths`` (int32 [batch]) counts the cached positions of each sequence with the new tokens among them: token
-        t of sequence b sees positions 0 .. lengths[b] - tokens + t; a token that sees none gives zeros.  Query head h
-        reads kv head h // (heads // kv_heads).  Scores are multiplied by ``scale`` (1 / sqrt(head_dim)).
+        t of sequence b sees positions 0 .. lengths[b] - tokens + t; a token that sees none gives zeros, one whose scores
+        hold a NaN or +infinity gives NaN.  Query head h reads kv head h // (heads // kv_heads).  Scores are multiplied by ``scale`` (1 / sqrt(head_dim)).
 
         ``shared`` positions (a multiple of page_size) from the front are common to the batch: they lie in the pages
         that row 0 of the table names, and are read once for all sequences.
