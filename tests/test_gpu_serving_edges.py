@@ -75,3 +75,21 @@ def test_attend_shows_what_is_not_finite(dev, dtype, tokens, n, shared):
     off = (got.double() - want.double()).abs() - tol
     assert float(off[0, -1, 4:].max()) <= 0 and float(off[2:].max()) <= 0
     assert tokens == 1 or float(off[0, :-1].max()) <= 0
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 40])
+def test_attend_ignores_what_is_masked_of_a_prefix(dev, tokens):
+    """NaN codes and scales in positions of a prefix read in common that lie behind every sequence's end."""
+    batch, shared = 104, 1024
+    c = make_cache(dev, 16 + batch, 4, 128, 64, "fp8_e4m3", "fp8_e4m3", seed=60)
+    table = make_table(dev, batch, 17, 16 + batch, 61, 16)
+    q = randn(dev, 62, batch, tokens, 8, 128, dtype=BF16)
+    for most in (777, 100, 1):
+        lengths = i32(dev, [max(most - 3 * b, 0) for b in range(batch)])
+        want = c.attend(q, table, lengths, shared=shared)
+        assert torch.isfinite(want).all()
+        for p in range(most, shared):
+            page = int(table[0, p // 64])
+            c.k_data[page, :, p % 64], c.v_data[page, :, p % 64] = 127, 255
+            c.k_scales[page, :, :, p % 64] = c.v_scales[page, :, :, p % 64] = 255
+        assert torch.equal(c.attend(q, table, lengths, shared=shared), want)

@@ -50,9 +50,16 @@ __device__ __forceinline__ void many_body(const AttendArgs& A, unsigned char* ld
   const int b = A.common ? r / TG : seq;
   const int rt = r - (A.common ? b * TG : 0), t = rt / A.G, h = j * A.G + rt % A.G;
   const int last = min(at_length(A, b), A.kcap + A.T) - A.T + t;  // the last position this row sees
-  // positions any row of the workgroup sees
+  // positions any row of the workgroup sees: of a prefix those of its longest sequence (behind it nothing may be written)
   int kend = A.kcap;
-  if (!A.common) kend = min(kend, at_length(A, b) - A.T + (min(tile * kManyRows + kManyRows, nrows) - 1) / A.G + 1);
+  if (A.common) {
+    int most = 0;
+    for (int s = tile * kManyRows / TG + lane; s <= (min(tile * kManyRows + kManyRows, nrows) - 1) / TG; s += 64)
+      most = max(most, at_length(A, s));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+    kend = min(kend, __builtin_amdgcn_readfirstlane(most));
+  } else kend = min(kend, at_length(A, b) - A.T + (min(tile * kManyRows + kManyRows, nrows) - 1) / A.G + 1);
   const int k_lo = A.k0 + z * A.chunk, k_hi = min(k_lo + A.chunk, kend);
   const int nblocks = k_hi > k_lo ? (k_hi - k_lo + kManyKeys - 1) / kManyKeys : 0;
   int wave_min = last;
