@@ -6,6 +6,8 @@ import math
 import pytest
 import torch
 
+from tinygrad_mi355x.runtime import kernels as K
+from tinygrad_mi355x.sampling import sample
 from test_gpu_serving import BF16, F16, F32, check_sample, i32, make_cache, make_table, randn
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +95,24 @@ def test_attend_ignores_what_is_masked_of_a_prefix(dev, tokens):
             c.k_data[page, :, p % 64], c.v_data[page, :, p % 64] = 127, 255
             c.k_scales[page, :, :, p % 64] = c.v_scales[page, :, :, p % 64] = 255
         assert torch.equal(c.attend(q, table, lengths, shared=shared), want)
+
+
+# ----------------------------------------------------------------------------- workspaces
+def test_workspaces_are_held_until_the_launch(dev, monkeypatch):
+    """Memory that another thread takes on the same stream between a call's allocations and its launch is not the call's
+    workspace."""
+    c = make_cache(dev, 64, 2, 128, 64, "fp8_e4m3", "fp8_e4m3", seed=70)
+    q, table, lengths = randn(dev, 71, 1, 1, 8, 128), make_table(dev, 1, 64, 64, 72), i32(dev, [4000])
+    logits, u = randn(dev, 73, 2, 5000), torch.rand(2, device=dev)
+    seen = []
+
+    def call(name, *args):
+        at, need = args[11], args[12]
+        other = torch.empty(need, dtype=torch.uint8, device=dev)
+        seen.append((name, need > 0 and (other.data_ptr() >= at + need or other.data_ptr() + need <= at)))
+
+    monkeypatch.setattr(K, "call", call)
+    for _ in range(2):
+        c.attend(q, table, lengths)
+        sample(logits, u)
+    assert seen == [("tgm_kv_attend", True), ("tgm_sample", True)] * 2

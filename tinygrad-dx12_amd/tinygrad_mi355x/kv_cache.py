@@ -190,11 +190,12 @@ class PackedKVCache:
         q_arg, ld, cols, batch, tokens, need, index = plan
         if out is None:
             out = q.new_empty(q.shape)
-        # the workspace is of the caching allocator, so that calls on several streams never share one
-        workspace = q.new_empty(need, dtype=torch.uint8).data_ptr() if need else None
+        # the workspace is of the caching allocator, so that calls on several streams never share one; held until the
+        # launch, or another thread's call on this stream could be given its memory before that
+        workspace = q.new_empty(need, dtype=torch.uint8) if need else None
         if batch and tokens:
             K.call("tgm_kv_attend", self._arg, q_arg, q.data_ptr(), table.data_ptr(), ld, cols, lengths.data_ptr(), batch,
-                   tokens, shared, scale, workspace, need, out.data_ptr(), K.stream_on(index))
+                   tokens, shared, scale, K.ptr(workspace), need, out.data_ptr(), K.stream_on(index))
         return out
 
     def _attend_plan(self, sig, q, table, lengths, shared) -> tuple:

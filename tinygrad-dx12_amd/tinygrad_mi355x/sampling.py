@@ -43,13 +43,14 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
         min_p = _filled(min_p, rows, torch.float32, logits.device)
     if out is None:
         out = logits.new_empty(rows, dtype=torch.int32)
-    # the workspace is of the caching allocator, so that calls on several streams never share one
-    workspace = logits.new_empty(need, dtype=torch.uint8).data_ptr() if need else None
+    # the workspace is of the caching allocator, so that calls on several streams never share one; held until the launch, or
+    # another thread's call on this stream could be given its memory before that
+    workspace = logits.new_empty(need, dtype=torch.uint8) if need else None
     if not rows:
         return out
     K.call("tgm_sample", logits.data_ptr(), dt, rows, vocab, ld, u.data_ptr(), temperature.data_ptr(),
            None if top_k is None else top_k.data_ptr(), None if top_p is None else top_p.data_ptr(),
-           None if min_p is None else min_p.data_ptr(), out.data_ptr(), workspace, need, K.stream_on(index))
+           None if min_p is None else min_p.data_ptr(), out.data_ptr(), K.ptr(workspace), need, K.stream_on(index))
     return out
 
 
