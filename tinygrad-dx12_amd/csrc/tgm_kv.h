@@ -151,7 +151,8 @@ inline int kv_check(const tgm_kv_cache* c, const int32_t* table, int64_t ld_tabl
                 "cache formats are fp8_e4m3 and fp4_e2m1");
   TGM_CHECK_ARG((((uintptr_t)c->k_data | (uintptr_t)c->k_scales | (uintptr_t)c->v_data | (uintptr_t)c->v_scales) & 15) == 0,
                 "the stores must be 16-byte aligned");
-  TGM_CHECK_ARG(table_cols >= 0 && ld_table >= table_cols && table_cols * c->page_size < (1ll << 30), "invalid page table");
+  TGM_CHECK_ARG(table_cols >= 0 && ld_table >= table_cols && table_cols < (1ll << 30) && table_cols * c->page_size < (1ll << 30),
+                "invalid page table");
   int shift = 0;
   while ((1ll << shift) < c->page_size) ++shift;
   k = {(uint8_t*)c->k_data, (uint8_t*)c->k_scales};

@@ -132,9 +132,10 @@ static void attend_go(const AttendPlan& p, AttendLaunch l, int shared, int cap, 
 }
 
 static bool attend_sizes_ok(const tgm_kv_cache* c, int64_t heads, int64_t batch, int64_t tokens, int64_t cols, int64_t shared) {
-  return c && c->kv_heads > 0 && c->page_size > 0 && heads > 0 && heads % c->kv_heads == 0 && heads <= 65535 && batch >= 0 &&
-         batch <= 65535 && tokens >= 0 && batch * tokens < (1ll << 24) && batch * tokens * heads < (1ll << 30) && cols >= 0 &&
-         cols * c->page_size < (1ll << 30) && shared >= 0 && shared <= cols * c->page_size && shared % c->page_size == 0;
+  return c && c->kv_heads > 0 && c->page_size > 0 && c->page_size <= 1024 && (c->head_dim == 64 || c->head_dim == 128) &&
+         heads > 0 && heads % c->kv_heads == 0 && heads <= 65535 && batch >= 0 && batch <= 65535 && tokens >= 0 &&
+         tokens < (1ll << 24) && batch * tokens < (1ll << 24) && batch * tokens * heads < (1ll << 30) && cols >= 0 &&
+         cols < (1ll << 30) && cols * c->page_size < (1ll << 30) && shared >= 0 && shared <= cols * c->page_size && shared % c->page_size == 0;
 }
 
 }  // namespace tgm

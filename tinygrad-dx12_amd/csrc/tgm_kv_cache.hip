@@ -222,7 +222,8 @@ extern "C" int tgm_kv_append(const tgm_kv_cache* cache, const tgm_rotary* rotary
   TGM_CHECK_ARG(k && v && (q != nullptr) == (q_out != nullptr), "null argument");
   if (rotary)
     if (const int e = rot_check(rotary, cache->head_dim)) return e;
-  TGM_CHECK_ARG(batch >= 0 && tokens >= 0 && batch * tokens < (1ll << 30), "sizes out of range");
+  TGM_CHECK_ARG(batch >= 0 && tokens >= 0 && batch < (1ll << 30) && tokens < (1ll << 30) && batch * tokens < (1ll << 30),
+                "sizes out of range");
   TGM_CHECK_ARG(heads_dtype_ok(k->dtype) && v->dtype == k->dtype && (!q || (q->dtype == k->dtype && q_out->dtype == k->dtype)),
                 "q, k and v must be f32, f16 or bf16 and alike");
   TGM_CHECK_ARG(k->heads == cache->kv_heads && v->heads == cache->kv_heads, "k and v must have the cache's heads");
