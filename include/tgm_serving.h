@@ -65,7 +65,8 @@ typedef struct tgm_heads {
 } tgm_heads;
 
 /* out = x rotated, token t of sequence b at position start[b] + t.  Angles, sines and products
- * are computed in 64 bits and rounded once to 32 and once to the output's type.  out may be x. */
+ * are computed in 64 bits and rounded once to 32 and once to the output's type.  out may be x;
+ * any other memory that the two share, or that elements of out share, is a race. */
 int tgm_rotate(const tgm_rotary* rotary, const tgm_heads* x, const void* x_data, const tgm_heads* out, void* out_data,
                const int32_t* start, int64_t batch, int64_t tokens, int64_t head_dim, void* stream);
 

@@ -15,6 +15,7 @@ import struct
 import torch
 
 from tinygrad_mi355x.runtime import kernels as K
+from tinygrad_mi355x.runtime.overlap import OutLayout
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 FLOATS = (torch.float32, torch.float16, torch.bfloat16)
@@ -132,7 +133,8 @@ class Rotary:
     def rotate(self, x: torch.Tensor, start: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
         """x [batch, tokens, heads, head_dim] rotated; token t of sequence b stands at position start[b] + t.
 
-        ``start``: int32 [batch].  ``out`` may be x itself.  Angles, sines and products are computed in 64 bits.
+        ``start``: int32 [batch].  ``out`` is x itself or shares no memory with it.  Angles, sines and products are computed in
+        64 bits.
         """
         sig = (x.shape, x.stride(), x.dtype, x.get_device(), start.shape, start.stride(), start.dtype, start.get_device())
         plan = self._plans.get(sig)
@@ -142,14 +144,19 @@ class Rotary:
         if out is None:
             out = x.new_empty(shape)
         else:
-            check_heads(out, "out")
-            if out.shape != shape or out.dtype is not x.dtype or out.device != x.device:
-                raise ValueError("out must be like x")
-            out_arg = heads_arg(out)
+            out_sig = (sig, out.shape, out.stride(), out.dtype, out.get_device())
+            out_arg, layout = self._plans.get(out_sig) or self._out_plan(out_sig, x, out)
+            layout.check(out, x, "x")
         if batch and tokens:
             K.call("tgm_rotate", self.arg, x_arg, x.data_ptr(), out_arg, out.data_ptr(), start.data_ptr(), batch, tokens,
                    self.head_dim, K.stream_on(index))
         return out
+
+    def _out_plan(self, sig, x: torch.Tensor, out: torch.Tensor) -> tuple:
+        check_heads(out, "out")
+        if out.shape != x.shape or out.dtype is not x.dtype or out.device != x.device:
+            raise ValueError("out must be like x")
+        return self._plans.keep(sig, (heads_arg(out), OutLayout(out, x)))
 
     def _plan(self, sig, x: torch.Tensor, start: torch.Tensor) -> tuple:
         check_heads(x, "x")
