@@ -92,8 +92,8 @@ int tgm_kv_read(const tgm_kv_cache* cache, const int32_t* table, int64_t ld_tabl
  * the cached positions of sequence b, the new tokens among them: token t sees the positions up to
  * lengths[b] - tokens + t; one that sees none gives zeros, one with a NaN among its scores or with
  * one of +infinity (a query that is not finite, a product beyond 32 bits) gives NaN.
- * out [batch, tokens, heads, head_dim] contiguous, of q's type; scores are multiplied by scale,
- * softmax and sums are held in 32 bits.
+ * out [batch, tokens, heads, head_dim] contiguous, of q's type, and q itself or memory that the two
+ * do not share; scores are multiplied by scale, softmax and sums are held in 32 bits.
  * shared > 0 (a multiple of page_size): positions below it lie in the same pages for every
  * sequence (those of row 0 of the table) and are read once for the whole batch.
  * workspace: tgm_kv_attend_workspace() bytes, 16-byte aligned. */

@@ -97,6 +97,18 @@ def test_attend_ignores_what_is_masked_of_a_prefix(dev, tokens):
         assert torch.equal(c.attend(q, table, lengths, shared=shared), want)
 
 
+@pytest.mark.parametrize("tokens,n,shared", [(1, 60, 0), (1, 1500, 0), (40, 60, 0), (40, 1500, 0), (1, 1100, 1024), (3, 1100, 1024)])
+def test_attend_in_place(dev, tokens, n, shared):
+    """out may be q itself: what every workgroup reads of it, it alone writes."""
+    batch = 104 if shared else 3
+    own = -(-n // 64) - shared // 64
+    c = make_cache(dev, shared // 64 + batch * own, 4, 128, 64, "fp8_e4m3", "fp4_e2m1", seed=65)
+    table, lengths = make_table(dev, batch, shared // 64 + own, shared // 64 + batch * own, 66, shared // 64), i32(dev, [n] * batch)
+    q = randn(dev, 67, batch, tokens, 8, 128, dtype=BF16)
+    want = c.attend(q, table, lengths, shared=shared)
+    assert c.attend(q, table, lengths, shared=shared, out=q) is q and torch.equal(q, want)
+
+
 # ----------------------------------------------------------------------------- workspaces
 def test_workspaces_are_held_until_the_launch(dev, monkeypatch):
     """Memory that another thread takes on the same stream between a call's allocations and its launch is not the call's

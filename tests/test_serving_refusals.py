@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from test_serving_host import c_cache, c_heads
+from tinygrad_mi355x.kv_cache import PackedKVCache
 from tinygrad_mi355x.rotary import Rotary
 from tinygrad_mi355x.runtime import kernels as K
 from tinygrad_mi355x.runtime.overlap import overlap, overlaps_itself
@@ -83,3 +84,22 @@ def test_rotate_refuses_an_output_that_overlaps(monkeypatch):
     with pytest.raises(ValueError):
         r.rotate(x[:, :, :1].expand_as(x), start, out=x[:, :, :1].expand_as(x))
     assert len(calls) == 5
+
+
+def test_attend_refuses_an_output_that_overlaps(monkeypatch):
+    calls = []
+    monkeypatch.setattr(K, "require_device", lambda t: None)
+    monkeypatch.setattr(K, "stream_on", lambda i: 0)
+    monkeypatch.setattr(K, "call", lambda name, *args: calls.append(name))
+    c, table, n = PackedKVCache(4, 2, 64, device="cpu"), torch.zeros((2, 2), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    flat = torch.zeros(3 * 3 * 4 * 64)
+    q, wide = flat[:2 * 3 * 4 * 64].view(2, 3, 4, 64), torch.zeros(2, 3, 8, 64)
+    for x, out in ((q, q), (q, torch.zeros_like(q)), (flat[256:512].view(1, 1, 4, 64), flat[:256].view(1, 1, 4, 64)),
+                   (wide[:, :, :4], torch.zeros_like(q))):
+        assert c.attend(x, table[:len(x)], n[:len(x)], out=out) is out
+    assert len(calls) == 4
+    for x, out in ((q, flat[64:][:q.numel()].view(2, 3, 4, 64)), (q, flat[768:].view(2, 3, 4, 64)),
+                   (wide[:, :, :4], wide.view(-1)[:q.numel()].view(2, 3, 4, 64))):
+        with pytest.raises(ValueError):
+            c.attend(x, table, n, out=out)
+    assert len(calls) == 4

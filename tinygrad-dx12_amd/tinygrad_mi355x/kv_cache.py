@@ -27,6 +27,7 @@ import torch
 
 from tinygrad_mi355x.rotary import _DT, _HEADS, Plans, Rotary, check_heads, check_index, heads_arg
 from tinygrad_mi355x.runtime import kernels as K
+from tinygrad_mi355x.runtime.overlap import OutLayout
 
 FORMATS = {"fp8_e4m3": (0, 8), "fp4_e2m1": (1, 4)}  # enum tgm_kv_format, bits of a code
 BLOCK = 32
@@ -167,11 +168,13 @@ class PackedKVCache:
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, *, shared: int = 0,
                scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-        """Attention of the newest tokens: q [batch, tokens, heads, head_dim] (rotated), out alike.
+        """Attention of the newest tokens: q [batch, tokens, heads, head_dim] (rotated), out alike; ``out``, if given, is
+        contiguous, and q itself or memory that the two do not share.
 
         ``lengths`` (int32 [batch]) counts the cached positions of each sequence with the new tokens among them: token
         t of sequence b sees positions 0 .. lengths[b] - tokens + t; a token that sees none gives zeros, one whose scores
-        hold a NaN or +infinity gives NaN.  Query head h reads kv head h // (heads // kv_heads).  Scores are multiplied by ``scale`` (1 / sqrt(head_dim)).
+        hold a NaN or +infinity gives NaN.  Query head h reads kv head h // (heads // kv_heads).  Scores are multiplied by
+        ``scale`` (1 / sqrt(head_dim)).
 
         ``shared`` positions (a multiple of page_size) from the front are common to the batch: they lie in the pages
         that row 0 of the table names, and are read once for all sequences.
@@ -190,6 +193,9 @@ class PackedKVCache:
         q_arg, ld, cols, batch, tokens, need, index = plan
         if out is None:
             out = q.new_empty(q.shape)
+        else:
+            out_sig = (q.shape, q.stride(), q.dtype)
+            (self._plans.get(out_sig) or self._plans.keep(out_sig, OutLayout(out, q))).check(out, q, "q")
         # the workspace is of the caching allocator, so that calls on several streams never share one; held until the
         # launch, or another thread's call on this stream could be given its memory before that
         workspace = q.new_empty(need, dtype=torch.uint8) if need else None
