@@ -43,6 +43,7 @@ class ServingDecoder(Decoder):
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self.u = torch.zeros(batch, dtype=torch.float32, device=self.device)
         self._filters: dict[str, torch.Tensor] = {}
+        self._prefix_loaded = prefix == 0
 
     def _allocate_cache(self) -> None:
         cfg, page = self.cfg, self._cache_kw["page_size"]
@@ -97,16 +98,21 @@ class ServingDecoder(Decoder):
         if not self.prefix:
             return
         self._check_prompt(tokens[None], 1, "prefix")
+        self._prefix_loaded = False
         self.pos.zero_()
         for t0 in range(0, self.prefix, self.max_prompt):
             chunk = tokens[t0:t0 + self.max_prompt]
             self._pass(chunk, 1, chunk.shape[0])
+        self._prefix_loaded = True
 
     def prefill(self, prompts: torch.Tensor) -> torch.Tensor:
-        """Run the prompts (int [batch, T], T of any length) behind the prefix; the first sampled tokens."""
+        """Run the prompts (int [batch, T], T of any length) behind the prefix, which has to be loaded; the first sampled
+        tokens."""
         self._check_prompt(prompts, self.batch, "prompts")
         if self.prefix + prompts.shape[1] > self.max_seq:
             raise ValueError("prefix + prompt exceed max_seq")
+        if not self._prefix_loaded:
+            raise RuntimeError(f"the prefix of {self.prefix} positions is not loaded: call load_prefix first")
         self.pos.fill_(self.prefix)
         for t0 in range(0, prompts.shape[1], self.max_prompt):
             chunk = prompts[:, t0:t0 + self.max_prompt]
