@@ -24,3 +24,29 @@ def test_prompts_need_the_prefix(dev):
     d.load_prefix(prompts_of(dev, 1, 64)[0])
     first = d.generate(prompts_of(dev, 2, 4), 3, u)
     assert torch.equal(d.generate(prompts_of(dev, 2, 4), 3, u), first)  # loaded once
+
+
+def test_a_held_graph_follows_the_filters(dev):
+    """A step captured once and replayed behind a later generate draws with that one's filters, as an eager step does."""
+    d = ServingDecoder(random_weights(SMALL, dev, seed=21), SMALL, 3, 128, 16)
+    prompts, u = prompts_of(dev, 3, 20, 22), torch.rand((3, 2), generator=torch.Generator().manual_seed(23)).to(dev)
+    d.generate(prompts, 2, u)
+    graph = d.capture()
+    drawn = []
+    for filters in (dict(temperature=0.0), dict(temperature=1.5), dict(temperature=torch.tensor([2.0, 0.0, 1.0]), top_k=1),
+                    dict(temperature=1.5, top_k=torch.tensor([0, 40, 3]), top_p=0.9, min_p=0.02), dict(temperature=1.5, top_p=0.3)):
+        for i in range(2):
+            d.generate(prompts, 2, u, **filters)
+            junk = [torch.full((3,), 7.0, device=dev) for _ in range(64)]  # what a freed parameter would read as
+            d.u.fill_(0.7 - 0.3 * i)
+            tokens, pos = d.tokens[:3].clone(), d.pos.clone()
+            d.step()
+            want, logits = d.tokens[:3].clone(), d.logits.clone()
+            d.tokens[:3], d.pos[:] = tokens, pos
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(d.logits, logits) and torch.equal(d.tokens[:3], want), filters
+            drawn.append(want.tolist())
+            del junk
+    assert len(set(map(str, drawn))) > 3  # they do differ

@@ -42,7 +42,10 @@ class ServingDecoder(Decoder):
         self.rotary = rotary
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self.u = torch.zeros(batch, dtype=torch.float32, device=self.device)
-        self._filters: dict[str, torch.Tensor] = {}
+        # written to and never replaced, as everything else that a step reads: a captured step holds their addresses
+        self._filters = {name: torch.full((batch,), value, dtype=dtype, device=self.device) for name, value, dtype in (
+            ("temperature", 1.0, torch.float32), ("top_k", 0, torch.int32), ("top_p", 1.0, torch.float32),
+            ("min_p", 0.0, torch.float32))}
         self._prefix_loaded = prefix == 0
 
     def _allocate_cache(self) -> None:
@@ -125,7 +128,8 @@ class ServingDecoder(Decoder):
         self._draw(0, 1)
 
     def capture(self) -> torch.cuda.CUDAGraph:
-        """One step as a graph, with the tensors it allocates in a pool of its own."""
+        """One step as a graph, with the tensors it allocates in a pool of its own.  Replays step on from where the decoder
+        is (``pos``, ``tokens``, ``u``), with the filters of the last ``generate``."""
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             self._decode_step()
@@ -139,9 +143,9 @@ class ServingDecoder(Decoder):
             raise ValueError("prefix + prompt + generated tokens exceed max_seq")
         if u.shape != (self.batch, new_tokens) or u.dtype is not torch.float32 or u.device != self.device:
             raise ValueError(f"u must be float32 [{self.batch}, {new_tokens}] on {self.device}")
-        for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                                   ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-            self._filters[name] = torch.as_tensor(value, dtype=dtype, device=self.device).expand(self.batch).contiguous()
+        for name, value in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+            held = self._filters[name]
+            held.copy_(torch.as_tensor(value, dtype=held.dtype, device=self.device).expand(self.batch))
         history = torch.empty((self.batch, new_tokens), dtype=torch.int32, device=self.device)
         self.u.copy_(u[:, 0])
         history[:, 0] = self.prefill(prompts)
