@@ -1,5 +1,7 @@
 """The serving loop in states that a program can bring it into."""
 
+from dataclasses import replace
+
 import pytest
 import torch
 
@@ -50,3 +52,20 @@ def test_a_held_graph_follows_the_filters(dev):
             drawn.append(want.tolist())
             del junk
     assert len(set(map(str, drawn))) > 3  # they do differ
+
+
+def test_traces_of_a_prefix_in_short_chunks(dev):
+    """Chunks of 5 to 7 tokens of one sequence in a decoder of 8: the traced feed-forward output is the one that the next
+    layer adds, in whatever form the down projection computes it (fp32 sums in another order: 2^-20 of the norm)."""
+    cfg = replace(SMALL, ffn=4096)
+    w = random_weights(cfg, dev, seed=24)
+    d = ServingDecoder(w, cfg, 8, 64, 6, prefix=16, page_size=16)
+    assert d.down_slices == 2
+    tokens, traces = prompts_of(dev, 1, 16, 25)[0], []
+    for slices in (2, 1):
+        d.down_slices, d.layer_trace = slices, []
+        d.load_prefix(tokens)
+        traces.append(d.layer_trace[:cfg.layers])  # of the first chunk; its first layer sees the same input both times
+    a, b = traces[0][0], traces[1][0]
+    assert torch.equal(a["act"], b["act"])
+    assert (a["delta"] - b["delta"]).norm() <= 2.0 ** -20 * b["delta"].norm()

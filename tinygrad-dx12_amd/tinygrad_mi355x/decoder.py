@@ -367,10 +367,11 @@ class Decoder:
     def _trace(self, rows: int, fused_norm: bool = False, parts: int = 0) -> None:
         if self.layer_trace is not None:
             delta = self.delta[:rows].clone()
-            if parts:  # the parts summed in the order the next norm adds them
-                delta = self.delta_parts[0, :rows].clone()
+            if parts:  # `rows` rows a part, summed in the order the next norm adds them
+                held = self.delta_parts.view(-1)[:parts * rows * self.cfg.hidden].view(parts, rows, -1)
+                delta = held[0].clone()
                 for p in range(1, parts):
-                    delta += self.delta_parts[p, :rows]
+                    delta += held[p]
             self.layer_trace.append({
                 "h": self.h[:rows].clone(), "delta": delta, "attn": self.attn[:rows].clone(),
                 "act": self.act[:rows].clone(), "x16": None if fused_norm else self.xn16[:rows].clone(),
