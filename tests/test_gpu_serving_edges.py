@@ -6,11 +6,31 @@ import math
 import pytest
 import torch
 
+from tinygrad_mi355x.rotary import Rotary
 from tinygrad_mi355x.runtime import kernels as K
 from tinygrad_mi355x.sampling import sample
 from test_gpu_serving import BF16, F16, F32, check_sample, i32, make_cache, make_table, randn
 
 pytestmark = pytest.mark.gpu
+
+
+# ----------------------------------------------------------------------------- rotary positions
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("head_dim,rotary_dim,layout", [(64, None, "half"), (128, None, "half"), (128, None, "interleaved"),
+                                                        (128, 64, "half"), (64, 32, "interleaved"), (96, None, "half"),
+                                                        (80, 48, "interleaved")])
+def test_rotate_rounds_to_32_bits_and_then_to_its_type(dev, dtype, head_dim, rotary_dim, layout):
+    """16-bit results are the 32-bit ones rounded, also where that is a tie which the exact value is not; the cache write's
+    queries are those of ``rotate``."""
+    print(f"roundings {dtype} {head_dim} {rotary_dim} {layout}", flush=True)
+    rot, start = Rotary(head_dim, rotary_dim, layout=layout, device=dev), i32(dev, [5, 1000, 77777])
+    x = randn(dev, 80, 3, 400, 16, head_dim, dtype=dtype)
+    got = rot.rotate(x, start)
+    assert torch.equal(got, rot.rotate(x.float(), start).to(dtype))
+    if head_dim in (64, 128):
+        c, none = make_cache(dev, 1, 1, head_dim, 64, "fp8_e4m3", "fp8_e4m3"), torch.full((3, 1), -1, dtype=torch.int32, device=dev)
+        k = randn(dev, 81, 3, 400, 1, head_dim, dtype=dtype)
+        assert torch.equal(c.append(k, k, none, start, rotary=rot, q=x).q, got)
 
 
 # ----------------------------------------------------------------------------- sampling

@@ -86,6 +86,7 @@ struct RotLane {
 template <int DT, int HD, int MODE>
 __device__ __forceinline__ void rot_apply(const RotArgs& rot, const RotLane<HD, MODE>& t, const double2* cs, int chunk,
                                           const void* x, int64_t at, float (&a)[8], float (&b)[8]) {
+#pragma clang fp contract(off)  // else the rounding to 32 bits may be merged with the caller's to 16
   if constexpr (MODE == kRotHalf) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {

@@ -47,6 +47,7 @@ constexpr int kRotAnyPairs = 512;
 template <int DT>
 __global__ void __launch_bounds__(256) rotate_any(RotArgs rot, RotView x, RotView y, int H, int D, int interleaved,
                                                   const int32_t* start, int T) {
+#pragma clang fp contract(off)  // else the rounding to 32 bits may be merged with the one to 16
   __shared__ double2 angles[kRotAnyPairs];
   const int64_t token = blockIdx.x;
   const int b = (int)(token / T), t = (int)(token - (int64_t)b * T);
