@@ -69,7 +69,10 @@ struct AttendPlan {
 
 static int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// Splits of `span` positions over about `want` workgroups per row tile, in chunks that are a multiple of `unit`.
+// Splits of `span` positions over about `want` workgroups per row tile, in chunks that are a multiple of `unit`.  The span
+// is the table's, since the lengths are on the device: in a table that is wider than its sequences fewer splits hold work
+// (512 tokens over 8500 positions take 123 us in a table of 8512, 348 in one of 32768; one token over 2000 of one
+// sequence 11 in a table of up to 8192, 15 of 32768, 36 of 131072).
 static void split_span(int64_t span, int64_t want, int64_t unit, int64_t most, int& chunk, int& splits) {
   int64_t n = want < 1 ? 1 : (want > most ? most : want);
   const int64_t c = round_up((span + n - 1) / n, unit);
@@ -81,11 +84,16 @@ static AttendPlan attend_plan(const tgm_kv_cache* c, int64_t dt, int64_t heads, 
                               int64_t shared) {
   AttendPlan p{};
   const int64_t G = heads / c->kv_heads, rows = tokens * G, cap = cols * c->page_size;
+  // attend_few as far as its columns reach: 16 rows of 16 sequences of 8000 positions take 73 us there and 109 in
+  // attend_many (one sequence 15 and 20), f32 with 10 rows 77 and 215 (16 and 32); from there on attend_many takes what its
+  // 128 rows take, 110 us for 24 rows (f32 217)
   p.many = rows > attend_few_rows((int)dt);
   // A prefix that a few rows read goes with each sequence, through row 0's pages and out of the caches: the products over
-  // 128 rows at a time, most of them empty, take longer.  In common and so, us, fp8: 8 sequences on 2048 positions of 8
-  // heads 17 and 17 (bf16), 16 of them 19 and 23, 32 of them 21 and 34; f32, whose rows split into three terms, 16 of them
-  // 26 and 25, 32 of them 29 and 38.
+  // 128 rows at a time, most of them empty, take longer.  In common and so, us, fp8, 8 kv heads of 4: 8 sequences on 2048
+  // positions 16.2 and 14.1 (bf16), 12 of them 17.5 and 16.9, 16 of them 19.6 and 19.6, 24 of them 20.7 and 24.0; 8 on 4096
+  // positions 18.2 and 19.9; f32, whose rows split into three terms, 16 on 2048 26.5 and 24.0, 24 of them 28.2 and 30.7, 12
+  // on 4096 32.2 and 30.5.  (One kv head on 16384 positions crosses later: 16 sequences 23.7 and 20.9, 32 of them 25.2 and
+  // 29.6.)
   const int64_t alone = dt == TGM_F32 ? 2 * kAlonePairs : kAlonePairs;
   p.prefix = shared > 0 && (p.many || batch * shared * c->kv_heads > alone) ? (int)shared : 0;
   const int64_t own = cap > p.prefix ? cap - p.prefix : 0;
@@ -99,8 +107,9 @@ static AttendPlan attend_plan(const tgm_kv_cache* c, int64_t dt, int64_t heads, 
     const int64_t tiles = (rows + kManyRows - 1) / kManyRows * heads_of_all;
     split_span(own, 512 / tiles, kManyKeys, most, p.chunk, p.splits);
   } else {
-    // six rounds of two workgroups a CU, a split at least one block a wave: fewer leave CUs idle at the end of ragged
-    // batches (16 sequences of up to 32700 positions: 155 us with half as many, 141 so, 145 with twice as many)
+    // six rounds of two workgroups a CU, a split at least one block a wave: fewer leave CUs idle at the end of long ragged
+    // batches (16 sequences of up to 32700 positions: 150 us with half as many, 132 so, 133 with twice as many; short ones
+    // would take fewer: 32 of up to 4000 37, 45 and 46)
     split_span(own, (6 * 512 + heads_of_all - 1) / heads_of_all, kFewWaves * kFewBlock, most, p.chunk, p.splits);
   }
   const int slots = p.splits + p.psplits;

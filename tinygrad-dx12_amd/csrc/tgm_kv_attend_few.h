@@ -15,11 +15,11 @@
 // column c in lane group g are then keys 16 g + 4 v + i, and the products with V take the keys with i = 0, 1 and then
 // those with i = 2, 3: V goes through LDS in these two halves.
 //
-// Bound by memory: 16 sequences of up to 32700 positions, 32 query and 8 kv heads of 128, fp8 (640 MB) take 129 us with
-// the join, 4.95 TB/s (a copy reaches 5.1), the vector instructions busy for a quarter of it and the matrix pipe for 6 %.
+// Bound by memory: 16 sequences of up to 32700 positions, 32 query and 8 kv heads of 128, fp8 (640 MB) take 132 us with
+// the join, 4.85 TB/s (a copy reaches 5.1), the vector instructions busy for a quarter of it and the matrix pipe for 6 %.
 // What keeps the memory busy is waves: three per SIMD that load a block of 64 positions (16 KB) and compute it beat two
 // that hold the next block in registers (140), and four, which spill (220).  f32 queries stay at two (16 x 16000 positions:
-// 118 us, at three, spilling, 122).  Short ones are a chain of latencies: 1000 positions of one sequence take 8 us, and
+// 121 us, at three, spilling, 123; 16 x 8000 61 and 58).  Short ones are a chain of latencies: 1000 positions of one sequence take 8 us, and
 // the join 3.
 #pragma once
 
