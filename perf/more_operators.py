@@ -78,7 +78,8 @@ def draw(rng):
         top_groups = rng.randint(1, groups)
         return dict(kind=kind, dtype=rng.choice(["float32", "float32", "bfloat16", "float16"]),
                     tokens=_log_int(rng, 1, 8192), experts=experts,
-                    top_k=rng.randint(1, min(8, experts // groups * top_groups)), score=rng.choice(["softmax", "sigmoid"]), bias=rng.choice([False, True]), groups=groups,
+                    top_k=rng.randint(1, min(8, experts // groups * top_groups)),
+                    score=rng.choice(["softmax", "sigmoid"]), bias=rng.choice([False, True]), groups=groups,
                     top_groups=top_groups, renormalize=rng.choice([False, True, True]), scale=rng.choice([1.0, 2.5]))
     if kind == "logprobs":
         vocab = _log_int(rng, 500, 131072)
