@@ -1,5 +1,5 @@
 """ctypes binding of the gfx950 kernel library ``libtgm_mi355x.so`` (include/tgm_packed.h,
-include/tgm_decoder.h, include/tgm_serving.h), with no torch dependency.
+include/tgm_decoder.h, include/tgm_serving.h, include/tgm_experts.h), with no torch dependency.
 
 This is the only route from Python into the packed kernels: the plugin-buffer path
 (``codegen/program.py``) calls it with plugin buffer addresses and the device stream, the
@@ -94,6 +94,8 @@ SIGNATURES = {
     "tgm_kv_read": (_P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _INT, _P),
     "tgm_kv_attend": (_P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, ctypes.c_double, _P, _I64, _P, _P),
     "tgm_sample": (_P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P),
+    # mixture-of-experts operators (include/tgm_experts.h)
+    "tgm_route": (_P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, ctypes.c_double, _P, _P, _P),
 }
 EXPORTS = ("tgm_abi_version", "tgm_last_error", "tgm_dec_attention_workspace", "tgm_gemm_w_split_workspace",
            "tgm_gemm_w_split_noalloc_capacity", "tgm_kv_attend_workspace", "tgm_sample_workspace", *SIGNATURES)
