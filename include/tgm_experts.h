@@ -58,7 +58,7 @@ typedef struct tgm_experts {
 /* y[t] = sum_j weights[t, j] down_e . (silu(gate_e . x[t]) * (up_e . x[t])),  e = ids[t, j]
  *
  * x [tokens, hidden] (row stride ldx, a multiple of 8; 16-byte aligned), ids and weights [tokens, top_k]
- * contiguous, y [tokens, hidden] (row stride ldy) of x's type or F32, sharing no memory with x.  An id
+ * contiguous, y [tokens, hidden] (row stride ldy) of x's type or F32; y may be x.  An id
  * outside [0, experts) names no expert and adds nothing; the same expert may be named twice.  Products
  * and sums over K, experts and tokens are float32; silu(gate) * up is rounded to x's type on its way into
  * the down product.  Results do not depend on the other tokens of the batch but for the rounding of sums,

@@ -39,3 +39,26 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, 
             if np.isnan(p).any():
                 weights[t] = np.nan
     return ids, weights
+
+
+def experts(x, ids, weights, gate_up, down, eps):
+    """y [tokens, hidden], and how far 32-bit sums and hidden values rounded to half a step ``eps / 2`` may be from it:
+    gate_up [experts, 2 ffn, hidden] and down [experts, hidden, ffn] are the weights' values.
+
+    A 32-bit sum of n products is off by at most n 2^-24 of their sizes' sum; silu has a slope below 1.1; exp, the quotient
+    and two products are off by at most 2^-21 of the hidden value together."""
+    y, tol, unit = np.zeros(x.shape), np.zeros(x.shape), 2.0 ** -24
+    d, f = x.shape[1], down.shape[2]
+    for e in sorted(set(ids.flatten().tolist())):
+        if not 0 <= e < len(gate_up):
+            continue
+        t, j = np.nonzero(ids == e)
+        g, u = (x[t] @ gate_up[e][i::2].T for i in (0, 1))
+        eg, eu = (d * unit * (np.abs(x[t]) @ np.abs(gate_up[e][i::2]).T) for i in (0, 1))
+        s = g / (1 + np.exp(-g))
+        h = s * u
+        eh = 1.1 * eg * (np.abs(u) + eu) + np.abs(s) * eu + (2.0 ** -21 + eps / 2) * np.abs(h)
+        w = np.abs(weights[t, j])[:, None]
+        np.add.at(y, t, weights[t, j][:, None] * (h @ down[e].T))
+        np.add.at(tol, t, w * ((eh * (1 + f * unit) + (f + ids.shape[1] + 1) * unit * np.abs(h)) @ np.abs(down[e]).T))
+    return y, tol

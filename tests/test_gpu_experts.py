@@ -9,7 +9,9 @@ import pytest
 import torch
 
 import experts_oracle as X
-from tinygrad_mi355x.experts import route
+import packed_oracle as O
+from tinygrad_mi355x.codegen.decomp.mi355x import PackedTensor
+from tinygrad_mi355x.experts import PackedExperts, route
 
 pytestmark = pytest.mark.gpu
 
@@ -113,3 +115,163 @@ def test_route_again_and_on_another_stream(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got.ids, want.ids) and torch.equal(got.weights, want.weights)
+
+
+# ----------------------------------------------------------------------------- the experts' products
+BITS = {"fp4_e2m1": 4, "fp6_e2m3": 6, "fp6_e3m2": 6, "int4": 4, "uint4": 4}
+
+
+def packed(dev, rng, fmt, shape, scales, block):
+    """A packed weight of values of about 0.1, and the values."""
+    codes = rng.integers(0, 1 << BITS[fmt], shape).astype(np.uint8)
+    data = O.pack_codes(codes.reshape(-1, shape[-1]), BITS[fmt])
+    if scales is None:
+        sc = numbers = None
+    elif scales == "e8m0":
+        e = rng.integers(120, 124, shape[:-1] + (shape[-1] // block,)).astype(np.uint8)
+        sc, numbers = torch.from_numpy(e).to(dev).view(torch.float8_e8m0fnu), O.e8m0_decode(e)
+    else:
+        sc = torch.from_numpy(rng.random(shape[:-1] + (shape[-1] // block,)) * 0.02 + 0.005).to(scales).to(dev)
+        numbers = np64(sc)
+    w = PackedTensor(torch.from_numpy(data).to(dev), fmt, shape, sc, block)
+    flat = (int(np.prod(shape[:-1])), shape[-1])
+    values = O.dequant_f64(data, fmt, flat, None if numbers is None else numbers.reshape(flat[0], -1), block)
+    return w, np.asarray(values, np.float64).reshape(shape)
+
+
+class Layer:
+    """Experts, and their values in 64 bits."""
+
+    def __init__(self, dev, fmt, experts, hidden, ffn, scales="e8m0", block=32, seed=0):
+        rng = np.random.default_rng(seed)
+        gate_up, self.gate_up = packed(dev, rng, fmt, (experts, 2 * ffn, hidden), scales, block)
+        down, self.down = packed(dev, rng, fmt, (experts, hidden, ffn), scales, block)
+        self.e = PackedExperts(gate_up, down)
+
+    def check(self, got, x, ids, weights):
+        want, tol = X.experts(np64(x), ids.cpu().numpy(), np64(weights), self.gate_up, self.down, torch.finfo(x.dtype).eps)
+        tol = tol + torch.finfo(got.dtype).eps / 2 * (np.abs(want) + tol) + 2.0 ** -25
+        off = np.abs(np64(got) - want) - tol
+        assert not (off > 0).any(), f"{int((off > 0).sum())} of {off.size} off, by up to {off.max():.3g} over the tolerance"
+
+
+def choice(dev, seed, tokens, experts, top_k, skew=1.0):
+    """Different experts for each token, some more often than others."""
+    rng = np.random.default_rng(seed)
+    score = rng.standard_normal((tokens, experts)) + skew * rng.standard_normal(experts)
+    ids = np.argsort(-score, axis=1)[:, :top_k].astype(np.int32)
+    return torch.from_numpy(np.ascontiguousarray(ids)).to(dev), torch.from_numpy(rng.random((tokens, top_k)).astype(np.float32)).to(dev)
+
+
+FORMATS = [("fp4_e2m1", "e8m0", 32), ("fp4_e2m1", None, 32), ("fp6_e2m3", "e8m0", 32), ("fp6_e3m2", "e8m0", 32), ("fp6_e2m3", None, 32),
+           ("int4", F16, 128), ("int4", BF16, 64), ("int4", F32, 32), ("uint4", F16, 32), ("uint4", F32, 128), ("uint4", F32, 64), ("int4", None, 32)]
+
+
+@pytest.mark.parametrize("fmt,scales,block", FORMATS)
+def test_experts_of_every_format(dev, fmt, scales, block):
+    print(f"experts {fmt} {scales} {block}", flush=True)
+    layer = Layer(dev, fmt, 5, 256, 384, scales, block)
+    size = 0.02 if scales is None else 0.5
+    for tokens, top_k in ((1, 2), (7, 3), (70, 2), (150, 3), (333, 4)):
+        ids, weights = choice(dev, tokens, tokens, 5, top_k)
+        x = randn(dev, tokens, tokens, 256, dtype=layer.e.dtype, scale=size)
+        layer.check(layer.e.apply(x, ids, weights), x, ids, weights)
+
+
+@pytest.mark.parametrize("fmt,scales,block", [("fp4_e2m1", "e8m0", 32), ("int4", F16, 128)])
+@pytest.mark.parametrize("experts,hidden,ffn", [(1, 128, 128), (3, 640, 128), (8, 128, 1152), (64, 256, 256), (130, 128, 128)])
+def test_experts_of_every_size(dev, fmt, scales, block, experts, hidden, ffn):
+    print(f"experts {fmt} {experts} {hidden} {ffn}", flush=True)
+    layer = Layer(dev, fmt, experts, hidden, ffn, scales, block)
+    for tokens in (1, 2, 3, 8, 16, 17, 31, 65, 200):
+        top_k = min(experts, 1 + tokens % 8)
+        ids, weights = choice(dev, tokens, tokens, experts, top_k)
+        x = randn(dev, tokens, tokens, hidden, dtype=layer.e.dtype, scale=0.5)
+        layer.check(layer.e.apply(x, ids, weights), x, ids, weights)
+
+
+def named(rows):
+    return torch.tensor(rows, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("fmt,scales,block", [("fp4_e2m1", "e8m0", 32), ("uint4", BF16, 64)])
+@pytest.mark.parametrize("tokens", [1, 5, 40, 300])
+def test_experts_that_tokens_may_name(dev, fmt, scales, block, tokens):
+    """None at all, ids of other machines' experts, one expert for all, the same one twice; weights that are NaN where no
+    expert is named; weights of zero and below."""
+    layer = Layer(dev, fmt, 6, 256, 256, scales, block)
+    x = randn(dev, 1, tokens, 256, dtype=layer.e.dtype, scale=0.5)
+    w = randn(dev, 2, tokens, 3)
+    none = torch.full((tokens, 3), -1, dtype=torch.int32, device=dev)
+    assert torch.equal(layer.e.apply(x, none, w * float("nan")), torch.zeros_like(x))
+    for row in ([2, 2, 2], [5, -1, 5], [-7, 0, 6], [2 ** 31 - 1, -2 ** 31, 3], [0, 1, 2]):
+        ids = named([row] * tokens).to(dev)
+        ids[tokens // 2:, 0] = 4
+        ids[::3] = -1
+        clean = torch.where((ids < 0) | (ids >= 6), torch.full_like(w, float("nan")), w)
+        got = layer.e.apply(x, ids, clean)
+        layer.check(got, x, ids, torch.where(clean != clean, torch.zeros_like(w), clean))
+        assert not got[::3].any()
+
+
+def test_experts_of_views(dev):
+    layer = Layer(dev, "fp4_e2m1", 8, 256, 256)
+    ids, weights = choice(dev, 1, 50, 8, 2)
+    rows = randn(dev, 1, 50, 3, 256, dtype=BF16)
+    for x in (rows[:, 1], rows[:, 2], rows.view(150, 256)[:50], rows[0:1, 0]):
+        i, w = ids[:x.shape[0]], weights[:x.shape[0]]
+        want = layer.e.apply(x.contiguous(), i, w)
+        layer.check(want, x, i, w)
+        assert torch.equal(layer.e.apply(x, i, w), want)
+        wide = torch.zeros((x.shape[0], 2, 256 + 1), device=dev)
+        got = layer.e.apply(x, i, w, out=wide[:, 1, 1:])  # rows apart, not aligned to vectors
+        layer.check(got, x, i, w)
+        assert torch.equal(got.to(BF16), want) and not wide[:, 0].any() and not wide[:, 1, 0].any()
+        same = x.clone()
+        assert layer.e.apply(same, i, w, out=same) is same and torch.equal(same, want)
+    empty = rows.view(150, 256)[:0]
+    assert layer.e.apply(empty, ids[:0], weights[:0]).shape == (0, 256)
+
+
+@pytest.mark.parametrize("tokens", [2, 300])
+def test_experts_again_and_on_other_streams(dev, tokens):
+    """Bit for bit alike whenever and wherever they run, replays among eager work included."""
+    layer = Layer(dev, "fp4_e2m1", 8, 256, 384)
+    ids, weights = choice(dev, 1, tokens, 8, 2)
+    x = randn(dev, 1, tokens, 256, dtype=BF16)
+    want = layer.e.apply(x, ids, weights)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(layer.e.apply(x, ids, weights))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer.e.apply(x, ids, weights)
+    for seed in (5, 6, 7):
+        x.copy_(randn(dev, seed, tokens, 256, dtype=BF16))
+        new = choice(dev, seed, tokens, 8, 2)
+        ids.copy_(new[0])
+        weights.copy_(new[1])
+        want = layer.e.apply(x, ids, weights)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        layer.check(out, x, ids, weights)
+
+
+def test_routed_experts(dev):
+    """The two as a layer uses them: a router's logits, the choice, the products."""
+    layer = Layer(dev, "fp4_e2m1", 16, 256, 256)
+    for tokens in (1, 6, 100):
+        x = randn(dev, tokens, tokens, 256, dtype=BF16)
+        logits = x.float() @ randn(dev, 9, 256, 16, scale=0.1)
+        r = route(logits, 4, score="sigmoid", bias=randn(dev, 3, 16, scale=0.1), groups=4, top_groups=2)
+        ids, weights = X.route(np64(logits), 4, "sigmoid", np64(randn(dev, 3, 16, scale=0.1)), 4, 2)
+        routes(r, (ids, weights))
+        layer.check(layer.e.apply(x, r.ids, r.weights), x, r.ids, r.weights)

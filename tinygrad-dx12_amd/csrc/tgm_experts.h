@@ -1,0 +1,29 @@
+// Shared by the kernels of tgm_experts_apply: the products of many experts' rows with their own weights.
+#pragma once
+
+#include "../../include/tgm_experts.h"
+#include "tgm_gemm_w_tile.h"
+
+namespace tgm {
+
+// Tiles of the grouped products, rows x columns: what the 32, 64, 128 and 128 wide rows of kExpertTiles mean.
+struct ExpertTile {
+  int rows, cols;
+};
+constexpr ExpertTile kExpertTiles[] = {{32, 64}, {64, 64}, {64, 128}, {128, 256}};
+constexpr int kExpertTileKinds = 4;
+
+// A grouped product on tiles of kExpertTiles[shape] with `most` tile rows at most; tgm_experts_tile_{mx,i4}.hip.
+int launch_experts_tile_mx(const WGroupArgs& p, int fmt, int shape, int64_t most, hipStream_t stream);
+int launch_experts_tile_i4(const WGroupArgs& p, int64_t group, int shape, int64_t most, hipStream_t stream);
+
+template <int KIND, int FA, int WN, int WK, int NBUF>
+int launch_experts_tile(const WGroupArgs& p, int64_t most, hipStream_t stream) {
+  using T = WTile<KIND, FA, WN, WK, NBUF>;
+  static_assert(T::kFits, "tile shape");
+  const int64_t tiles = most * ((p.N + T::kBN - 1) / T::kBN);
+  hipLaunchKernelGGL((gemm_w_tile<KIND, FA, WN, WK, NBUF, WGroupArgs>), dim3((unsigned)tiles), dim3(T::kThreads), 0, stream, p);
+  return launch_status("tgm_experts_apply");
+}
+
+}  // namespace tgm

@@ -68,6 +68,7 @@ constexpr int kind_scale_bytes(int kind) { return kind & 1 ? 4 : 2; }
 constexpr int kWtK = 128;  // K step
 
 struct WTileArgs {
+  static constexpr bool kGrouped = false;
   const uint8_t* a;
   const uint8_t* w;
   const uint8_t* scales;  // E8M0 bytes [N, K / 32] or INT4 group scales [N, K / G] of dtype sdt; null = unscaled
@@ -78,6 +79,16 @@ struct WTileArgs {
   int steps_per_split;  // > 0: blockIdx.y takes that many K steps and writes its fp32 product to part [splits][M][N]
   float* part;
   int swiglu;  // rows of W interleave gate and up: C has N / 2 columns, silu(gate) * up
+};
+
+// The same product for the rows of many experts, each with a weight of its own (tgm_experts.hip): tile row tm is entry tm
+// of a list that lies on the device, the count of them before it.  M and the rows of A are those of one entry.
+struct WGroupArgs : WTileArgs {
+  static constexpr bool kGrouped = true;
+  const int* tiles;           // [0] count; from [4] on, per tile {expert, first position, positions, 0}
+  const int* rows;            // row of A at each position; null: the position itself
+  unsigned a_bytes;           // of all rows of A, where rows name them
+  int64_t w_bytes, s_bytes;   // of an expert's codes and scales
 };
 
 // 16-bit values to LDS, one zero-extended dword per lane.
@@ -173,10 +184,10 @@ struct WTile {
   static constexpr bool kFits = 8 * FA % WN == 0 && kLoads * (NBUF - 1) < 64 && kLds <= 160 * 1024;
 };
 
-template <int KIND, int FA, int WN, int WK, int NBUF>
+template <int KIND, int FA, int WN, int WK, int NBUF, class Args = WTileArgs>
 __global__ void __launch_bounds__(64 * WN * WK) 
 __attribute__((amdgpu_waves_per_eu(WTile<KIND, FA, WN, WK, NBUF>::kOccupancy, WTile<KIND, FA, WN, WK, NBUF>::kOccupancy)))
-gemm_w_tile(WTileArgs p) {
+gemm_w_tile(Args p) {
   using T = WTile<KIND, FA, WN, WK, NBUF>;
   constexpr bool I4 = T::kI4;
   constexpr int G = T::kG;
@@ -184,20 +195,42 @@ gemm_w_tile(WTileArgs p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave % WN, wk = wave / WN;
-  const int tiles_m = (p.M + T::kBM - 1) / T::kBM, tiles_n = (p.N + T::kBN - 1) / T::kBN;
+  int tiles_m = (p.M + T::kBM - 1) / T::kBM;
+  const int tiles_n = (p.N + T::kBN - 1) / T::kBN;
   int tm, tn;
+  if constexpr (Args::kGrouped) {  // the launch covers the most tiles that the rows can make
+    tiles_m = p.tiles[0];
+    if ((int)blockIdx.x >= tiles_m * tiles_n) return;
+  }
   tile_of_ranges(blockIdx.x, p.K, tiles_m, tiles_n, 8, tm, tn);
-  const int m0 = tm * T::kBM, n0 = tn * T::kBN;
+  const int n0 = tn * T::kBN;
+  int m0 = tm * T::kBM, m_end = p.M;
+  const uint8_t *pa = p.a, *pw = p.w, *ps = p.scales;
+  unsigned a_bytes = (unsigned)(p.M - 1) * p.lda_bytes + (unsigned)p.K * 2u;
+  if constexpr (Args::kGrouped) {
+    const int* entry = p.tiles + 4 + 4 * tm;
+    const int expert = __builtin_amdgcn_readfirstlane(entry[0]);
+    m0 = __builtin_amdgcn_readfirstlane(entry[1]);
+    m_end = m0 + __builtin_amdgcn_readfirstlane(entry[2]);
+    pw += expert * p.w_bytes;
+    ps += p.scales ? expert * p.s_bytes : 0;
+    if (p.rows) {
+      a_bytes = p.a_bytes;
+    } else {
+      pa += (int64_t)m0 * p.lda_bytes;
+      a_bytes = (unsigned)(m_end - m0 - 1) * p.lda_bytes + (unsigned)p.K * 2u;
+    }
+  }
   // split K (WK == 1 shapes only): steps s_begin .. of this workgroup
-  const int s_begin = WK == 1 && p.part ? (int)blockIdx.y * p.steps_per_split : 0;
-  const int nsteps = WK == 1 && p.part ? min(p.steps_per_split, p.K / kWtK - s_begin) : p.K / kWtK;
+  const int s_begin = !Args::kGrouped && WK == 1 && p.part ? (int)blockIdx.y * p.steps_per_split : 0;
+  const int nsteps = !Args::kGrouped && WK == 1 && p.part ? min(p.steps_per_split, p.K / kWtK - s_begin) : p.K / kWtK;
   const int nstages = (nsteps + WK - 1) / WK;
   const unsigned kbw = (unsigned)p.K / 8u * (T::kRow == 64 ? 4u : 6u);  // packed bytes per W row
-  const i32x4v ra = buffer_rsrc(p.a, (unsigned)(p.M - 1) * p.lda_bytes + (unsigned)p.K * 2u);
-  const i32x4v rw = buffer_rsrc(p.w, (unsigned)p.N * kbw);
+  const i32x4v ra = buffer_rsrc(pa, a_bytes);
+  const i32x4v rw = buffer_rsrc(pw, (unsigned)p.N * kbw);
   constexpr unsigned ssize = (unsigned)kind_scale_bytes(KIND);                   // INT4 scale bytes
   const unsigned srow = I4 ? (G ? (unsigned)(p.K / (G ? G : 1)) * ssize : 0u) : (unsigned)p.K / 32u;  // scale bytes per W row
-  const i32x4v rs = buffer_rsrc(p.scales, p.scales ? (unsigned)p.N * srow : 0u);
+  const i32x4v rs = buffer_rsrc(ps, p.scales ? (unsigned)p.N * srow : 0u);
   const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
 
   // Loads: the WN waves of K group wk fill the panels of its step.  A instruction i = wn + WN q covers
@@ -207,7 +240,12 @@ gemm_w_tile(WTileArgs p) {
 #pragma unroll
   for (int q = 0; q < T::kLoadsA; ++q) {
     const int row = 4 * (wn + WN * q) + (lane >> 4);
-    voa[q] = (unsigned)(m0 + row) * p.lda_bytes + (unsigned)(((lane & 15) ^ (row & 15)) * 16 + wk * kWtK * 2);
+    unsigned at = (unsigned)(m0 + row) * p.lda_bytes;
+    if constexpr (Args::kGrouped) {  // past the entry's rows: past A, which the host keeps below 2 GiB
+      at = 0xC0000000u;
+      if (row < m_end - m0) at = (unsigned)(p.rows ? p.rows[m0 + row] : row) * p.lda_bytes;
+    }
+    voa[q] = at + (unsigned)(((lane & 15) ^ (row & 15)) * 16 + wk * kWtK * 2);
   }
 #pragma unroll
   for (int q = 0; q < T::kLoadsW; ++q) {
@@ -419,12 +457,12 @@ gemm_w_tile(WTileArgs p) {
   float* ep = parts + (WK - 1) * WN * FA * 1024 + wn * 32 * 36;
 #pragma unroll
   for (int t = 0; t < FA; ++t) {
-    if (WK == 1 && p.part)
+    if (!Args::kGrouped && WK == 1 && p.part)
       store_tile32(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, p.M, p.N, p.part + (int64_t)blockIdx.y * p.M * p.N, TGM_F32,
                    p.N);
-    else if (!I4 && p.swiglu)
-      store_tile32_swiglu(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, p.M, p.N, p.c, p.cdt, p.ldc);
-    else store_tile32(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, p.M, p.N, p.c, p.cdt, p.ldc);
+    else if ((!I4 || Args::kGrouped) && p.swiglu)
+      store_tile32_swiglu(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, m_end, p.N, p.c, p.cdt, p.ldc);
+    else store_tile32(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, m_end, p.N, p.c, p.cdt, p.ldc);
   }
 }
 

@@ -14,10 +14,12 @@ Results and workspaces come from torch's caching allocator: to replay calls as a
 from __future__ import annotations
 
 import math
+import struct
 from typing import NamedTuple
 
 import torch
 
+from tinygrad_mi355x.codegen.decomp.mi355x import MX_FORMATS, PackedTensor
 from tinygrad_mi355x.rotary import _DT, Plans
 from tinygrad_mi355x.runtime import kernels as K
 
@@ -89,3 +91,111 @@ def _route_plan(sig, logits, top_k, score, bias, groups, top_groups, renormalize
     head = (_DT[logits.dtype], tokens, experts, max(logits.stride(0), experts))
     return _plans.keep(sig, ((SCORES[score], groups, top_groups, top_k, bool(renormalize), float(scale)), head,
                              (tokens, top_k), logits.get_device()))
+
+
+class PackedExperts:
+    """The feed-forward blocks of a layer's experts on packed weights: gate_up [experts, 2 ffn, hidden], gate (2 i) and up
+    (2 i + 1) rows in turn as in ``DecoderWeights``, and down [experts, hidden, ffn].
+
+    Both of one format, hidden and ffn multiples of 128: fp4_e2m1, fp6_e2m3 or fp6_e3m2 with E8M0 scales per 32 values (or
+    none) for bfloat16 activations; int4 or uint4 with float16, bfloat16 or float32 scales per 32, 64 or 128 (or none) for
+    float16 ones.
+    """
+
+    def __init__(self, gate_up: PackedTensor, down: PackedTensor) -> None:
+        for w, name in ((gate_up, "gate_up"), (down, "down")):
+            if not isinstance(w, PackedTensor) or len(w.shape) != 3:
+                raise ValueError(f"{name} must be a PackedTensor [experts, rows, columns]")
+        self.experts, rows, self.hidden = gate_up.shape
+        self.ffn = rows // 2
+        if rows % 2 or down.shape != (self.experts, self.hidden, self.ffn):
+            raise ValueError(f"down must be [{self.experts}, {self.hidden}, {rows / 2:g}] beside gate_up {gate_up.shape}, got {down.shape}")
+        if not 1 <= self.experts <= MAX_EXPERTS:
+            raise ValueError(f"a layer holds 1 to {MAX_EXPERTS} experts, got {self.experts}")
+        if not self.hidden or not self.ffn or self.hidden % 128 or self.ffn % 128:
+            raise ValueError(f"hidden and ffn must be multiples of 128, got {self.hidden} and {self.ffn}")
+        if gate_up.format != down.format or _scales(gate_up) != _scales(down) or gate_up.device != down.device:
+            raise ValueError("gate_up and down must be of one format, with scales of one type and block, on one device")
+        integer = gate_up.format not in MX_FORMATS
+        if gate_up.scales is not None:
+            dt, block = _scales(gate_up)
+            if integer and (dt not in _DT or block not in (32, 64, 128)):
+                raise ValueError(f"{gate_up.format} experts take float16, bfloat16 or float32 scales per 32, 64 or 128 values, got "
+                                 f"{dt} per {block}")
+            if not integer and (dt is not torch.float8_e8m0fnu or block != 32):
+                raise ValueError(f"{gate_up.format} experts take E8M0 scales per 32 values, got {dt} per {block}")
+        for w, name in ((gate_up, "gate_up"), (down, "down")):
+            if not w.data.is_contiguous() or w.scales is not None and not w.scales.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+            if w.data.data_ptr() % 16 or w.scales is not None and w.scales.data_ptr() % 4:
+                raise ValueError(f"codes of {name} must be 16-byte and scales 4-byte aligned")
+        self.gate_up, self.down, self.device = gate_up, down, gate_up.device
+        self.dtype = torch.float16 if integer else torch.bfloat16  # of the activations
+        dt, block = _scales(gate_up)
+        # struct tgm_experts; the weights are never replaced
+        self._arg = struct.pack("PPPPqqqqqq", gate_up.data.data_ptr(), K.ptr(gate_up.scales) or 0, down.data.data_ptr(),
+                                K.ptr(down.scales) or 0, self.experts, self.hidden, self.ffn, K.FORMAT_IDS[gate_up.format],
+                                -1 if dt is None else K.dtype_id(dt), block)
+        self._plans = Plans()
+
+    def apply(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The weighted sum of each token's experts: x [tokens, hidden] of ``dtype``, ids (int32) and weights (float32)
+        [tokens, top_k] as ``route`` gives them.
+
+        ``out`` [tokens, hidden] is of x's type or float32 (x's type), with contiguous rows; it may be x.  An id outside
+        0 .. experts - 1 names no expert and adds nothing, whatever its weight: a row without any is zero.  The same expert
+        may be named twice.  Products and sums are float32; silu(gate) * up is rounded to x's type before the down product.
+        """
+        sig = (x.shape, x.stride(), x.dtype, x.get_device(), ids.shape, ids.stride(), ids.dtype, ids.get_device(), weights.shape,
+               weights.stride(), weights.dtype, weights.get_device())
+        if out is not None:
+            sig += (out.shape, out.stride(), out.dtype, out.get_device())
+        plan = self._plans.get(sig)
+        if plan is None:
+            plan = self._apply_plan(sig, x, ids, weights, out)
+        head, top_k, tail, need, index = plan
+        if out is None:
+            out = x.new_empty(x.shape)
+        if x.shape[0]:
+            # the workspace is of the caching allocator, so that calls on several streams never share one; held until the
+            # launches, or another thread's call on this stream could be given its memory before them
+            workspace = x.new_empty(need, dtype=torch.uint8)
+            K.call("tgm_experts_apply", self._arg, x.data_ptr(), *head, ids.data_ptr(), weights.data_ptr(), top_k,
+                   out.data_ptr(), *tail, workspace.data_ptr(), need, K.stream_on(index))
+        return out
+
+    def _apply_plan(self, sig, x, ids, weights, out) -> tuple:
+        _check_rows(x, "x", self.hidden)
+        if x.dtype is not self.dtype:
+            raise ValueError(f"x must be {self.dtype} beside {self.gate_up.format} experts, got {x.dtype}")
+        tokens = x.shape[0]
+        if ids.dtype is not torch.int32 or ids.dim() != 2 or ids.shape[0] != tokens or ids.shape[1] < 1 or not ids.is_contiguous():
+            raise ValueError(f"ids must be contiguous int32 [{tokens}, top_k], got {ids.dtype} {tuple(ids.shape)}")
+        if weights.dtype is not torch.float32 or weights.shape != ids.shape or not weights.is_contiguous():
+            raise ValueError(f"weights must be contiguous float32 {tuple(ids.shape)}, got {weights.dtype} {tuple(weights.shape)}")
+        ldy, odt = self.hidden, x.dtype
+        if out is not None:
+            _check_rows(out, "out", self.hidden)
+            if out.shape != x.shape or out.dtype not in (x.dtype, torch.float32):
+                raise ValueError(f"out must be {x.dtype} or float32 {tuple(x.shape)}, got {out.dtype} {tuple(out.shape)}")
+            ldy, odt = max(out.stride(0), self.hidden), out.dtype
+        for t, name in ((x, "x"), (ids, "ids"), (weights, "weights"), (out, "out")):
+            if t is not None and t.device != self.device:
+                raise ValueError(f"{name} is on {t.device}, the experts on {self.device}")
+        ldx = max(x.stride(0), self.hidden)
+        if ldx % 8 and tokens > 1:
+            raise ValueError(f"rows of x must be 16-byte aligned, got a stride of {ldx}")
+        K.require_device(x)
+        need = K.load_library().tgm_experts_workspace(self._arg, tokens, ids.shape[1])
+        return self._plans.keep(sig, ((_DT[x.dtype], tokens, ldx), ids.shape[1], (_DT[odt], ldy), need, x.get_device()))
+
+
+def _scales(w: PackedTensor) -> tuple:
+    return (None, 32) if w.scales is None else (w.scales.dtype, w.block_size)
+
+
+def _check_rows(t: torch.Tensor, name: str, hidden: int) -> None:
+    if t.dim() != 2 or t.shape[1] != hidden:
+        raise ValueError(f"{name} must be [tokens, {hidden}], got {tuple(t.shape)}")
+    if t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < hidden:
+        raise ValueError(f"rows of {name} must be contiguous and apart")
