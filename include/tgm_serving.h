@@ -1,7 +1,7 @@
 /*
  * Serving operators between a decoder's matrix products (libtgm_mi355x.so): rotary positions, a
  * quantised paged key/value cache (write, read, attention over it, attention of a batch that
- * shares a prefix) and token sampling.
+ * shares a prefix), token sampling and log probabilities.
  *
  * The reference has no model code; these are what a serving loop around its packed matmul
  * (alexandreteles/tinygrad-dx12 src/tinygrad_dx12/codegen/decomp/dx12.py:108-112) needs next
@@ -116,6 +116,18 @@ int64_t tgm_sample_workspace(int64_t rows, int64_t vocab, int64_t dtype);
 int tgm_sample(const void* logits, int64_t dtype, int64_t rows, int64_t vocab, int64_t ld, const float* u,
                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens,
                void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Log probabilities of one given token per row of logits [rows, vocab] (row stride ld), natural logarithms in 32 bits:
+ *   logprobs[r]  of tokens[r];  ranks[r]  how many tokens come before it by falling logit, equal ones by index
+ *   entropy[r]   of the row's distribution;  top_ids, top_logprobs [rows, top]  the likeliest tokens, the first first
+ * top is 0 to 64 (top_ids and top_logprobs may be NULL for 0), at most vocab.  A token outside the vocabulary names none: its
+ * logprob is 0 and its rank -1.  A row with a NaN or +infinity, or of -infinities alone, has NaN probabilities and
+ * entropy; NaN ranks behind everything.
+ * workspace: tgm_log_probs_workspace() bytes, 16-byte aligned (NULL when 0). */
+int64_t tgm_log_probs_workspace(int64_t rows, int64_t vocab, int64_t dtype, int64_t top);
+int tgm_log_probs(const void* logits, int64_t dtype, int64_t rows, int64_t vocab, int64_t ld, const int32_t* tokens,
+                  int64_t top, float* logprobs, int32_t* ranks, float* entropy, int32_t* top_ids, float* top_logprobs,
+                  void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -62,3 +62,21 @@ def experts(x, ids, weights, gate_up, down, eps):
         np.add.at(y, t, weights[t, j][:, None] * (h @ down[e].T))
         np.add.at(tol, t, w * ((eh * (1 + f * unit) + (f + ids.shape[1] + 1) * unit * np.abs(h)) @ np.abs(down[e]).T))
     return y, tol
+
+
+def log_probs(logits, tokens, top):
+    """logprobs, ranks, entropy, top_ids and top_logprobs of logits [rows, vocab]."""
+    rows, n = logits.shape
+    got = np.zeros(rows), np.full(rows, -1), np.zeros(rows), np.zeros((rows, top), np.int64), np.zeros((rows, top))
+    with np.errstate(all="ignore"):
+        for r in range(rows):
+            x = logits[r].astype(np.float64)
+            m = x.max()
+            p = np.exp(x - m) / np.exp(x - m).sum()
+            logp = (x - m) - np.log(np.exp(x - m).sum())
+            got[2][r] = -np.where(p == 0, 0.0, p * logp).sum()
+            order = np.lexsort((np.arange(n), -np.where(x != x, -np.inf, x), x != x))
+            got[3][r], got[4][r] = order[:top], logp[order[:top]]
+            if 0 <= tokens[r] < n:
+                got[0][r], got[1][r] = logp[tokens[r]], (x > x[tokens[r]]).sum() + (x[:tokens[r]] == x[tokens[r]]).sum()
+    return got

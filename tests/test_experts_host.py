@@ -1,4 +1,4 @@
-"""Refusals of the mixture-of-experts operators: no GPU needed."""
+"""Refusals of the mixture-of-experts operators and of log probabilities: no GPU needed."""
 
 import struct
 
@@ -8,6 +8,7 @@ import torch
 from tinygrad_mi355x.codegen.decomp.mi355x import PackedTensor
 from tinygrad_mi355x.experts import PackedExperts, route
 from tinygrad_mi355x.runtime import kernels as K
+from tinygrad_mi355x.sampling import log_probs
 
 
 # ----------------------------------------------------------------------------- routing
@@ -141,3 +142,35 @@ def test_experts_workspace_of_no_tokens_and_of_more():
     assert lib.tgm_experts_workspace(experts_arg(), 0, 2) == 0
     few, more = (lib.tgm_experts_workspace(experts_arg(), t, 2) for t in (4, 4000))
     assert few >= 8 * (384 * 2 + 256 * 4) and more >= 8000 * (384 * 2 + 256 * 4)
+
+
+# ----------------------------------------------------------------------------- log probabilities
+@pytest.mark.parametrize("logits,tokens,top", [
+    (torch.zeros(8), torch.zeros(8, dtype=I32), 0), (torch.zeros(4, 8, dtype=torch.float64), torch.zeros(4, dtype=I32), 0),
+    (torch.zeros(4, 0), torch.zeros(4, dtype=I32), 0), (torch.zeros(1, (1 << 20) + 1), torch.zeros(1, dtype=I32), 0),
+    (torch.zeros(8, 4).t(), torch.zeros(4, dtype=I32), 0), (torch.zeros(1, 8).expand(4, 8), torch.zeros(4, dtype=I32), 0),
+    (torch.zeros(4, 8), torch.zeros(3, dtype=I32), 0), (torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64), 0),
+    (torch.zeros(4, 8), torch.zeros(8, dtype=I32)[::2], 0), (torch.zeros(4, 8), 3, 0), (torch.zeros(4, 8), torch.zeros(4, 1, dtype=I32), 0),
+    (torch.zeros(4, 8), torch.zeros(4, dtype=I32, device="meta"), 0), (torch.zeros(4, 8), torch.zeros(4, dtype=I32), 9),
+    (torch.zeros(4, 100), torch.zeros(4, dtype=I32), 65), (torch.zeros(4, 8), torch.zeros(4, dtype=I32), -1),
+    (torch.zeros(4, 8), torch.zeros(4, dtype=I32), 2.0)])
+def test_log_probs_refuses(logits, tokens, top):
+    with pytest.raises(ValueError):
+        log_probs(logits, tokens, top=top)
+
+
+def test_log_probs_needs_the_device():
+    with pytest.raises(RuntimeError):
+        log_probs(torch.zeros(4, 8), torch.zeros(4, dtype=I32), top=2)
+
+
+@pytest.mark.parametrize("args", [
+    (4096, 9, 4, 8, 8, 4096, 2, 4096, 4096, 4096, 4096, 4096, None, 0), (4096, 13, -1, 8, 8, 4096, 2, 4096, 4096, 4096, 4096, 4096, None, 0),
+    (4096, 13, 4, 0, 8, 4096, 0, 4096, 4096, 4096, 4096, 4096, None, 0), (4096, 13, 4, 8, 7, 4096, 2, 4096, 4096, 4096, 4096, 4096, None, 0),
+    (4096, 13, 4, 8, 8, 4096, 9, 4096, 4096, 4096, 4096, 4096, None, 0), (4096, 13, 4, 100, 100, 4096, 65, 4096, 4096, 4096, 4096, 4096, None, 0),
+    (None, 13, 4, 8, 8, 4096, 2, 4096, 4096, 4096, 4096, 4096, None, 0), (4096, 13, 4, 8, 8, 4096, 2, 4096, 4096, 4096, None, 4096, None, 0),
+    (4098, 13, 4, 8, 8, 4096, 2, 4096, 4096, 4096, 4096, 4096, None, 0),
+    (4096, 13, 4, 200000, 200000, 4096, 2, 4096, 4096, 4096, 4096, 4096, None, 0)])
+def test_log_probs_entry_point_refuses(args):
+    with pytest.raises(ValueError):
+        K.call("tgm_log_probs", *args, None)

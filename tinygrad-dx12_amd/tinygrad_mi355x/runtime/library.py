@@ -94,13 +94,14 @@ SIGNATURES = {
     "tgm_kv_read": (_P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _INT, _P),
     "tgm_kv_attend": (_P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _I64, ctypes.c_double, _P, _I64, _P, _P),
     "tgm_sample": (_P, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P),
+    "tgm_log_probs": (_P, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _P),
     # mixture-of-experts operators (include/tgm_experts.h)
     "tgm_route": (_P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, ctypes.c_double, _P, _P, _P),
     "tgm_experts_apply": (_P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _P, _I64, _P),
 }
 EXPORTS = ("tgm_abi_version", "tgm_last_error", "tgm_dec_attention_workspace", "tgm_gemm_w_split_workspace",
            "tgm_gemm_w_split_noalloc_capacity", "tgm_kv_attend_workspace", "tgm_sample_workspace",
-           "tgm_experts_workspace", *SIGNATURES)
+           "tgm_experts_workspace", "tgm_log_probs_workspace", *SIGNATURES)
 
 
 def library_path() -> Path:
@@ -140,6 +141,8 @@ def load_library() -> ctypes.CDLL:
         lib.tgm_kv_attend_workspace.restype = _I64
         lib.tgm_sample_workspace.argtypes = (_I64, _I64, _I64)
         lib.tgm_sample_workspace.restype = _I64
+        lib.tgm_log_probs_workspace.argtypes = (_I64, _I64, _I64, _I64)
+        lib.tgm_log_probs_workspace.restype = _I64
         lib.tgm_experts_workspace.argtypes = (_P, _I64, _I64)
         lib.tgm_experts_workspace.restype = _I64
         _lib = lib

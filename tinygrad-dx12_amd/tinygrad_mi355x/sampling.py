@@ -1,4 +1,4 @@
-"""Token sampling from logits with given random numbers (include/tgm_serving.h).
+"""Token sampling from logits with given random numbers, and log probabilities (include/tgm_serving.h).
 
 The reference has no model code; this serves models around its packed matmul
 (alexandreteles/tinygrad-dx12 src/tinygrad_dx12/codegen/decomp/dx12.py:108-112).
@@ -6,12 +6,14 @@ The reference has no model code; this serves models around its packed matmul
 
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from tinygrad_mi355x.rotary import _DT, Plans
 from tinygrad_mi355x.runtime import kernels as K
 
-MAX_VOCAB = 1 << 20
+MAX_VOCAB, MAX_TOP = 1 << 20, 64
 _plans = Plans()
 
 
@@ -63,14 +65,7 @@ def _filled(value, rows: int, dtype: torch.dtype, device: torch.device):
 
 
 def _plan(sig, logits, u, temperature, top_k, top_p, min_p) -> tuple:
-    if logits.dim() != 2 or logits.dtype not in _DT:
-        raise ValueError(f"logits must be float32, float16 or bfloat16 [rows, vocab], got {logits.dtype} "
-                         f"{tuple(logits.shape)}")
-    rows, vocab = logits.shape
-    if not 1 <= vocab <= MAX_VOCAB:
-        raise ValueError(f"the vocabulary must hold 1 to {MAX_VOCAB} tokens, got {vocab}")
-    if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
-        raise ValueError("rows of logits must be contiguous and apart")
+    rows, vocab, ld = _check_logits(logits)
     if not isinstance(u, torch.Tensor):
         raise ValueError("u must be a tensor: one random number per row")
     numbers = False
@@ -88,7 +83,20 @@ def _plan(sig, logits, u, temperature, top_k, top_p, min_p) -> tuple:
     K.require_device(logits)
     dt = _DT[logits.dtype]
     need = K.load_library().tgm_sample_workspace(rows, vocab, dt)
-    return _plans.keep(sig, (dt, rows, vocab, max(logits.stride(0), vocab), need, logits.get_device(), numbers))
+    return _plans.keep(sig, (dt, rows, vocab, ld, need, logits.get_device(), numbers))
+
+
+def _check_logits(logits: torch.Tensor) -> tuple[int, int, int]:
+    """Rows, tokens of the vocabulary, and the row stride."""
+    if logits.dim() != 2 or logits.dtype not in _DT:
+        raise ValueError(f"logits must be float32, float16 or bfloat16 [rows, vocab], got {logits.dtype} "
+                         f"{tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    if not 1 <= vocab <= MAX_VOCAB:
+        raise ValueError(f"the vocabulary must hold 1 to {MAX_VOCAB} tokens, got {vocab}")
+    if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
+        raise ValueError("rows of logits must be contiguous and apart")
+    return rows, vocab, max(logits.stride(0), vocab)
 
 
 def _per_row(t: torch.Tensor, name: str, rows: int, dtype: torch.dtype, device: torch.device) -> None:
@@ -96,3 +104,51 @@ def _per_row(t: torch.Tensor, name: str, rows: int, dtype: torch.dtype, device: 
         raise ValueError(f"{name} must be a number or contiguous {dtype} [{rows}], got {t.dtype} {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+class LogProbs(NamedTuple):
+    """What ``log_probs`` returns, [rows] and [rows, top]."""
+    logprobs: torch.Tensor
+    ranks: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> LogProbs:
+    """Log probabilities (natural, float32) of one token (int32 [rows]) per row of logits [rows, vocab].
+
+    Beside ``logprobs``: ``ranks`` (int32), how many tokens come before it by falling logit, equal ones by index;
+    ``entropy`` (float32) of the row's distribution; ``top_ids`` (int32) and ``top_logprobs``, the ``top`` likeliest tokens
+    (0 to 64), the first first.  A token outside the vocabulary, such as a padded row's -1, names none: its logprob is 0
+    and its rank -1.  A row with a NaN or +infinity, or of -infinities alone, has NaN probabilities and entropy; NaN
+    ranks behind everything.
+    """
+    sig = ("log_probs", logits.shape, logits.stride(), logits.dtype, logits.get_device(), _signature(tokens), top)
+    plan = _plans.get(sig)
+    if plan is None:
+        plan = _log_probs_plan(sig, logits, tokens, top)
+    head, rows, need, index = plan
+    numbers = logits.new_empty((2, rows), dtype=torch.float32)
+    ranks = logits.new_empty(rows, dtype=torch.int32)
+    top_ids, top_logprobs = logits.new_empty((rows, top), dtype=torch.int32), logits.new_empty((rows, top), dtype=torch.float32)
+    # of the caching allocator and held until the launch, as in sample
+    workspace = logits.new_empty(need, dtype=torch.uint8) if need else None
+    got = LogProbs(numbers[0], ranks, numbers[1], top_ids, top_logprobs)
+    if rows:
+        K.call("tgm_log_probs", logits.data_ptr(), *head, tokens.data_ptr(), top, got.logprobs.data_ptr(), ranks.data_ptr(),
+               got.entropy.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(), K.ptr(workspace), need, K.stream_on(index))
+    return got
+
+
+def _log_probs_plan(sig, logits, tokens, top) -> tuple:
+    rows, vocab, ld = _check_logits(logits)
+    if not isinstance(tokens, torch.Tensor):
+        raise ValueError("tokens must be a tensor: one token per row")
+    _per_row(tokens, "tokens", rows, torch.int32, logits.device)
+    if not isinstance(top, int) or not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}, got {top}")
+    K.require_device(logits)
+    dt = _DT[logits.dtype]
+    need = K.load_library().tgm_log_probs_workspace(rows, vocab, dt, top)
+    return _plans.keep(sig, ((dt, rows, vocab, ld), rows, need, logits.get_device()))
