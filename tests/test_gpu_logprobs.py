@@ -141,3 +141,16 @@ def test_log_probs_of_sampled_tokens(dev):
     assert not got.ranks.any() and torch.equal(got.top_logprobs[:, 0], got.logprobs)
     got = check(logits, sample(logits, u, top_k=7), 7)
     assert int(got.ranks.max()) < 7
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_ranks_of_tokens_that_are_ruled_out(dev, dtype):
+    """-infinity ranks by index behind what is finite, in rows of every alignment, of one stretch and of several."""
+    for vocab in (40, 32001, 66000):
+        flat = torch.zeros(vocab + 16, dtype=dtype, device=dev)
+        for off in (0, 1, 5, 7):
+            x = flat[off:off + vocab].view(1, vocab)
+            x.copy_(randn(dev, off, 1, vocab, dtype=dtype))
+            x[0, ::3] = -float("inf")
+            for token in (0, 3, 9, 36, vocab - 1 - (vocab - 1) % 3):
+                check(x, torch.tensor([token], dtype=torch.int32, device=dev), 5)

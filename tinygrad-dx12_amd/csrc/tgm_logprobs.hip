@@ -4,7 +4,7 @@
 //
 //   log p_i = d_i - log S        entropy = -sum p_i log p_i = log S - T / S
 //
-// A workgroup reads a stretch of a row into registers, 32 logits a thread, and everything else comes from there: the
+// A workgroup reads a stretch of a row into registers, 32 logits a thread (64 of 16 bits where there are many rows), and everything else comes from there: the
 // largest, then S, T and the token's rank, then the likeliest tokens.  Those are looked for among the logits that reach a
 // bound which enough of them are sure to reach: the n-th largest of the waves' largest logits, or, with more tokens than
 // waves, the least over the waves of their q-th largest thread's.  Of independent logits a few dozen reach it; they are
@@ -21,7 +21,7 @@
 
 namespace tgm {
 
-constexpr int kLpMost = 1024, kLpEach = 32, kLpTop = 64, kLpList = 512, kLpJoin = 256;
+constexpr int kLpMost = 1024, kLpTop = 64, kLpList = 512, kLpJoin = 256;
 typedef unsigned long long lp_u64;
 typedef unsigned lp_u32x4 __attribute__((ext_vector_type(4)));
 
@@ -88,11 +88,31 @@ __device__ __forceinline__ float lp_load(const void* p, int64_t i) {
   else return (float)((const _Float16*)p)[i];
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kLpMost) logprob_rows(LpArgs a) {
-  constexpr int SIZE = DT == TGM_F32 ? 4 : 2, VEC = 16 / SIZE, NV = kLpEach / VEC;
-  __shared__ float wave_a[16], wave_b[16], wave_c[16];
-  __shared__ int wave_i[16];
+// Reductions over the 16 lanes of a row, in every lane.
+__device__ __forceinline__ float lp_row_max(float v) {
+  v = fmaxf(v, xor1(v));
+  v = fmaxf(v, xor2(v));
+  v = fmaxf(v, xor4(v));
+  return fmaxf(v, xor8(v));
+}
+__device__ __forceinline__ float lp_row_sum(float v) {
+  v += xor1(v);
+  v += xor2(v);
+  v += xor4(v);
+  return v + xor8(v);
+}
+// How many of the 16 lanes of a row hold more than v.
+template <int K = 1>
+__device__ __forceinline__ int lp_row_above(float v) {
+  if constexpr (K < 16) return (dpp<0x120 + K>(v) > v) + lp_row_above<K + 1>(v);  // rotated by K lanes
+  else return 0;
+}
+
+// Waves of 64 registers, eight on a SIMD: a row's loads go under others' arithmetic.
+template <int DT, int EACH>
+__global__ void __launch_bounds__(32 * kLpMost / EACH) __attribute__((amdgpu_waves_per_eu(8, 8))) logprob_rows(LpArgs a) {
+  constexpr int SIZE = DT == TGM_F32 ? 4 : 2, VEC = 16 / SIZE, NV = EACH / VEC;
+  __shared__ float wave_max[16], wave_reach[16], wave_sum[16], wave_dot[16], wave_rank[16];
   __shared__ lp_u64 list[kLpList];
   __shared__ lp_u64 best[16];
   __shared__ int listed;
@@ -100,35 +120,46 @@ __global__ void __launch_bounds__(kLpMost) logprob_rows(LpArgs a) {
   const int64_t row = blockIdx.x / a.stretches;
   const int stretch = blockIdx.x % a.stretches;
   const char* base = (const char*)a.logits + row * a.ld * SIZE;
-  const int tok = a.tokens[row];
-  const bool named = (unsigned)tok < (unsigned)a.n;
-  const float at = named ? lp_load<DT>(base, tok) : 0.0f;
   // whole aligned vectors: the first may begin before the row and the last end behind it, in its 16 bytes
   const int shift = (int)((uintptr_t)base % 16) / SIZE;
   const lp_u32x4* vectors = (const lp_u32x4*)(base - shift * SIZE);
   const int count = (a.n + shift + VEC - 1) / VEC;
   const int v0 = stretch * (int)blockDim.x * NV + (int)threadIdx.x;
+  constexpr unsigned NONE = DT == TGM_F32 ? 0xFF800000u : DT == TGM_BF16 ? 0xFF80FF80u : 0xFC00FC00u;  // -infinity
   lp_u32x4 raw[NV];
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
     const int v = v0 + q * (int)blockDim.x;
-    raw[q] = v < count ? __builtin_nontemporal_load(vectors + v) : lp_u32x4{};
+    raw[q] = v < count ? __builtin_nontemporal_load(vectors + v) : lp_u32x4{NONE, NONE, NONE, NONE};
   }
-  auto index = [&](int r) __attribute__((always_inline)) { return (v0 + r / VEC * (int)blockDim.x) * VEC - shift + r % VEC; };
-  auto raw_value = [&](int r) __attribute__((always_inline)) {
+  const int tok = a.tokens[row];
+  const bool named = (unsigned)tok < (unsigned)a.n;
+  const float at = named ? lp_load<DT>(base, tok) : 0.0f;
+  auto value = [&](int r) __attribute__((always_inline)) {
     const lp_u32x4 v = raw[r / VEC];
     if constexpr (DT == TGM_F32) return bits_f32(v[r % VEC]);
     const unsigned pair = v[r % VEC / 2];
     if constexpr (DT == TGM_BF16) return bits_f32(r % 2 ? pair & 0xFFFF0000u : pair << 16);
     return (float)__builtin_bit_cast(_Float16, (unsigned short)(r % 2 ? pair >> 16 : pair));
   };
-  // -infinity where there is no element
-  float x[kLpEach];
+  // the first and the last vector: -infinity where there is no element
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    const int v = v0 + q * (int)blockDim.x;
+    if (v == 0 || v == count - 1) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        constexpr int PER = 4 / SIZE;
+        const unsigned mask = DT == TGM_F32 ? ~0u : i % 2 ? 0xFFFF0000u : 0xFFFFu;
+        if ((unsigned)(v * VEC - shift + i) >= (unsigned)a.n) raw[q][i / PER] = (raw[q][i / PER] & ~mask) | (NONE & mask);
+      }
+    }
+  }
   float top = -INFINITY;
 #pragma unroll
-  for (int r = 0; r < kLpEach; ++r) {
-    x[r] = (unsigned)index(r) < (unsigned)a.n ? raw_value(r) : -INFINITY;
-    top = fmaxf(top, x[r]);
+  for (int r = 0; r < EACH; ++r) {
+    top = fmaxf(top, value(r));
+    if (r % 8 == 7) __builtin_amdgcn_sched_barrier(0);
   }
   // the stretch's largest, and a bound that `top` logits reach
   if (threadIdx.x == 0) listed = 0;
@@ -144,48 +175,79 @@ __global__ void __launch_bounds__(kLpMost) logprob_rows(LpArgs a) {
       left = holds && lane == __builtin_ctzll(holds) ? -INFINITY : left;
     }
   }
-  if (lane == 0) wave_a[wave] = wave_top, wave_b[wave] = reach;
+  if (lane == 0) wave_max[wave] = wave_top, wave_reach[wave] = reach;
   __syncthreads();
-  float max = -INFINITY, bound = INFINITY;
-  for (int w = 0; w < waves; ++w) {
-    const float t = wave_a[w];
-    max = fmaxf(max, t);
-    if (a.top > waves) {
-      bound = fminf(bound, wave_b[w]);
-    } else {  // the top-th largest
-      int before = 0;
-      for (int o = 0; o < waves; ++o) before += wave_a[o] > t || (wave_a[o] == t && o < w);
-      bound = before == a.top - 1 ? t : bound;
-    }
-  }
+  const int w16 = lane & 15;
+  const float each_max = w16 < waves ? wave_max[w16] : -INFINITY;
+  const float max = lp_row_max(each_max);
+  float bound;
+  if (a.top > waves) bound = -lp_row_max(w16 < waves ? -wave_reach[w16] : -INFINITY);
+  else bound = -lp_row_max(lp_row_above(each_max) < a.top ? -each_max : -INFINITY);
   const float zero = max == -INFINITY ? 0.0f : max;
-  float sum = 0.0f, dot = 0.0f;
-  int rank = 0;
+  // unpacked anew: kept from one pass to the next, the values would not fit the registers
 #pragma unroll
-  for (int r = 0; r < kLpEach; ++r) {
-    const float d = x[r] - zero;
-    const float e = __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
-    sum += e;
-    dot = __builtin_fmaf(e, fmaxf(d, -1000.0f), dot);  // nothing times infinity adds nothing
-    rank += x[r] > at || (x[r] == at && (unsigned)index(r) < (unsigned)tok);
-  }
+  for (int q = 0; q < NV; ++q) asm volatile("" : "+v"(raw[q]));
+  // The rank counts equal logits before the token: vectors before its own compare with the next number below it (NaN below
+  // -infinity, where all of them count), its own vector's are counted at the end.
+  int rank = 0;
+  const float below = at == 0.0f ? -bits_f32(1u) : bits_f32(f32_bits(at) + (at > 0.0f ? -1 : 1));
+  // exp(x - m) = 2^(x L - m L), L = log2 e.  With m L in two parts, of which the second is left out of every term, one
+  // fused step gives an exponent that is off by its own rounding alone; from 2^20 on the second part is not small, and the
+  // difference comes first.
+  constexpr float L = 1.44269504088896340736f;
+  const float zero_l = zero * L, low = fabsf(zero) < 0x1p20f ? __builtin_fmaf(zero, L, -zero_l) : 0.0f;
+  float sum = 0.0f, dot = 0.0f;
+  auto pass = [&](auto exponent) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      const float over = (v0 + q * (int)blockDim.x + 1) * VEC - shift <= tok ? below : at;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float x = value(q * VEC + i);
+        const float d = exponent(x);
+        const float e = __builtin_amdgcn_exp2f(d);
+        sum += e;
+        dot = __builtin_fmaf(e, fmaxf(d, -1000.0f), dot);  // nothing times infinity adds nothing
+        rank += __builtin_popcountll(__ballot(!(x <= over)));
+      }
+      __builtin_amdgcn_sched_barrier(0);  // ahead of its vector's turn, an unpacked value takes a register
+    }
+  };
+  if (fabsf(zero) < 0x1p20f) pass([&](float x) __attribute__((always_inline)) { return __builtin_fmaf(x, L, -zero_l); });
+  else pass([&](float x) __attribute__((always_inline)) { return (x - zero) * L; });
   sum = lp_wave_sum(sum), dot = lp_wave_sum(dot);
-  const int ranked = (int)lp_wave_sum((float)rank);  // at most 2048
-  if (lane == 0) wave_c[wave] = sum, wave_i[wave] = ranked;
-  __syncthreads();
-  if (lane == 0) wave_b[wave] = dot;
+  // back to sums of exp(d) and exp(d) d: max is finite, or they are 0 or NaN
+  dot = (dot - low * sum) * 0.69314718055994530942f;
+  const float by = __builtin_amdgcn_exp2f(-low);
+  if (lane == 0) wave_sum[wave] = sum * by, wave_dot[wave] = dot * by, wave_rank[wave] = (float)rank;  // at most 2^20
   // list what reaches the bound
   if (a.top && __any(top >= bound)) {
+    lp_u64 reaches = 0;
 #pragma unroll
-    for (int r = 0; r < kLpEach; ++r)
-      if (x[r] >= bound && (unsigned)index(r) < (unsigned)a.n) {
-        const int o = atomicAdd(&listed, 1);
-        if (o < kLpList) list[o] = lp_entry(lp_key(x[r]), index(r));
-      }
+    for (int r = 0; r < EACH; ++r) reaches |= value(r) >= bound ? 1ull << r : 0ull;
+    while (reaches) {
+      const int r = __builtin_ctzll(reaches);
+      reaches &= reaches - 1;
+      const int i = (v0 + r / VEC * (int)blockDim.x) * VEC - shift + r % VEC;
+      if ((unsigned)i >= (unsigned)a.n) continue;
+      const int o = atomicAdd(&listed, 1);
+      if (o < kLpList) list[o] = lp_entry(lp_key(lp_load<DT>(base, i)), i);
+    }
   }
   __syncthreads();
-  sum = 0.0f, dot = 0.0f, rank = 0;
-  for (int w = 0; w < waves; ++w) sum += wave_c[w], dot += wave_b[w], rank += wave_i[w];
+  const int c = listed;
+  const int begin = stretch * (int)blockDim.x * EACH - shift, end = begin + (int)blockDim.x * EACH;
+  const int held = (end < a.n ? end : a.n) - (begin > 0 ? begin : 0);  // elements of the stretch; fewer than top end its list
+  const bool in_turn = c > kLpList || c < (held < a.top ? held : a.top);
+  if (wave > 0 && !in_turn) return;
+  sum = lp_row_sum(w16 < waves ? wave_sum[w16] : 0.0f);
+  dot = lp_row_sum(w16 < waves ? wave_dot[w16] : 0.0f);
+  rank = (int)lp_row_sum(w16 < waves ? wave_rank[w16] : 0.0f);
+  if (stretch == 0 && named) {
+    const int before = (tok + shift) % VEC, i = tok - before + lane;  // in the token's vector
+    rank += __builtin_popcountll(__ballot(lane < before && i >= 0 && lp_load<DT>(base, i < 0 ? 0 : i) == at));
+    if (at == -INFINITY && VEC - shift <= tok) rank -= shift;  // what the first vector holds before the row
+  }
   const bool whole = a.stretches == 1;
   if (threadIdx.x == 0) {
     if (whole) lp_write(a, row, max, sum, dot, rank, at, named);
@@ -201,24 +263,24 @@ __global__ void __launch_bounds__(kLpMost) logprob_rows(LpArgs a) {
       a.lists[(int64_t)blockIdx.x * a.top + at_place] = entry;
     }
   };
-  const int c = listed;
-  if (c >= a.top && c <= kLpList) {
-    for (int i = threadIdx.x; i < c; i += blockDim.x) {
+  if (!in_turn) {
+    for (int i = lane; i < c; i += 64) {
       const lp_u64 mine = list[i];
       int before = 0;
+#pragma unroll 8
       for (int o = 0; o < c; ++o) before += list[o] > mine;
       if (before < a.top) place(before, mine);
     }
+    for (int i = c + lane; i < a.top; i += 64) place(i, 0);
     return;
   }
-  // one after another: the largest entry below the last one; 0 where the stretch has no more elements
+  // one after another, read again: the largest entry below the last one; 0 where the stretch has no more elements
   lp_u64 last = ~0ull;
   for (int j = 0; j < a.top; ++j) {
     lp_u64 mine = 0;
-#pragma unroll
-    for (int r = 0; r < kLpEach; ++r) {
-      const int i = index(r);
-      const lp_u64 entry = (unsigned)i < (unsigned)a.n ? lp_entry(lp_key(x[r]), i) : 0;
+#pragma unroll 8
+    for (int i = begin + (int)threadIdx.x; i < end; i += blockDim.x) {
+      const lp_u64 entry = (unsigned)i < (unsigned)a.n ? lp_entry(lp_key(lp_load<DT>(base, i)), i) : 0;
       mine = entry < last && entry > mine ? entry : mine;
     }
 #pragma unroll
@@ -241,21 +303,14 @@ __global__ void __launch_bounds__(kLpJoin) logprob_join(LpArgs a) {
   const int64_t row = blockIdx.x;
   const LpPart* parts = a.parts + row * a.stretches;
   const lp_u64* lists = a.lists + row * a.stretches * a.top;
-  float max = -INFINITY;
-  for (int s = 0; s < a.stretches; ++s) max = fmaxf(max, parts[s].max);
-  float sum = 0.0f, dot = 0.0f;
-  int rank = 0;
-  for (int s = 0; s < a.stretches; ++s) {
-    const LpPart p = parts[s];
-    rank += p.rank;
-    if (p.max == -INFINITY) {  // a sum of 0, or NaN
-      sum += p.sum;
-    } else {
-      const float d = p.max - max, by = expf(d);
-      sum += p.sum * by;
-      dot += (p.dot + p.sum * fmaxf(d, -1000.0f)) * by;
-    }
-  }
+  const int lane = threadIdx.x & 63;  // a stretch each: at most 33
+  LpPart p{-INFINITY, 0.0f, 0.0f, 0};
+  if (lane < a.stretches) p = parts[lane];
+  const float max = lp_wave_max(p.max);
+  const float d = p.max - max, by = p.max == -INFINITY ? 1.0f : expf(d);  // of -infinities alone the sums are 0, or NaN
+  const float sum = lp_wave_sum(p.sum * by);
+  const float dot = lp_wave_sum(p.max == -INFINITY ? 0.0f : (p.dot + p.sum * fmaxf(d, -1000.0f)) * by);
+  const int rank = (int)lp_wave_sum((float)p.rank);  // whole numbers of at most 2^20
   if (threadIdx.x == 0) {
     const int tok = a.tokens[row];
     const bool named = (unsigned)tok < (unsigned)a.n;
@@ -285,16 +340,18 @@ __global__ void __launch_bounds__(kLpJoin) logprob_join(LpArgs a) {
 }
 
 struct LpSizes {
-  int threads, stretches;
+  int each, threads, stretches;
   int64_t lists, bytes;
 };
 // Threads of a workgroup and stretches of a row.
 static LpSizes lp_sizes(int64_t rows, int64_t vocab, int64_t dtype, int64_t top) {
-  const int vec = dtype == TGM_F32 ? 4 : 8, each = kLpEach / vec;
+  const int vec = dtype == TGM_F32 ? 4 : 8;
   const int64_t vectors = (vocab + 2 * vec - 2) / vec;  // at most, by the alignment of the row
   LpSizes z;
-  const int64_t need = (vectors + each - 1) / each;  // threads for one stretch
-  z.threads = need >= kLpMost ? kLpMost : (int)((need + 63) / 64 * 64);
+  z.each = dtype != TGM_F32 && rows >= 512 ? 64 : 32;
+  const int64_t need = (vectors + z.each / vec - 1) / (z.each / vec);  // threads for one stretch
+  const int most = 32 * kLpMost / z.each;
+  z.threads = need >= most ? most : (int)((need + 63) / 64 * 64);
   z.stretches = (int)((need + z.threads - 1) / z.threads);
   z.lists = (rows * z.stretches * (int64_t)sizeof(LpPart) + 255) / 256 * 256;
   z.bytes = z.stretches == 1 ? 0 : z.lists + rows * z.stretches * top * 8;
@@ -303,7 +360,13 @@ static LpSizes lp_sizes(int64_t rows, int64_t vocab, int64_t dtype, int64_t top)
 
 template <int DT>
 static void lp_launch(const LpArgs& a, int64_t rows, const LpSizes& z, hipStream_t st) {
-  hipLaunchKernelGGL((logprob_rows<DT>), dim3((unsigned)(rows * z.stretches)), dim3(z.threads), 0, st, a);
+  const dim3 grid((unsigned)(rows * z.stretches)), block(z.threads);
+  if constexpr (DT != TGM_F32) {
+    if (z.each == 64) hipLaunchKernelGGL((logprob_rows<DT, 64>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((logprob_rows<DT, 32>), grid, block, 0, st, a);
+  } else {
+    hipLaunchKernelGGL((logprob_rows<DT, 32>), grid, block, 0, st, a);
+  }
   if (z.stretches > 1) hipLaunchKernelGGL((logprob_join<DT>), dim3((unsigned)rows), dim3(kLpJoin), 0, st, a);
 }
 
