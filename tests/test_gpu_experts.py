@@ -77,6 +77,21 @@ def test_route_next_to_a_border(dev, experts, groups):
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,top_k", [(64, 8, 6), (64, 1, 30), (256, 8, 8), (12, 4, 2), (96, 1, 17), (512, 16, 8), (1024, 2, 60)])
+def test_route_by_large_biases(dev, score, experts, groups, top_k):
+    """Biases that are much larger than the scores, many of them equal: experts in runs of equal 32-bit keys, groups whose
+    two best keys cancel."""
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((30, experts)).astype(np.float32) * 2
+    for bias in (np.round(rng.standard_normal(experts)) * 1000, np.where(np.arange(experts) % 2 == 0, 5000.0, -5000.0) +
+                 rng.standard_normal(experts), np.full(experts, 3e4), np.where(np.arange(experts) % 3 == 0, -np.inf, 0.25)):
+        bias = bias.astype(np.float32)
+        got = route(torch.from_numpy(x).to(dev), top_k, score=score, bias=torch.from_numpy(bias).to(dev), groups=groups,
+                    top_groups=(groups + 1) // 2)
+        routes(got, X.route(x, top_k, score, bias, groups, (groups + 1) // 2))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route_of_what_is_not_finite(dev, score):
     inf, nan = float("inf"), float("nan")
     rows = [[1, -inf, 2, -inf, 0, -inf, -inf, 3], [-inf] * 8, [nan, 1, 2, 3, nan, 5, 6, 7], [nan] * 8, [0, inf, 1, 2, 3, 4, 5, 6],

@@ -1,12 +1,15 @@
 // The choice of experts (tgm_route): scores, keys, groups, the top k and their weights, in one launch.
 //
 // A token's logits lie in W lanes, R consecutive ones a lane, so that a wave holds 64 / W tokens and the steps of a
-// reduction over one token are a reduction over all of them.  The k largest keys come one after another: a lane looks
-// through its R keys, log2(W) exchanges settle the token's best, and its lane marks it with its rank.
+// reduction over one token are a reduction over all of them.  The k largest keys come one after another: the largest of a
+// lane's R and of the W lanes, then the lowest expert that has it, whose number goes to a list in LDS.  At the end a lane
+// takes an entry of the list and computes its weight from the logit.
 //
 // The keys' order is that of 64 bits, which are needed next to a border only.  Without a bias the logits' own order is the
-// keys' and 32 bits hold it exactly.  With one, keys are computed in 32 bits first; where two that the choice compares, or
-// two groups, are nearer than their errors allow, the wave does the choice again in 64 bits.
+// keys' and 32 bits hold it exactly.  With one, keys are computed in 32 bits first, and the list goes on to the first
+// distance that is larger than their errors allow.  Where neighbours in it are nearer, its entries' keys are computed in 64
+// bits, one a lane, and put in order; where it does not end in time, or groups on either side of their border are that
+// near, the wave does the choice again in 64 bits.
 //
 // What bounds it: instructions.  8192 tokens of 256 experts read 8.4 MB, 2 us of memory time.
 #include <math.h>
@@ -72,21 +75,22 @@ __device__ __forceinline__ T lanes_sum(T v) {
   if constexpr (M < W) return lanes_sum<W, M * 2>(v + lane_xor<M>(v));
   else return v;
 }
-template <int W, int M = 1>
-__device__ __forceinline__ float lanes_max(float v) {
-  if constexpr (M < W) return lanes_max<W, M * 2>(fmaxf(v, lane_xor<M>(v)));
-  else return v;
-}
-// The largest key and, of equal ones, the lowest expert.
-template <int W, int M = 1, class Key>
-__device__ __forceinline__ void lanes_best(Key& key, int& e) {
+template <int W, int M = 1, class T>
+__device__ __forceinline__ T lanes_max(T v) {
   if constexpr (M < W) {
-    const Key k = lane_xor<M>(key);
-    const int o = (int)lane_xor<M>((unsigned)e);
-    const bool take = k > key || (k == key && o < e);
-    key = take ? k : key;
-    e = take ? o : e;
-    lanes_best<W, M * 2>(key, e);
+    const T o = lane_xor<M>(v);
+    return lanes_max<W, M * 2>(o > v ? o : v);
+  } else {
+    return v;
+  }
+}
+template <int W, int M = 1>
+__device__ __forceinline__ int lanes_min(int v) {
+  if constexpr (M < W) {
+    const int o = (int)lane_xor<M>((unsigned)v);
+    return lanes_min<W, M * 2>(o < v ? o : v);
+  } else {
+    return v;
   }
 }
 // The two largest of v1 >= v2 over the lanes.
@@ -108,91 +112,131 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Leaves out the keys of all but the best groups.  V: the type that groups' sums are held in; tol: their values may be off
-// by tol + 2.4e-7 of them each.  Returns whether two groups are nearer than that.
+// Leaves out the keys of all but the best groups.  V: the type that groups' sums are held in; in 32 bits they may be off by
+// tol and by two roundings of the keys and one of their sum each.  Returns whether a group that stays and one that goes are nearer than that.
 template <int W, int R, class V, class Key>
 __device__ __forceinline__ bool route_groups(const RouteArgs& a, int l, const V (&c)[R], Key (&key)[R], V* sums, V tol) {
-  const int per = a.experts / a.groups;
-  for (int g = 0; g < a.groups; ++g) {
-    V v1 = -INFINITY, v2 = -INFINITY;
+  const int per = a.experts / a.groups, lanes = per / R;
+  // groups of whole lanes, 2^i of them: each lane looks through its own
+  const bool whole = per % R == 0 && (lanes & (lanes - 1)) == 0;
+  auto two = [&](int first, int end, V& v1, V& v2) __attribute__((always_inline)) {
+    v1 = v2 = -INFINITY;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int e = l * R + r;
-      const V v = e >= g * per && e < (g + 1) * per && key[r] > 1 ? c[r] : (V)-INFINITY;
+      const V v = e >= first && e < end && key[r] > 1 ? c[r] : (V)-INFINITY;
       v2 = v > v1 ? v1 : (v > v2 ? v : v2);
       v1 = v > v1 ? v : v1;
     }
-    lanes_two<W>(v1, v2);
-    if (l == 0) sums[g] = per > 1 ? v1 + v2 : v1;
+  };
+  V v1, v2;
+  float size = 0.0f;  // the largest terms of a sum, if they are finite
+  if (whole) {
+    two(0, a.experts, v1, v2);
+    if (lanes > 1) lanes_two<2, 1>(v1, v2);
+    if (lanes > 2) lanes_two<4, 2>(v1, v2);
+    if (W > 8 && lanes > 4) lanes_two<8, 4>(v1, v2);
+    if (W > 8 && lanes > 8) lanes_two<16, 8>(v1, v2);
+    if constexpr (W > 32) {
+      if (lanes > 16) lanes_two<32, 16>(v1, v2);
+    }
+    size = fabsf((float)v1) + fabsf((float)v2);
+    if (l % lanes == 0 && l / lanes < a.groups) sums[l / lanes] = per > 1 ? v1 + v2 : v1;
+  } else {
+    for (int g = 0; g < a.groups; ++g) {
+      two(g * per, (g + 1) * per, v1, v2);
+      lanes_two<W>(v1, v2);
+      const float s = fabsf((float)v1) + fabsf((float)v2);
+      size = s < INFINITY ? fmaxf(size, s) : size;
+      if (l == 0) sums[g] = per > 1 ? v1 + v2 : v1;
+    }
   }
   wave_lds_fence();
-  bool near = false;
+  // the least that stays and the largest that goes
   unsigned long long kept = 0;
+  V least = INFINITY, most = -INFINITY;
   for (int g0 = 0; g0 < a.groups; g0 += W) {
     const int g = g0 + l;
     int rank = 0;
     const V v = g < a.groups ? sums[g] : (V)0;
-    if (g < a.groups)
-      for (int o = 0; o < a.groups; ++o) {
-        const V u = sums[o];
-        const Key ku = route_key(u), kv = route_key(v);
-        rank += ku > kv || (ku == kv && o < g);
-        if constexpr (sizeof(V) == 4) near |= o != g && !(fabsf(u - v) > tol + 2.4e-7f * (fabsf(u) + fabsf(v)));
-      }
-    const unsigned long long in = __ballot(g < a.groups && rank < a.top_groups);
+    const Key kv = route_key(v);
+#pragma unroll 8
+    for (int o = 0; o < a.groups; ++o) {
+      const Key ku = route_key(sums[o]);
+      rank += ku > kv || (ku == kv && o < g);
+    }
+    const bool stays = g < a.groups && rank < a.top_groups;
+    if (stays) least = v < least ? v : least;
+    else if (g < a.groups) most = v > most ? v : most;
+    const unsigned long long in = __ballot(stays);
     const unsigned long long mine = W == 64 ? in : (in >> ((threadIdx.x & 63) / W * W)) & ((1ull << (W & 63)) - 1);
     kept |= mine << g0;
   }
   wave_lds_fence();
+  if (whole) {
+    const bool stays = kept >> (l / lanes < 63 ? l / lanes : 63) & 1;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int e = l * R + r;
-    if (e < a.experts && !(kept >> (e / per) & 1)) key[r] = 0;
+    for (int r = 0; r < R; ++r) key[r] = stays || l * R + r >= a.experts ? key[r] : 0;
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int e = l * R + r;
+      if (e < a.experts && !(kept >> (e / per) & 1)) key[r] = 0;
+    }
   }
-  return near;
+  if constexpr (sizeof(V) == 8) return false;
+  least = -lanes_max<W>(-least), most = lanes_max<W>(most);
+  size = lanes_max<W>(size < INFINITY ? size : 0.0f);
+  return !(least - most > tol + 2.4e-7f * size);
 }
 
-// Marks the top k of the keys with their ranks (from 1).  Returns whether two neighbours of the order, the first that is
-// left out among them, are nearer than their errors (32-bit keys of sums with a bias).
+// The keys of a list go on to kRouteMore entries past the top k.
+constexpr int kRouteMore = 4;
+
+// Lists the experts of the largest keys, the top k of them and, with `check`, on to the first that is clearly less than its
+// neighbour; key 0 is none.  Returns the entries, and whether two neighbours are nearer than the errors of 32-bit keys
+// allow; -1 where the list does not end in time.
 template <int W, int R, class Key>
-__device__ __forceinline__ bool route_choose(const RouteArgs& a, int l, Key (&key)[R], int (&rank)[R], bool check, float tol) {
-  bool near = false;
+__device__ __forceinline__ int route_choose(const RouteArgs& a, int l, Key (&key)[R], int* list, bool check, float tol, bool& near) {
   float last = 0.0f;
-  const int rounds = a.top_k + (check && a.top_k < a.experts ? 1 : 0);
+  bool open = true;
+  int entries = 0;
+  near = false;
+  const int rounds = a.top_k + (check ? kRouteMore : 0);
   for (int j = 0; j < rounds; ++j) {
     Key best = key[0];
-    int at = 0;
 #pragma unroll
-    for (int r = 1; r < R; ++r) {
-      at = key[r] > best ? r : at;
-      best = key[r] > best ? key[r] : best;
+    for (int r = 1; r < R; ++r) best = key[r] > best ? key[r] : best;
+    best = lanes_max<W>(best);
+    if (check) {
+      const float v = route_value((unsigned)best);
+      // no key is left, or this one is clearly less; a NaN or equal infinities are near
+      const bool clear = best == 0 || last - v > tol + 1.2e-7f * (fabsf(last) + fabsf(v));
+      if (j > 0 && open) near |= !clear;
+      open = open && !(j >= a.top_k && clear);
+      last = v;
+      if (j >= a.top_k && !__any(open)) break;
     }
-    int e = l * R + at;
-    lanes_best<W>(best, e);
-    if constexpr (sizeof(Key) == 4) {
-      if (check) {
-        const float v = route_value(best);
-        // a key that is left out is no rival; a NaN or equal infinities are near, and the 64 bits decide
-        if (j > 0 && best != 0) near |= !(last - v > tol + 2.4e-7f * (fabsf(last) + fabsf(v)));
-        last = v;
-      }
-    }
-    if (j < a.top_k && e / R == l) {
+    int e = 1 << 20;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        rank[r] = e % R == r ? j + 1 : rank[r];
-        key[r] = e % R == r ? 0 : key[r];
-      }
-    }
+    for (int r = R - 1; r >= 0; --r) e = key[r] == best ? l * R + r : e;
+    e = lanes_min<W>(e);
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = l * R + r == e ? 0 : key[r];
+    if (open && l == 0) list[j] = e;
+    entries += open;
   }
-  return near;
+  return check && open ? -1 : entries;
 }
 
 template <int DT, int W, int R>
 __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
-  __shared__ double sums[kRouteThreads / W][kRouteMaxGroups];
+  constexpr int SLOTS = kRouteThreads / W;
+  __shared__ double sums[SLOTS][kRouteMaxGroups];  // of groups, then the listed experts' keys
+  extern __shared__ int lists[];                   // [slot][top_k + kRouteMore]
   const int l = threadIdx.x % W, slot = threadIdx.x / W;
-  const int64_t token = (int64_t)blockIdx.x * (kRouteThreads / W) + slot;
+  int* list = lists + slot * (a.top_k + kRouteMore);
+  const int64_t token = (int64_t)blockIdx.x * SLOTS + slot;
   const bool live = token < a.tokens;
   const int64_t base = (live ? token : a.tokens - 1) * a.ld;  // waves stay whole: exchanges run in every lane
   float x[R];
@@ -226,80 +270,128 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
   float top = -INFINITY;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const bool in = l * R + r < a.experts;
-    x[r] = in ? x[r] : -INFINITY;
+    x[r] = l * R + r < a.experts ? x[r] : -INFINITY;
     bad |= x[r] != x[r];
     top = fmaxf(top, x[r]);
   }
-  top = lanes_max<W>(top);
-  bad |= !a.sigmoid && top == INFINITY;
+  const bool soft = !a.sigmoid, limited = a.top_groups < a.groups, biased = a.bias != nullptr;
+  if (soft) top = lanes_max<W>(top);
+  bad |= soft && top == INFINITY;
   const unsigned long long seen = __ballot(bad);
   bad = ((W == 64 ? seen : seen >> ((threadIdx.x & 63) / W * W) & ((1ull << (W & 63)) - 1))) != 0;
-
-  // scores, under a softmax still to be divided by their sum
-  float p[R], sum = 0.0f;
   const float zero = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    p[r] = a.sigmoid ? 1.0f / (1.0f + expf(-x[r])) : expf(x[r] - zero);
-    sum += p[r];
-  }
-  sum = a.sigmoid ? 1.0f : lanes_sum<W>(sum);
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  auto score = [&](float v) __attribute__((always_inline)) {  // under a softmax still to be divided by their sum
+    return soft ? expf(v - zero) : 1.0f / (1.0f + expf(-v));
+  };
 
   unsigned key[R];
-  int rank[R];
-  const bool limited = a.top_groups < a.groups, biased = a.bias != nullptr;
-  bool near = false;
-  {
-    // errors of a score: 20 roundings and a difference of logits under a softmax, whose largest is inv; 4 of a sigmoid
-    const float tol = a.sigmoid ? 1e-6f : 4e-5f * inv + 1e-37f;
+  float sum = 1.0f;
+  bool near = false, again = false;
+  int entries;
+  if (biased || limited) {
     float c[R];
+    sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      c[r] = score(x[r]);
+      sum += c[r];
+    }
+    sum = soft ? lanes_sum<W>(sum) : 1.0f;
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    // Errors of two scores.  Sigmoid: exp, sum and quotient are off by 2^-23, 2^-24 and 2^-24 of at most 1.  Softmax: of the
+    // largest, inv, a difference of logits up to 104 (below, the score is 0), exp, R + 6 sums and two products, 2^-16.
+    const float tol = soft ? 3.1e-5f * inv + 1e-37f : 4.8e-7f;
+    float b[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) b[r] = 0.0f;
+    if (biased) {
+      if (R >= 4 && a.vectors && (uintptr_t)a.bias % 16 == 0) {
+#pragma unroll
+        for (int q = 0; q < R / 4; ++q) {
+          typedef float f4 __attribute__((ext_vector_type(4)));
+          const int e = l * R + 4 * q;
+          const f4 v = e < a.experts ? *(const f4*)(a.bias + e) : f4{};
+          b[4 * q] = v[0], b[4 * q + 1] = v[1], b[4 * q + 2] = v[2], b[4 * q + 3] = v[3];
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) b[r] = l * R + r < a.experts ? a.bias[l * R + r] : 0.0f;
+      }
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int e = l * R + r;
-      rank[r] = 0;
-      c[r] = p[r] * inv + (biased && e < a.experts ? a.bias[e] : 0.0f);
+      c[r] = c[r] * inv + b[r];
       c[r] = x[r] != x[r] ? x[r] : c[r];
       key[r] = e < a.experts ? route_key(biased ? c[r] : x[r]) : 0u;
     }
-    if (limited) near = route_groups<W, R>(a, l, c, key, (float*)sums[slot], tol);
-    near |= route_choose<W, R>(a, l, key, rank, biased, tol);
-  }
-  if (__any(near && !bad)) {  // the whole wave again, in 64 bits
-    unsigned long long key64[R];
-    double c[R], total = 0.0;
+    if (limited) again = route_groups<W, R>(a, l, c, key, (float*)sums[slot], 2 * tol);
+    entries = route_choose<W, R>(a, l, key, list, biased, tol, near);
+    again |= entries < 0 || (near && entries > W);
+  } else {
+    if (soft && !a.renormalize) {
+      sum = 0.0f;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      c[r] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[r])) : exp((double)x[r] - (double)zero);
-      total += c[r];
+      for (int r = 0; r < R; ++r) sum += expf(x[r] - zero);
+      sum = lanes_sum<W>(sum);
     }
-    total = a.sigmoid ? 1.0 : lanes_sum<W>(total);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int e = l * R + r;
-      rank[r] = 0;
-      c[r] = (total > 0.0 ? c[r] / total : 0.0) + (biased && e < a.experts ? (double)a.bias[e] : 0.0);
-      c[r] = x[r] != x[r] ? (double)x[r] : c[r];
-      key64[r] = e < a.experts ? route_key(biased ? c[r] : (double)x[r]) : 0ull;
-    }
-    if (limited) route_groups<W, R>(a, l, c, key64, sums[slot], 0.0);
-    route_choose<W, R>(a, l, key64, rank, false, 0.0f);
+    for (int r = 0; r < R; ++r) key[r] = l * R + r < a.experts ? route_key(x[r]) : 0u;
+    entries = route_choose<W, R>(a, l, key, list, false, 0.0f, near);
   }
+  if (__any((near || again) && !bad)) {
+    double total = 1.0;
+    if (soft) {
+      total = 0.0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) total += exp((double)x[r] - (double)zero);
+      total = lanes_sum<W>(total);
+    }
+    auto wide_key = [&](float v, int e) __attribute__((always_inline)) {
+      const double p = soft ? exp((double)v - (double)zero) : 1.0 / (1.0 + exp(-(double)v));
+      return v != v ? (double)v : (total > 0.0 ? p / total : 0.0) + (biased ? (double)a.bias[e] : 0.0);
+    };
+    if (__any(again && !bad)) {  // the whole wave
+      unsigned long long wide[R];
+      double c[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int e = l * R + r;
+        c[r] = e < a.experts ? wide_key(x[r], e) : 0.0;
+        wide[r] = e < a.experts ? route_key(biased ? c[r] : (double)x[r]) : 0ull;
+      }
+      if (limited) route_groups<W, R>(a, l, c, wide, sums[slot], 0.0);
+      bool unused;
+      route_choose<W, R>(a, l, wide, list, false, 0.0f, unused);
+    } else {
+      wave_lds_fence();
+      const bool holds = near && l < entries;
+      const int e = holds ? list[l] : 0;
+      const unsigned long long mine = holds ? route_key(wide_key(load_f32(a.logits, DT, base + e), e)) : 0ull;
+      if (holds) sums[slot][l] = __builtin_bit_cast(double, mine);
+      wave_lds_fence();
+      int rank = 0;
+      for (int o = 0; o < (near ? entries : 0); ++o) {
+        const unsigned long long k = __builtin_bit_cast(unsigned long long, sums[slot][o]);
+        rank += k > mine || (k == mine && list[o] < e);
+      }
+      wave_lds_fence();
+      if (holds && rank < a.top_k) list[rank] = e;
+    }
+  }
+  wave_lds_fence();
 
+  // the weights, an entry a lane
   float chosen = 0.0f;
-#pragma unroll
-  for (int r = 0; r < R; ++r) chosen += rank[r] ? p[r] : 0.0f;
+  for (int j = l; j < a.top_k; j += W) chosen += score(load_f32(a.logits, DT, base + list[j]));
   chosen = a.renormalize ? lanes_sum<W>(chosen) : sum;
   const float by = chosen > 0.0f ? a.scale / chosen : 0.0f;
   if (!live) return;
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-    if (rank[r]) {
-      const int64_t o = token * a.top_k + rank[r] - 1;
-      a.ids[o] = l * R + r;
-      a.weights[o] = bad ? NAN : p[r] * by;
-    }
+  for (int j = l; j < a.top_k; j += W) {
+    const int e = list[j];
+    a.ids[token * a.top_k + j] = e;
+    a.weights[token * a.top_k + j] = bad ? NAN : score(load_f32(a.logits, DT, base + e)) * by;
+  }
 }
 
 template <int DT>
@@ -307,7 +399,7 @@ static void route_launch(const RouteArgs& a, hipStream_t st) {
   // few lanes a token make few exchanges; up to 16 of its logits a lane stay in registers
 #define TGM_ROUTE(W, R)                                                                                             \
   hipLaunchKernelGGL((route_rows<DT, W, R>), dim3((unsigned)((a.tokens + kRouteThreads / W - 1) / (kRouteThreads / W))), \
-                     dim3(kRouteThreads), 0, st, a)
+                     dim3(kRouteThreads), kRouteThreads / W * (a.top_k + kRouteMore) * sizeof(int), st, a)
   if (a.experts <= 8) TGM_ROUTE(8, 1);
   else if (a.experts <= 16) TGM_ROUTE(16, 1);
   else if (a.experts <= 32) TGM_ROUTE(16, 2);
