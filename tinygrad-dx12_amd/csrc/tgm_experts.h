@@ -12,6 +12,7 @@ struct ExpertTile {
 };
 constexpr ExpertTile kExpertTiles[] = {{32, 64}, {64, 64}, {64, 128}, {128, 256}};
 constexpr int kExpertTileKinds = 4;
+constexpr int kMaxExperts = 1024;
 
 // A grouped product on tiles of kExpertTiles[shape] with `most` tile rows at most; tgm_experts_tile_{mx,i4}.hip.
 int launch_experts_tile_mx(const WGroupArgs& p, int fmt, int shape, int64_t most, hipStream_t stream);

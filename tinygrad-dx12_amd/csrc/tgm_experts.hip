@@ -13,11 +13,11 @@
 //
 // The count of tiles is known on the device alone: a launch covers the most that the pairs can make, and workgroups past
 // the count end at once.
-#include "tgm_experts.h"
+#include "tgm_experts_few.h"
 
 namespace tgm {
 
-constexpr int kPlanThreads = 1024, kMaxExperts = 1024;
+constexpr int kPlanThreads = 1024;
 
 struct PlanArgs {
   const int32_t* ids;
@@ -123,7 +123,7 @@ static ExpertSizes expert_sizes(const tgm_experts& e, int64_t tokens, int64_t to
     z.most[i] = z.pairs / kExpertTiles[i].rows + (z.pairs < e.experts ? z.pairs : e.experts);
     most = z.most[i] > most ? z.most[i] : most;
   }
-  z.tiles = take(16 * (1 + most));
+  z.tiles = take(16 * (1 + most) > (int64_t)sizeof(FewList) ? 16 * (1 + most) : (int64_t)sizeof(FewList));
   z.source = take(4 * z.pairs);
   z.place = take(4 * z.pairs);
   z.hidden = take(2 * z.pairs * e.ffn);
@@ -194,12 +194,53 @@ extern "C" int tgm_experts_apply(const tgm_experts* experts, const void* x, int6
                 "x and the weights must be 16-byte and scales 4-byte aligned");
   const ExpertSizes z = expert_sizes(e, tokens, top_k);
   TGM_CHECK_ARG(workspace && workspace_bytes >= z.bytes && ((uintptr_t)workspace & 15) == 0, "workspace too small or misaligned");
+  const int64_t bits = format_info((int)e.format).bits;
+  const int64_t per = scaled ? (e.scale_dtype == TGM_E8M0 ? 1 : dtype_size((int)e.scale_dtype)) : 0;
+  const int64_t block = scaled ? e.block_size : 128;
+  const hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  if (tokens <= kFewTokens && z.pairs <= kFewPairs) {
+    const int known = stream_cu_count(st), cus = known > 0 ? known : 256;
+    auto product = [&](bool up) {
+      FewArgs p{};
+      p.w = (const uint8_t*)(up ? e.gate_up : e.down);
+      p.scales = scaled ? (const uint8_t*)(up ? e.gate_up_scales : e.down_scales) : nullptr;
+      p.N = (int)(up ? 2 * e.ffn : e.hidden), p.K = (int)(up ? e.hidden : e.ffn);
+      p.w_bytes = (int64_t)p.N * p.K * bits / 8, p.s_bytes = (int64_t)p.N * (p.K / block) * per;
+      p.a = (const uint8_t*)(up ? x : ws + z.hidden), p.lda = 2 * (up ? ldx : e.ffn);
+      p.a_bytes = (unsigned)(up ? ((tokens - 1) * ldx + e.hidden) * 2 : z.pairs * e.ffn * 2);
+      p.list = ws + z.tiles;
+      p.ids = ids, p.weights = weights, p.tokens = (int)tokens, p.top_k = (int)top_k, p.experts = (int)e.experts;
+      p.sdt = (int)e.scale_dtype, p.is_signed = e.format == TGM_FMT_INT4;
+      p.y = up ? ws + z.hidden : y, p.ldy = up ? e.ffn : ldy, p.ydt = up ? (int)x_dtype : (int)y_dtype;
+      int groups;
+      if (up) {
+        // One workgroup a compute unit.  As many of the rows' slices as waves end together best, where a unit's own work counts
+        // as half a group; the experts that tokens name are taken as chosen at random.
+        const int waves = ints ? experts_few_waves_i4(scaled ? (int)e.scale_dtype : TGM_NONE, e.block_size) : experts_few_waves_mx((int)e.format);
+        const double named = (double)e.experts * (1.0 - pow(1.0 - 1.0 / (double)e.experts, (double)z.pairs));
+        const int64_t units = (int64_t)(named + 0.5) * (p.N / 16), all = (int64_t)cus * waves, parts = (p.K + 511) / 512;
+        double least = 0.0;
+        for (int s = 1; s <= 4 && s <= parts; s *= 2) {
+          const double cost = (double)((units * s + all - 1) / all) * ((double)((parts + s - 1) / s) + 0.5);
+          if (s == 1 || cost < least) least = cost, p.slices = s;
+        }
+        const int64_t most = (units * p.slices + waves - 1) / waves;
+        groups = (int)(most < cus ? most : cus);
+      } else {
+        // rounds of one workgroup a compute unit, their rows even
+        const int64_t rounds = (p.N + 16 * cus - 1) / (16 * cus);
+        p.rows = (int)((p.N + cus * rounds - 1) / (cus * rounds));
+        groups = (p.N + p.rows - 1) / p.rows;
+      }
+      return ints ? launch_experts_few_i4(p, e.block_size, up, groups, st) : launch_experts_few_mx(p, (int)e.format, up, groups, st);
+    };
+    if (const int status = product(true); status != TGM_OK) return status;
+    return product(false);
+  }
   const int shape = expert_tile(e, z.pairs);
   const int64_t wide = 2 * e.ffn > e.hidden ? 2 * e.ffn : e.hidden;
   TGM_CHECK_ARG(z.most[shape] * ((wide + kExpertTiles[shape].cols - 1) / kExpertTiles[shape].cols) < (1ll << 31), "too many tiles");
-  const hipStream_t st = (hipStream_t)stream;
-  char* ws = (char*)workspace;
-
   PlanArgs plan;
   plan.ids = ids, plan.pairs = (int)z.pairs, plan.top_k = (int)top_k, plan.experts = (int)e.experts;
   plan.rows = kExpertTiles[shape].rows;
@@ -207,9 +248,6 @@ extern "C" int tgm_experts_apply(const tgm_experts* experts, const void* x, int6
   hipLaunchKernelGGL(experts_plan, dim3(1), dim3(kPlanThreads), 0, st, plan);
   if (const int status = launch_status("tgm_experts_apply"); status != TGM_OK) return status;
 
-  const int64_t bits = format_info((int)e.format).bits;
-  const int64_t per = scaled ? (e.scale_dtype == TGM_E8M0 ? 1 : dtype_size((int)e.scale_dtype)) : 0;
-  const int64_t block = scaled ? e.block_size : 128;
   auto product = [&](bool up) {
     WGroupArgs p{};
     p.a = (const uint8_t*)(up ? x : ws + z.hidden);
