@@ -6,17 +6,15 @@
 
 namespace tgm {
 
-// Tiles of the grouped products, rows x columns: what the 32, 64, 128 and 128 wide rows of kExpertTiles mean.
-struct ExpertTile {
-  int rows, cols;
-};
-constexpr ExpertTile kExpertTiles[] = {{32, 64}, {64, 64}, {64, 128}, {128, 256}};
-constexpr int kExpertTileKinds = 4;
+// Tiles of the grouped products, rows by the rows that experts have on average: of 32, 64 or 128, each 128 or 256 wide.
+constexpr int kExpertRows[] = {32, 64, 128};
+constexpr int kExpertTileKinds = 3;
 constexpr int kMaxExperts = 1024;
 
-// A grouped product on tiles of kExpertTiles[shape] with `most` tile rows at most; tgm_experts_tile_{mx,i4}.hip.
-int launch_experts_tile_mx(const WGroupArgs& p, int fmt, int shape, int64_t most, hipStream_t stream);
-int launch_experts_tile_i4(const WGroupArgs& p, int64_t group, int shape, int64_t most, hipStream_t stream);
+// A grouped product on tiles of kExpertRows[shape] rows and 128 or (wide) 256 columns, `most` tile rows at most;
+// tgm_experts_tile_{mx,i4}.hip.
+int launch_experts_tile_mx(const WGroupArgs& p, int fmt, int shape, bool wide, int64_t most, hipStream_t stream);
+int launch_experts_tile_i4(const WGroupArgs& p, int64_t group, int shape, bool wide, int64_t most, hipStream_t stream);
 
 template <int KIND, int FA, int WN, int WK, int NBUF>
 int launch_experts_tile(const WGroupArgs& p, int64_t most, hipStream_t stream) {

@@ -13,6 +13,8 @@
 //
 // The count of tiles is known on the device alone: a launch covers the most that the pairs can make, and workgroups past
 // the count end at once.
+#include <math.h>
+
 #include "tgm_experts_few.h"
 
 namespace tgm {
@@ -49,15 +51,26 @@ __device__ __forceinline__ int block_before(int v, int* buf, int& total) {
   return before;
 }
 
-// One workgroup.  A pair's position among those of its expert goes by an atomic's order, which changes nothing else: every
-// row is computed alike wherever it stands.
+// One workgroup; a thread's first kPlanEach ids stay in registers, so that all of them are loaded at once and once.  A pair's
+// position among those of its expert goes by an atomic's order, which changes nothing else: every row is computed alike
+// wherever it stands.
+constexpr int kPlanEach = 16;
 __global__ void __launch_bounds__(kPlanThreads) experts_plan(PlanArgs a) {
   __shared__ int count[kMaxExperts];
   __shared__ int buf[kPlanThreads / 64];
   const int e = threadIdx.x;
+  unsigned ids[kPlanEach];
+#pragma unroll
+  for (int i = 0; i < kPlanEach; ++i) {
+    const int pair = i * kPlanThreads + threadIdx.x;
+    ids[i] = pair < a.pairs ? (unsigned)a.ids[pair] : ~0u;
+  }
   count[e] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < a.pairs; i += kPlanThreads) {
+#pragma unroll
+  for (int i = 0; i < kPlanEach; ++i)
+    if (ids[i] < (unsigned)a.experts) atomicAdd(&count[ids[i]], 1);
+  for (int i = kPlanEach * kPlanThreads + threadIdx.x; i < a.pairs; i += kPlanThreads) {
     const unsigned id = (unsigned)a.ids[i];
     if (id < (unsigned)a.experts) atomicAdd(&count[id], 1);
   }
@@ -76,15 +89,18 @@ __global__ void __launch_bounds__(kPlanThreads) experts_plan(PlanArgs a) {
   }
   count[e] = first;
   __syncthreads();
-  for (int i = threadIdx.x; i < a.pairs; i += kPlanThreads) {
-    const unsigned id = (unsigned)a.ids[i];
+  auto put = [&](int pair, unsigned id) __attribute__((always_inline)) {
     int p = -1;
     if (id < (unsigned)a.experts) {
       p = atomicAdd(&count[id], 1);
-      a.source[p] = i / a.top_k;
+      a.source[p] = pair / a.top_k;
     }
-    a.place[i] = p;
-  }
+    a.place[pair] = p;
+  };
+#pragma unroll
+  for (int i = 0; i < kPlanEach; ++i)
+    if (i * kPlanThreads + (int)threadIdx.x < a.pairs) put(i * kPlanThreads + threadIdx.x, ids[i]);
+  for (int i = kPlanEach * kPlanThreads + threadIdx.x; i < a.pairs; i += kPlanThreads) put(i, (unsigned)a.ids[i]);
 }
 
 // A token's rows, four columns a thread.
@@ -120,7 +136,7 @@ static ExpertSizes expert_sizes(const tgm_experts& e, int64_t tokens, int64_t to
   };
   for (int i = 0; i < kExpertTileKinds; ++i) {
     // every expert that a pair names may end in a tile that is not full
-    z.most[i] = z.pairs / kExpertTiles[i].rows + (z.pairs < e.experts ? z.pairs : e.experts);
+    z.most[i] = z.pairs / kExpertRows[i] + (z.pairs < e.experts ? z.pairs : e.experts);
     most = z.most[i] > most ? z.most[i] : most;
   }
   z.tiles = take(16 * (1 + most) > (int64_t)sizeof(FewList) ? 16 * (1 + most) : (int64_t)sizeof(FewList));
@@ -132,10 +148,22 @@ static ExpertSizes expert_sizes(const tgm_experts& e, int64_t tokens, int64_t to
   return z;
 }
 
-// Rows of x per expert, on average, decide the tile: the smallest that holds them.
+// Experts that pairs name, taken as chosen at random.
+static double experts_named(const tgm_experts& e, int64_t pairs) {
+  return (double)e.experts * (1.0 - pow(1.0 - 1.0 / (double)e.experts, (double)pairs));
+}
+// Rows of the tiles by the rows of x that an expert has on average.  us of the two products of 64 experts of 2048 x 1408 with 32,
+// 64 and 128 rows, FP4: 6 rows an expert 80, 86, -; 24 rows 105, 108, 116; 192 rows -, 331, 303.  FP6, 32 experts, 64 rows
+// 131, 117, 130.
 static int expert_tile(const tgm_experts& e, int64_t pairs) {
-  const int64_t mean = pairs / (pairs < e.experts ? pairs : e.experts);
-  return mean <= 32 ? 0 : mean <= 48 ? 1 : mean <= 96 ? 2 : 3;
+  const double mean = (double)pairs / experts_named(e, pairs);
+  return mean <= 32.0 ? 0 : mean <= 96.0 ? 1 : 2;
+}
+// Whether tiles of 256 columns are enough to give every compute unit one.  INT4, 17 tile rows x 4096: 38 us, and 41 on 128 columns;
+// FP4, 8 tile rows x 4096: 103 and 68.
+static bool expert_wide(const tgm_experts& e, int64_t pairs, int64_t columns, int shape, int cus) {
+  const double named = experts_named(e, pairs), rows = named + (double)(pairs / kExpertRows[shape]) / 2;
+  return rows * (double)((columns + 255) / 256) >= cus;
 }
 
 static bool expert_ints(int64_t format) { return format == TGM_FMT_INT4 || format == TGM_FMT_UINT4; }
@@ -199,8 +227,8 @@ extern "C" int tgm_experts_apply(const tgm_experts* experts, const void* x, int6
   const int64_t block = scaled ? e.block_size : 128;
   const hipStream_t st = (hipStream_t)stream;
   char* ws = (char*)workspace;
+  const int known = stream_cu_count(st), cus = known > 0 ? known : 256;
   if (tokens <= kFewTokens && z.pairs <= kFewPairs) {
-    const int known = stream_cu_count(st), cus = known > 0 ? known : 256;
     auto product = [&](bool up) {
       FewArgs p{};
       p.w = (const uint8_t*)(up ? e.gate_up : e.down);
@@ -216,10 +244,9 @@ extern "C" int tgm_experts_apply(const tgm_experts* experts, const void* x, int6
       int groups;
       if (up) {
         // One workgroup a compute unit.  As many of the rows' slices as waves end together best, where a unit's own work counts
-        // as half a group; the experts that tokens name are taken as chosen at random.
+        // as half a group.
         const int waves = ints ? experts_few_waves_i4(scaled ? (int)e.scale_dtype : TGM_NONE, e.block_size) : experts_few_waves_mx((int)e.format);
-        const double named = (double)e.experts * (1.0 - pow(1.0 - 1.0 / (double)e.experts, (double)z.pairs));
-        const int64_t units = (int64_t)(named + 0.5) * (p.N / 16), all = (int64_t)cus * waves, parts = (p.K + 511) / 512;
+        const int64_t units = (int64_t)(experts_named(e, z.pairs) + 0.5) * (p.N / 16), all = (int64_t)cus * waves, parts = (p.K + 511) / 512;
         double least = 0.0;
         for (int s = 1; s <= 4 && s <= parts; s *= 2) {
           const double cost = (double)((units * s + all - 1) / all) * ((double)((parts + s - 1) / s) + 0.5);
@@ -239,11 +266,11 @@ extern "C" int tgm_experts_apply(const tgm_experts* experts, const void* x, int6
     return product(false);
   }
   const int shape = expert_tile(e, z.pairs);
-  const int64_t wide = 2 * e.ffn > e.hidden ? 2 * e.ffn : e.hidden;
-  TGM_CHECK_ARG(z.most[shape] * ((wide + kExpertTiles[shape].cols - 1) / kExpertTiles[shape].cols) < (1ll << 31), "too many tiles");
+  const int64_t most_columns = 2 * e.ffn > e.hidden ? 2 * e.ffn : e.hidden;
+  TGM_CHECK_ARG(z.most[shape] * ((most_columns + 127) / 128) < (1ll << 31), "too many tiles");
   PlanArgs plan;
   plan.ids = ids, plan.pairs = (int)z.pairs, plan.top_k = (int)top_k, plan.experts = (int)e.experts;
-  plan.rows = kExpertTiles[shape].rows;
+  plan.rows = kExpertRows[shape];
   plan.tiles = (int*)(ws + z.tiles), plan.source = (int*)(ws + z.source), plan.place = (int*)(ws + z.place);
   hipLaunchKernelGGL(experts_plan, dim3(1), dim3(kPlanThreads), 0, st, plan);
   if (const int status = launch_status("tgm_experts_apply"); status != TGM_OK) return status;
@@ -262,8 +289,9 @@ extern "C" int tgm_experts_apply(const tgm_experts* experts, const void* x, int6
     p.tiles = plan.tiles, p.rows = up ? plan.source : nullptr;
     p.a_bytes = (unsigned)(((tokens - 1) * ldx + e.hidden) * 2);
     p.w_bytes = (int64_t)p.N * p.K * bits / 8, p.s_bytes = (int64_t)p.N * (p.K / block) * per;
-    return ints ? launch_experts_tile_i4(p, e.block_size, shape, z.most[shape], st)
-                : launch_experts_tile_mx(p, (int)e.format, shape, z.most[shape], st);
+    const bool wide = expert_wide(e, z.pairs, p.N, shape, cus);
+    return ints ? launch_experts_tile_i4(p, e.block_size, shape, wide, z.most[shape], st)
+                : launch_experts_tile_mx(p, (int)e.format, shape, wide, z.most[shape], st);
   };
   if (const int status = product(true); status != TGM_OK) return status;
   if (const int status = product(false); status != TGM_OK) return status;

@@ -3,24 +3,22 @@
 
 namespace tgm {
 
-// The 32 x 64 shape holds two stages with scales per 32, whose third would not fit the LDS.
 template <int KIND>
-static int launch_kind(const WGroupArgs& p, int shape, int64_t most, hipStream_t st) {
-  switch (shape) {
-    case 0: return launch_experts_tile<KIND, 1, 2, 4, kind_group(KIND) == 32 ? 2 : 3>(p, most, st);
-    case 1: return launch_experts_tile<KIND, 2, 2, 2, 3>(p, most, st);
-    case 2: return launch_experts_tile<KIND, 2, 4, 1, 3>(p, most, st);
-    default: return launch_experts_tile<KIND, 4, 8, 1, 2>(p, most, st);
-  }
+static int launch_kind(const WGroupArgs& p, int shape, bool wide, int64_t most, hipStream_t st) {
+  constexpr bool FINE = kind_group(KIND) == 32;
+  if (shape == 0)
+    return wide ? launch_experts_tile<KIND, 1, 8, 1, FINE ? 2 : 3>(p, most, st) : launch_experts_tile<KIND, 1, 4, 1, FINE ? 3 : 4>(p, most, st);
+  if (shape == 1) return wide ? launch_experts_tile<KIND, 2, 8, 1, 3>(p, most, st) : launch_experts_tile<KIND, 2, 4, 1, 3>(p, most, st);
+  return wide ? launch_experts_tile<KIND, 4, 8, 1, 2>(p, most, st) : launch_experts_tile<KIND, 4, 4, 1, 2>(p, most, st);
 }
 
-int launch_experts_tile_i4(const WGroupArgs& p, int64_t group, int shape, int64_t most, hipStream_t st) {
-  if (!p.scales) return launch_kind<kKindI4>(p, shape, most, st);
-  const bool wide = p.sdt == TGM_F32;
+int launch_experts_tile_i4(const WGroupArgs& p, int64_t group, int shape, bool wide, int64_t most, hipStream_t st) {
+  if (!p.scales) return launch_kind<kKindI4>(p, shape, wide, most, st);
+  const bool f32 = p.sdt == TGM_F32;
   switch (group) {
-    case 32: return wide ? launch_kind<kKindI4 + 33>(p, shape, most, st) : launch_kind<kKindI4 + 32>(p, shape, most, st);
-    case 64: return wide ? launch_kind<kKindI4 + 65>(p, shape, most, st) : launch_kind<kKindI4 + 64>(p, shape, most, st);
-    default: return wide ? launch_kind<kKindI4 + 129>(p, shape, most, st) : launch_kind<kKindI4 + 128>(p, shape, most, st);
+    case 32: return f32 ? launch_kind<kKindI4 + 33>(p, shape, wide, most, st) : launch_kind<kKindI4 + 32>(p, shape, wide, most, st);
+    case 64: return f32 ? launch_kind<kKindI4 + 65>(p, shape, wide, most, st) : launch_kind<kKindI4 + 64>(p, shape, wide, most, st);
+    default: return f32 ? launch_kind<kKindI4 + 129>(p, shape, wide, most, st) : launch_kind<kKindI4 + 128>(p, shape, wide, most, st);
   }
 }
 

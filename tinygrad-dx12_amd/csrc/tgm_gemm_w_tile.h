@@ -47,6 +47,8 @@
 // scale is added to the accumulator.
 #pragma once
 
+#include <type_traits>
+
 #include "tgm_mfma_common.h"
 
 namespace tgm {
@@ -303,10 +305,11 @@ gemm_w_tile(Args p) {
   for (int t = 0; t < FA; ++t) {
     acc[t] = f32x16{};
   }
-  auto read_a = [&](int buf, int j, u32x4 (&dst)[FA]) __attribute__((always_inline)) {
+  auto read_a = [&](auto blocks, int buf, int j, u32x4 (&dst)[FA]) __attribute__((always_inline)) {
+    constexpr int NF = decltype(blocks)::value;
     const int col = (I4 ? 2 * j + half : 8 * half + j) ^ (l32 & 15);
 #pragma unroll
-    for (int t = 0; t < FA; ++t)
+    for (int t = 0; t < NF; ++t)
       dst[t] = *(const u32x4*)(lds + buf * T::kStage + wk * T::kStep + (32 * t + l32) * 256 + col * 16);
   };
   auto read_w = [&](int buf, unsigned (&r)[RAW], unsigned (&sb)[T::kNS ? T::kNS : 1]) __attribute__((always_inline)) {
@@ -344,8 +347,10 @@ gemm_w_tile(Args p) {
   // and substep 0's weights are decoded.  Substep j reads A of j + 2 and decodes ahead; before substep 6,
   // when every LDS read of the stage is done, the wave waits for its share of the next stage, the barrier
   // publishes it and frees this buffer, and substeps 6 and 7 cover the refill's issue, the next stage's
-  // first reads and its first decode.
-  auto stage = [&](int st, int prv, int cur, int nxt) __attribute__((always_inline)) {
+  // first reads and its first decode.  Of the tile's blocks of 32 rows the first `blocks` are multiplied: the
+  // rows of an expert rarely fill its last tile.
+  auto stage = [&](auto blocks, int st, int prv, int cur, int nxt) __attribute__((always_inline)) {
+    constexpr int NF = decltype(blocks)::value;
     f32x16 part[FA];  // the sums of the current scale group
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -354,12 +359,12 @@ gemm_w_tile(Args p) {
         wait_loads<(NBUF - 2) * T::kLoads>();
         lds_barrier();
         read_w(nxt, rawn, sbitsn);
-        read_a(nxt, 0, fa[0]);
+        read_a(blocks, nxt, 0, fa[0]);
 
       } else if (j > 8 - PD) {
-        read_a(nxt, j + PD - 8, fa[j + PD - 8]);
+        read_a(blocks, nxt, j + PD - 8, fa[j + PD - 8]);
       } else {
-        read_a(cur, j + PD, fa[(j + PD) % SL]);
+        read_a(blocks, cur, j + PD, fa[(j + PD) % SL]);
       }
       // this substep's share of the loads, one after each MFMA: stage st + NBUF into this buffer from substep
       // 8 - PD on, the rest of stage st + NBUF - 1 into the previous stage's buffer before
@@ -377,9 +382,11 @@ gemm_w_tile(Args p) {
         if (j < 7) wi[(j + 1) & 1] = decode_nibbles(raw[j + 1], nib);
 #pragma unroll
         for (int t = 0; t < FA; ++t) {
-          const wt_f16x8 a = __builtin_bit_cast(wt_f16x8, fa[j % SL][t]);
-          if constexpr (G == 0) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wi[j & 1], acc[t], 0, 0, 0);
-          else part[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wi[j & 1], j % JPG ? part[t] : f32x16{}, 0, 0, 0);
+          if (t < NF) {
+            const wt_f16x8 a = __builtin_bit_cast(wt_f16x8, fa[j % SL][t]);
+            if constexpr (G == 0) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wi[j & 1], acc[t], 0, 0, 0);
+            else part[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wi[j & 1], j % JPG ? part[t] : f32x16{}, 0, 0, 0);
+          }
           pieces(t);
         }
         if (j == 7) wi[0] = decode_nibbles(rawn[0], nib);
@@ -388,19 +395,20 @@ gemm_w_tile(Args p) {
           const float sv = ssize == 2 && p.sdt == TGM_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)bits)
                                                           : __builtin_bit_cast(float, bits << sshift);
 #pragma unroll
-          for (int t = 0; t < FA; ++t)
+          for (int t = 0; t < NF; ++t)
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[t][v] += part[t][v] * sv;
           // pins these sums here: left to itself the compiler collects every group's at the stage's end,
           // and with them every group's 16 FA partial sums (G = 32: 512 registers)
 #pragma unroll
-          for (int t = 0; t < FA; ++t) asm volatile("" : "+v"(acc[t]));
+          for (int t = 0; t < NF; ++t) asm volatile("" : "+v"(acc[t]));
         }
       } else {
         if (j == 2) mx_block(raw, sbits[0], 1);
 #pragma unroll
         for (int t = 0; t < FA; ++t) {
-          acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(wt_bf16x8, fa[j % SL][t]), wd[j], acc[t], 0, 0, 0);
+          if (t < NF)
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(wt_bf16x8, fa[j % SL][t]), wd[j], acc[t], 0, 0, 0);
           pieces(t);
         }
         if (j == 7) mx_block(rawn, sbitsn[0], 0);
@@ -422,17 +430,40 @@ gemm_w_tile(Args p) {
   wait_loads<(NBUF - 2) * T::kLoads + T::first_piece(0)>();
   lds_barrier();
   read_w(0, raw, sbits);
+  int used = FA;
+  if constexpr (!Args::kGrouped) {
+    constexpr std::integral_constant<int, FA> all{};
 #pragma unroll
-  for (int j = 0; j < PD; ++j) read_a(0, j, fa[j]);
-  if constexpr (I4) wi[0] = decode_nibbles(raw[0], nib);
-  else mx_block(raw, sbits[0], 0);
-  int prv = NBUF - 1, cur = 0;
+    for (int j = 0; j < PD; ++j) read_a(all, 0, j, fa[j]);
+    if constexpr (I4) wi[0] = decode_nibbles(raw[0], nib);
+    else mx_block(raw, sbits[0], 0);
+    int prv = NBUF - 1, cur = 0;
 #pragma unroll 1
-  for (int st = 0; st < nstages; ++st) {
-    const int nxt = cur + 1 < NBUF ? cur + 1 : 0;
-    stage(st, prv, cur, nxt);
-    prv = cur;
-    cur = nxt;
+    for (int st = 0; st < nstages; ++st) {
+      const int nxt = cur + 1 < NBUF ? cur + 1 : 0;
+      stage(all, st, prv, cur, nxt);
+      prv = cur;
+      cur = nxt;
+    }
+  } else {
+    auto stages = [&](auto blocks) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < PD; ++j) read_a(blocks, 0, j, fa[j]);
+      if constexpr (I4) wi[0] = decode_nibbles(raw[0], nib);
+      else mx_block(raw, sbits[0], 0);
+      int prv = NBUF - 1, cur = 0;
+#pragma unroll 1
+      for (int st = 0; st < nstages; ++st) {
+        const int nxt = cur + 1 < NBUF ? cur + 1 : 0;
+        stage(blocks, st, prv, cur, nxt);
+        prv = cur;
+        cur = nxt;
+      }
+    };
+    used = (m_end - m0 + 31) / 32;
+    if (FA > 1 && used == 1) stages(std::integral_constant<int, 1>{});
+    else if (FA > 2 && used == 2) stages(std::integral_constant<int, FA < 2 ? FA : 2>{});
+    else stages(std::integral_constant<int, FA>{});
   }
   wait_loads<0>();
   __syncthreads();  // the epilogue reuses the LDS
@@ -457,6 +488,7 @@ gemm_w_tile(Args p) {
   float* ep = parts + (WK - 1) * WN * FA * 1024 + wn * 32 * 36;
 #pragma unroll
   for (int t = 0; t < FA; ++t) {
+    if (Args::kGrouped && t >= used) break;
     if (!Args::kGrouped && WK == 1 && p.part)
       store_tile32(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, p.M, p.N, p.part + (int64_t)blockIdx.y * p.M * p.N, TGM_F32,
                    p.N);
