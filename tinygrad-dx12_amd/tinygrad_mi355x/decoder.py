@@ -8,7 +8,8 @@ that consumer, the one that turns the packed kernels into tokens per second:
 * attention projections: INT4 weights with fp16 scales per 128 K-elements; q, k and v rows
   are stacked into one weight so that a token needs one QKV product;
 * feed-forward: FP4 E2M1 weights with E8M0 scales per 32; gate and up rows interleaved in one
-  weight, so that the one-token GEMV applies SwiGLU in its epilogue;
+  weight, so that the one-token GEMV applies SwiGLU in its epilogue; with ``experts``, as many such blocks a layer and a
+  bf16 router that chooses among them (tinygrad_mi355x.experts);
 * embeddings and output head: bf16; RMSNorm weights bf16; residual stream fp32;
 * RoPE (rotate-half pairs, base 10000) and grouped-query attention over a bf16 KV cache.
 
@@ -30,6 +31,7 @@ from dataclasses import dataclass
 import torch
 
 from tinygrad_mi355x.codegen.decomp.mi355x import PackedTensor, quantize_mx
+from tinygrad_mi355x.experts import SCORES, PackedExperts
 from tinygrad_mi355x.runtime import kernels as K
 from tinygrad_mi355x.runtime.graph import StreamGraph
 
@@ -58,16 +60,21 @@ class DecoderConfig:
     eps: float = 1e-5
     rope_base: float = 10000.0
     attn_group: int = 128  # INT4 scale group along K
+    experts: int = 0  # feed-forward blocks of a layer to choose from; 0: one block, no router
+    experts_per_token: int = 2
+    router_score: str = "softmax"
 
     @property
     def qkv_rows(self) -> int:
         return (self.heads + 2 * self.kv_heads) * self.head_dim
 
     def weight_bytes_per_token(self) -> int:
-        """Weight bytes one decode step streams: packed layers plus the bf16 output head."""
+        """Weight bytes one decode step of one token streams: packed layers plus the bf16 output head."""
         d, f = self.hidden, self.ffn
         attn = (self.qkv_rows + d) * d // 2 + (self.qkv_rows + d) * (d // self.attn_group) * 2
         ffn = 3 * d * f // 2 + 3 * d * f // 32
+        if self.experts:
+            ffn = self.experts_per_token * ffn + self.experts * d * 2
         norms = 2 * d * 2
         return self.layers * (attn + ffn + norms) + self.vocab * d * 2 + d * 2
 
@@ -78,8 +85,9 @@ class LayerWeights:
     wqkv: PackedTensor           # int4 [(H + 2 HK) hd, D], fp16 scales per attn_group
     wo: PackedTensor             # int4 [D, H hd]
     ffn_norm: torch.Tensor       # bf16 [D]
-    w_gate_up: PackedTensor      # fp4 [2 F, D], E8M0 per 32; row 2 i is gate i, row 2 i + 1 is up i
-    w_down: PackedTensor         # fp4 [D, F]
+    w_gate_up: PackedTensor      # fp4 [2 F, D], E8M0 per 32; row 2 i is gate i, row 2 i + 1 is up i (of E experts [E, 2 F, D])
+    w_down: PackedTensor         # fp4 [D, F] ([E, D, F])
+    router: torch.Tensor | None = None  # bf16 [E, D]
 
 
 @dataclass
@@ -94,7 +102,7 @@ def random_weights(cfg: DecoderConfig, device: str | torch.device = "cuda", seed
     """Synthetic random-init weights of the configured shape, generated on the device.
 
     INT4 codes are uniform over all 16 nibbles with scales in [0.002, 0.005]; FP4 weights are
-    N(0, 0.02) MX-quantised along K; norms 1 + 0.1 N(0, 1); embeddings N(0, 1); head N(0, 0.02).
+    N(0, 0.02) MX-quantised along K; norms 1 + 0.1 N(0, 1); embeddings N(0, 1); head and routers N(0, 0.02).
     """
     g = torch.Generator(device=device)
     g.manual_seed(seed)
@@ -105,23 +113,26 @@ def random_weights(cfg: DecoderConfig, device: str | torch.device = "cuda", seed
         scales = (torch.rand((n, k // cfg.attn_group), device=device, generator=g) * 0.003 + 0.002).to(torch.float16)
         return PackedTensor(data, "int4", (n, k), scales, cfg.attn_group)
 
-    def fp4(n: int, k: int) -> PackedTensor:
-        return quantize_mx(torch.randn((n, k), device=device, generator=g) * 0.02, "fp4_e2m1")
+    def fp4(*shape: int) -> PackedTensor:
+        return quantize_mx(torch.randn(shape, device=device, generator=g) * 0.02, "fp4_e2m1")
 
     def norm() -> torch.Tensor:
         return (1.0 + 0.1 * torch.randn(d, device=device, generator=g)).to(torch.bfloat16)
 
-    layers = []
+    layers, per = [], (cfg.experts,) if cfg.experts else ()
     for _ in range(cfg.layers):
         layers.append(LayerWeights(norm(), int4(cfg.qkv_rows, d), int4(d, cfg.heads * cfg.head_dim), norm(),
-                                   fp4(2 * cfg.ffn, d), fp4(d, cfg.ffn)))
+                                   fp4(*per, 2 * cfg.ffn, d), fp4(*per, d, cfg.ffn)))
+        if cfg.experts:
+            layers[-1].router = (torch.randn((cfg.experts, d), device=device, generator=g) * 0.02).to(torch.bfloat16)
     embed = torch.randn((cfg.vocab, d), device=device, generator=g).to(torch.bfloat16)
     final_norm = norm()
     lm_head = (torch.randn((cfg.vocab, d), device=device, generator=g) * 0.02).to(torch.bfloat16)
     return DecoderWeights(embed, layers, final_norm, lm_head)
 
 
-_LAYER_FIELDS = ("attn_norm", "wqkv", "wo", "ffn_norm", "w_gate_up", "w_down")
+def _layer_fields(cfg: DecoderConfig) -> tuple[str, ...]:
+    return ("attn_norm", "wqkv", "wo", "ffn_norm", "w_gate_up", "w_down") + (("router",) if cfg.experts else ())
 
 
 def save_weights(path, w: DecoderWeights, cfg: DecoderConfig) -> None:
@@ -132,7 +143,7 @@ def save_weights(path, w: DecoderWeights, cfg: DecoderConfig) -> None:
 
     tensors = {"embed": w.embed, "final_norm": w.final_norm, "lm_head": w.lm_head}
     for i, layer in enumerate(w.layers):
-        for field in _LAYER_FIELDS:
+        for field in _layer_fields(cfg):
             tensors[f"layers.{i}.{field}"] = getattr(layer, field)
     checkpoint.save(path, tensors, {"decoder": asdict(cfg)})
 
@@ -146,7 +157,8 @@ def load_weights(path, device: str | torch.device = "cuda") -> tuple[DecoderWeig
         raise ValueError(f"{path} holds no decoder configuration")
     cfg = DecoderConfig(**meta["decoder"])
     try:
-        layers = [LayerWeights(*(tensors[f"layers.{i}.{field}"] for field in _LAYER_FIELDS)) for i in range(cfg.layers)]
+        layers = [LayerWeights(*(tensors[f"layers.{i}.{field}"] for field in _layer_fields(cfg)))
+                  for i in range(cfg.layers)]
         weights = DecoderWeights(tensors["embed"], layers, tensors["final_norm"], tensors["lm_head"])
     except KeyError as error:
         raise ValueError(f"{path} lacks decoder tensor {error}") from error
@@ -207,8 +219,11 @@ class Decoder:
         self.xnb = torch.empty((rows, d), dtype=torch.bfloat16, device=dev)
         self.qkv = torch.empty((rows, cfg.qkv_rows), **f32)
         self.attn = torch.empty((rows, cfg.heads * cfg.head_dim), dtype=torch.float16, device=dev)
-        self.gu = torch.empty((rows, 2 * cfg.ffn), **f32)
-        self.act = torch.empty((rows, cfg.ffn), dtype=torch.bfloat16, device=dev)
+        if cfg.experts:
+            self._allocate_experts(rows)
+        else:
+            self.gu = torch.empty((rows, 2 * cfg.ffn), **f32)
+            self.act = torch.empty((rows, cfg.ffn), dtype=torch.bfloat16, device=dev)
         self.logits = torch.empty((batch, cfg.vocab), **f32)
         self._allocate_cache()
         # decode attention: one pass or position splits (ONE_PASS_SHORT_LEN)
@@ -234,7 +249,7 @@ class Decoder:
         self.fuse_swiglu_rows = cfg.hidden % 128 == 0
         # one token: each RMSNorm runs inside the projection after it (tgm_dec_norm_gemv), the
         # residual stream alternating between h and h_alt
-        self.fuse_norm = (batch == 1 and cfg.hidden in (2048, 4096) and self.fuse_swiglu
+        self.fuse_norm = (batch == 1 and not cfg.experts and cfg.hidden in (2048, 4096) and self.fuse_swiglu
                           and all(_norm_gemv_fits(L.wqkv, False) and _norm_gemv_fits(L.w_gate_up, True)
                                   for L in weights.layers))
         self.h_alt = torch.empty((batch, d), **f32) if self.fuse_norm else None
@@ -243,7 +258,7 @@ class Decoder:
         # activations for 64 weight rows instead of all 14336 columns for 16 rows
         # (4096 x 14336 at 8 tokens: 13.7 -> 10.8 us)
         wd = weights.layers[0].w_down
-        self.down_slices = cfg.ffn // 2048 if (batch >= 5 and cfg.ffn % 2048 == 0 and 2 <= cfg.ffn // 2048 <= 16
+        self.down_slices = cfg.ffn // 2048 if (batch >= 5 and not cfg.experts and cfg.ffn % 2048 == 0 and 2 <= cfg.ffn // 2048 <= 16
                                                and wd.format in ("fp4_e2m1", "fp6_e2m3", "fp6_e3m2")
                                                and (wd.scales is None or wd.block_size == 32)) else 1
         self.delta_parts = torch.empty((self.down_slices, batch, d), **f32) if self.down_slices > 1 else None
@@ -260,10 +275,44 @@ class Decoder:
         # "h" the residual after attention and "delta" the feed-forward output (fp32, the layer's
         # output is their sum), "x16" the normed f16 input of the QKV projection, "attn" the f16
         # attention output, "xb" the normed bf16 input of gate|up and "act" the bf16 SwiGLU
-        # output; "x16" and "xb" are None when the norm runs inside the projection
+        # output; "x16" and "xb" are None when the norm runs inside the projection; of experts
+        # "act" is None, and "router" (fp32 logits), "ids" and "expert_weights" are the choice
         self.layer_trace: list[dict[str, torch.Tensor | None]] | None = None
 
     # ---------------------------------------------------------------- building blocks
+    def _allocate_experts(self, rows: int) -> None:
+        cfg = self.cfg
+        if not 1 <= cfg.experts_per_token <= cfg.experts or cfg.router_score not in SCORES:
+            raise ValueError(f"experts_per_token must be 1 to {cfg.experts} and router_score one of {tuple(SCORES)}")
+        self.experts = [PackedExperts(L.w_gate_up, L.w_down) for L in self.w.layers]
+        for L, e in zip(self.w.layers, self.experts):
+            if (e.experts, e.hidden, e.ffn, e.dtype) != (cfg.experts, cfg.hidden, cfg.ffn, torch.bfloat16):
+                raise ValueError(f"a layer must hold {cfg.experts} experts of {cfg.hidden} x {cfg.ffn} in an FP4 or FP6 format")
+            if L.router is None or L.router.shape != (cfg.experts, cfg.hidden) or L.router.dtype is not torch.bfloat16:
+                raise ValueError(f"a layer's router must be bfloat16 [{cfg.experts}, {cfg.hidden}]")
+        f32, k = dict(dtype=torch.float32, device=self.device), cfg.experts_per_token
+        self.router_logits = torch.empty((rows, cfg.experts), **f32)
+        self.expert_ids = torch.empty((rows, k), dtype=torch.int32, device=self.device)
+        self.expert_weights = torch.empty((rows, k), **f32)
+        # of the longest pass: shorter ones need no more
+        self.expert_workspace = torch.empty(max(e.workspace_bytes(rows, k) for e in self.experts), dtype=torch.uint8,
+                                            device=self.device)
+
+    def _run_experts(self, li: int, rows: int, stream: int) -> None:
+        """The feed-forward output of layer ``li`` from ``xnb``, through each token's experts, into ``delta``."""
+        cfg, d, k, router = self.cfg, self.cfg.hidden, self.cfg.experts_per_token, self.w.layers[li].router
+        if rows <= 8 and rows * d <= 32768:
+            K.call("tgm_dec_gemv_bf16", router.data_ptr(), cfg.experts, d, self.xnb.data_ptr(), rows, d,
+                   self.router_logits.data_ptr(), cfg.experts, stream)
+        else:
+            K.call("tgm_gemm_dense", self.xnb.data_ptr(), BF16, rows, d, router.data_ptr(), BF16, cfg.experts, d, d,
+                   self.router_logits.data_ptr(), F32, cfg.experts, stream)
+        K.call("tgm_route", self.router_logits.data_ptr(), F32, rows, cfg.experts, cfg.experts, None, SCORES[cfg.router_score],
+               1, 1, k, 1, 1.0, self.expert_ids.data_ptr(), self.expert_weights.data_ptr(), stream)
+        K.call("tgm_experts_apply", self.experts[li].arg, self.xnb.data_ptr(), BF16, rows, d, self.expert_ids.data_ptr(),
+               self.expert_weights.data_ptr(), k, self.delta.data_ptr(), F32, d, self.expert_workspace.data_ptr(),
+               self.expert_workspace.numel(), stream)
+
     def _allocate_cache(self) -> None:
         cfg = self.cfg
         cache = (cfg.layers, self.batch, cfg.kv_heads, self.max_seq, cfg.head_dim)
@@ -322,6 +371,10 @@ class Decoder:
                 continue
             K.call("tgm_dec_add_rmsnorm", self.h.data_ptr(), self.delta.data_ptr(), rows, d, L.ffn_norm.data_ptr(),
                    cfg.eps, self.xnb.data_ptr(), BF16, stream)
+            if cfg.experts:
+                self._run_experts(li, rows, stream)
+                self._trace(rows)
+                continue
             if (rows == 1 and self.fuse_swiglu) or (1 < rows <= GEMV_MAX_ROWS and self.fuse_swiglu_rows):
                 w = L.w_gate_up  # gate|up GEMV with the SwiGLU epilogue
                 K.call("tgm_gemv_swiglu", w.data.data_ptr(), K.FORMAT_IDS[w.format], 2 * cfg.ffn, d, K.ptr(w.scales),
@@ -372,9 +425,13 @@ class Decoder:
                 delta = held[0].clone()
                 for p in range(1, parts):
                     delta += held[p]
+            choice = {}
+            if self.cfg.experts:
+                choice = {"router": self.router_logits[:rows].clone(), "ids": self.expert_ids[:rows].clone(),
+                          "expert_weights": self.expert_weights[:rows].clone()}
             self.layer_trace.append({
-                "h": self.h[:rows].clone(), "delta": delta, "attn": self.attn[:rows].clone(),
-                "act": self.act[:rows].clone(), "x16": None if fused_norm else self.xn16[:rows].clone(),
+                **choice, "h": self.h[:rows].clone(), "delta": delta, "attn": self.attn[:rows].clone(),
+                "act": None if choice else self.act[:rows].clone(), "x16": None if fused_norm else self.xn16[:rows].clone(),
                 "xb": None if fused_norm else self.xnb[:rows].clone()})
 
     def _prefill_attention(self, rows: int, t: int, kc: torch.Tensor, vc: torch.Tensor, stream: int) -> None:

@@ -133,7 +133,7 @@ class PackedExperts:
         self.dtype = torch.float16 if integer else torch.bfloat16  # of the activations
         dt, block = _scales(gate_up)
         # struct tgm_experts; the weights are never replaced
-        self._arg = struct.pack("PPPPqqqqqq", gate_up.data.data_ptr(), K.ptr(gate_up.scales) or 0, down.data.data_ptr(),
+        self.arg = struct.pack("PPPPqqqqqq", gate_up.data.data_ptr(), K.ptr(gate_up.scales) or 0, down.data.data_ptr(),
                                 K.ptr(down.scales) or 0, self.experts, self.hidden, self.ffn, K.FORMAT_IDS[gate_up.format],
                                 -1 if dt is None else K.dtype_id(dt), block)
         self._plans = Plans()
@@ -160,9 +160,13 @@ class PackedExperts:
             # the workspace is of the caching allocator, so that calls on several streams never share one; held until the
             # launches, or another thread's call on this stream could be given its memory before them
             workspace = x.new_empty(need, dtype=torch.uint8)
-            K.call("tgm_experts_apply", self._arg, x.data_ptr(), *head, ids.data_ptr(), weights.data_ptr(), top_k,
+            K.call("tgm_experts_apply", self.arg, x.data_ptr(), *head, ids.data_ptr(), weights.data_ptr(), top_k,
                    out.data_ptr(), *tail, workspace.data_ptr(), need, K.stream_on(index))
         return out
+
+    def workspace_bytes(self, tokens: int, top_k: int) -> int:
+        """The workspace that a call on so many tokens takes, which one on fewer can take too."""
+        return K.load_library().tgm_experts_workspace(self.arg, tokens, top_k)
 
     def _apply_plan(self, sig, x, ids, weights, out) -> tuple:
         _check_rows(x, "x", self.hidden)
@@ -186,7 +190,7 @@ class PackedExperts:
         if ldx % 8 and tokens > 1:
             raise ValueError(f"rows of x must be 16-byte aligned, got a stride of {ldx}")
         K.require_device(x)
-        need = K.load_library().tgm_experts_workspace(self._arg, tokens, ids.shape[1])
+        need = self.workspace_bytes(tokens, ids.shape[1])
         return self._plans.keep(sig, ((_DT[x.dtype], tokens, ldx), ids.shape[1], (_DT[odt], ldy), need, x.get_device()))
 
 

@@ -6,7 +6,7 @@ The reference has no model code (see ``decoder``).  ``ServingDecoder`` is ``Deco
 * any ``Rotary`` positions (layouts, partial heads, scaled frequencies) in place of the fixed ones;
 * prompts of any length, in chunks of ``max_prompt`` tokens over what is cached of them;
 * a common prefix: stored once, run through the model once, and read once per step for the whole batch;
-* ``sample`` in place of the greedy choice.
+* ``sample`` in place of the greedy choice, and ``log_probs`` of what it drew.
 
 ``python -m tinygrad_mi355x.serving`` runs it on random weights.
 """
@@ -23,7 +23,7 @@ from tinygrad_mi355x.decoder import Decoder, DecoderConfig, DecoderWeights, rand
 from tinygrad_mi355x.kv_cache import PackedKVCache
 from tinygrad_mi355x.rotary import Rotary
 from tinygrad_mi355x.runtime import kernels as K
-from tinygrad_mi355x.sampling import sample
+from tinygrad_mi355x.sampling import MAX_TOP, LogProbs, log_probs, sample
 
 
 class ServingDecoder(Decoder):
@@ -136,19 +136,31 @@ class ServingDecoder(Decoder):
         return graph
 
     def generate(self, prompts: torch.Tensor, new_tokens: int, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0,
-                 min_p=0.0, graph: bool = True) -> torch.Tensor:
+                 min_p=0.0, graph: bool = True, logprobs: int | None = None) -> torch.Tensor | tuple[torch.Tensor, LogProbs]:
         """[batch, new_tokens] sampled token ids; ``u`` float32 [batch, new_tokens] in [0, 1) are the random numbers,
-        the filters (``sampling.sample``) one number or one per sequence."""
+        the filters (``sampling.sample``) one number or one per sequence.
+
+        With ``logprobs`` (0 to 64) also what ``log_probs`` tells of them and of so many alternatives, [batch, new_tokens] and
+        [batch, new_tokens, logprobs]: of the model's own distribution, without temperature or filters."""
         if new_tokens < 1 or self.prefix + prompts.shape[1] + new_tokens - 1 > self.max_seq:
             raise ValueError("prefix + prompt + generated tokens exceed max_seq")
         if u.shape != (self.batch, new_tokens) or u.dtype is not torch.float32 or u.device != self.device:
             raise ValueError(f"u must be float32 [{self.batch}, {new_tokens}] on {self.device}")
+        if logprobs is not None and not 0 <= logprobs <= min(MAX_TOP, self.cfg.vocab):
+            raise ValueError(f"logprobs must be 0 to {min(MAX_TOP, self.cfg.vocab)}, got {logprobs}")
         for name, value in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
             held = self._filters[name]
             held.copy_(torch.as_tensor(value, dtype=held.dtype, device=self.device).expand(self.batch))
         history = torch.empty((self.batch, new_tokens), dtype=torch.int32, device=self.device)
+        told = []
+
+        def tell() -> None:
+            if logprobs is not None:
+                told.append(log_probs(self.logits, self.tokens[:self.batch], top=logprobs))
+
         self.u.copy_(u[:, 0])
         history[:, 0] = self.prefill(prompts)
+        tell()
         step = self._decode_step
         for i in range(1, new_tokens):
             # the first step runs eagerly: it also performs every kernel's one-time set-up
@@ -157,7 +169,8 @@ class ServingDecoder(Decoder):
             self.u.copy_(u[:, i])
             step()
             history[:, i] = self.tokens[:self.batch]
-        return history
+            tell()
+        return history if logprobs is None else (history, LogProbs(*(torch.stack(steps, 1) for steps in zip(*told))))
 
 
 def main() -> None:
@@ -168,8 +181,11 @@ def main() -> None:
     p.add_argument("--prompt", type=int, default=200)
     p.add_argument("--new", type=int, default=64)
     p.add_argument("--v-format", default="fp8_e4m3")
+    p.add_argument("--experts", type=int, default=0, help="experts of a layer (0: one feed-forward block)")
+    p.add_argument("--experts-per-token", type=int, default=2)
+    p.add_argument("--logprobs", type=int, help="tell the log probabilities of the tokens and of so many alternatives")
     a = p.parse_args()
-    cfg = DecoderConfig(layers=a.layers)
+    cfg = DecoderConfig(layers=a.layers, experts=a.experts, experts_per_token=a.experts_per_token)
     max_seq = 64 * math.ceil((a.prefix + a.prompt + a.new) / 64)
     rotary = Rotary(cfg.head_dim, base=cfg.rope_base, scaling=dict(kind="yarn", factor=4.0, trained=4096))
     d = ServingDecoder(random_weights(cfg), cfg, a.batch, max_seq, 512, prefix=a.prefix, v_format=a.v_format, rotary=rotary)
@@ -180,11 +196,15 @@ def main() -> None:
     for _ in range(2):  # the first one sets kernels up
         torch.cuda.synchronize()
         start = time.perf_counter()
-        out = d.generate(tokens[a.prefix:].view(a.batch, a.prompt), a.new, u, temperature=0.8, top_k=50, top_p=0.95)
+        out = d.generate(tokens[a.prefix:].view(a.batch, a.prompt), a.new, u, temperature=0.8, top_k=50, top_p=0.95,
+                         logprobs=a.logprobs)
         torch.cuda.synchronize()
         took = time.perf_counter() - start
     print(f"{a.batch} sequences of {a.prompt} tokens behind {a.prefix} common ones, {a.new} sampled each: {took * 1e3:.1f} ms, "
           f"cache {sum(c.nbytes() for c in d.caches) / 2**20:.1f} MiB")
+    if a.logprobs is not None:
+        out, told = out
+        print("log probabilities", [[round(x, 2) for x in row] for row in told.logprobs[:, :12].tolist()])
     print(out[:, :12].tolist())
 
 
