@@ -290,3 +290,29 @@ def test_routed_experts(dev):
         ids, weights = X.route(np64(logits), 4, "sigmoid", np64(randn(dev, 3, 16, scale=0.1)), 4, 2)
         routes(r, (ids, weights))
         layer.check(layer.e.apply(x, r.ids, r.weights), x, r.ids, r.weights)
+
+
+@pytest.mark.parametrize("fmt,scales,block", [("fp4_e2m1", "e8m0", 32), ("fp6_e2m3", "e8m0", 32), ("int4", F16, 32)])
+@pytest.mark.parametrize("experts,hidden,ffn,tokens,top_k", [(64, 128, 1152, 600, 4), (64, 512, 1152, 300, 4), (24, 256, 2176, 700, 5),
+                                                             (64, 640, 384, 60, 8)])
+def test_more_tiles_than_workgroups(dev, fmt, scales, block, experts, hidden, ffn, tokens, top_k):
+    """Workgroups that go through several tiles, of one K step up to more than are loaded ahead."""
+    print(f"tiles {fmt} {experts} {hidden} {ffn} {tokens}", flush=True)
+    layer = Layer(dev, fmt, experts, hidden, ffn, scales, block)
+    ids, weights = choice(dev, tokens, tokens, experts, top_k)
+    x = randn(dev, tokens, tokens, hidden, dtype=layer.e.dtype, scale=0.5)
+    got = layer.e.apply(x, ids, weights)
+    layer.check(got, x, ids, weights)
+    for _ in range(3):
+        assert torch.equal(layer.e.apply(x, ids, weights), got)
+
+
+@pytest.mark.parametrize("tokens", [3, 40, 200])
+def test_gates_of_every_size(dev, tokens):
+    """Gates from 0 to a few hundred, of both signs: silu is the gate, or nothing."""
+    layer = Layer(dev, "fp4_e2m1", 4, 256, 256)
+    ids, weights = choice(dev, 1, tokens, 4, 2)
+    x = randn(dev, 2, tokens, 256, dtype=BF16) * torch.logspace(-3, 2.5, tokens, device=dev)[:, None].to(BF16)
+    gates = np64(x) @ layer.gate_up[0][::2].T
+    assert gates.max() > 90 and gates.min() < -90
+    layer.check(layer.e.apply(x, ids, weights, out=torch.empty((tokens, 256), device=dev)), x, ids, weights)

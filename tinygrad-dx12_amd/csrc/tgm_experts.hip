@@ -6,9 +6,9 @@
 //
 //   experts_plan  puts the pairs in the order of their experts (a position each), and cuts each expert's positions into
 //                 tiles of rows;
-//   gemm_w_tile   gate|up over those tiles, the rows of x gathered as they are loaded, silu(gate) * up in the epilogue:
+//   gemm_w_group  gate|up over those tiles, the rows of x gathered as they are loaded, silu(gate) * up in the epilogue:
 //                 the hidden activations [position, ffn] in x's type;
-//   gemm_w_tile   down over the same tiles: a row of fp32 per position;
+//   gemm_w_group  down over the same tiles: a row of fp32 per position;
 //   experts_sum   each token's rows, weighted and summed in the order of its choices.
 //
 // The count of tiles is known on the device alone: a launch covers the most that the pairs can make, and workgroups past
@@ -136,11 +136,11 @@ static ExpertSizes expert_sizes(const tgm_experts& e, int64_t tokens, int64_t to
   };
   for (int i = 0; i < kExpertTileKinds; ++i) {
     // every expert that a pair names may end in a tile that is not full
-    z.most[i] = z.pairs / kExpertRows[i] + (z.pairs < e.experts ? z.pairs : e.experts);
+    z.most[i] = z.pairs / expert_rows(e.format, i) + (z.pairs < e.experts ? z.pairs : e.experts);
     most = z.most[i] > most ? z.most[i] : most;
   }
   z.tiles = take(16 * (1 + most) > (int64_t)sizeof(FewList) ? 16 * (1 + most) : (int64_t)sizeof(FewList));
-  z.source = take(4 * z.pairs);
+  z.source = take(4 * z.pairs);  // read in whole groups of 4 up to a tile's height: at most 512 bytes on, of what follows
   z.place = take(4 * z.pairs);
   z.hidden = take(2 * z.pairs * e.ffn);
   z.rows = take(4 * z.pairs * e.hidden);
@@ -152,17 +152,18 @@ static ExpertSizes expert_sizes(const tgm_experts& e, int64_t tokens, int64_t to
 static double experts_named(const tgm_experts& e, int64_t pairs) {
   return (double)e.experts * (1.0 - pow(1.0 - 1.0 / (double)e.experts, (double)pairs));
 }
-// Rows of the tiles by the rows of x that an expert has on average.  us of the two products of 64 experts of 2048 x 1408 with 32,
-// 64 and 128 rows, FP4: 6 rows an expert 80, 86, -; 24 rows 105, 108, 116; 192 rows -, 331, 303.  FP6, 32 experts, 64 rows
-// 131, 117, 130.
+// Rows of the tiles by the rows of x that an expert has on average: the kind of tile.  us of the two products of 64 (FP6: 32)
+// experts of 2048 x 1408 on tiles of 32, 64 and 128 (96) rows.  FP4: 24 rows an expert 100, 101, 103; 48 rows 132, 123, 132;
+// 72 rows 169, 150, 163; 96 rows 195, 170, 170; 192 rows -, -, 257.  FP6: 32 rows -, 90, 94; 48 rows -, 91, 100; 64 rows 130,
+// 110, 99; 96 rows -, 124, 126; 192 rows -, 328, 293.
 static int expert_tile(const tgm_experts& e, int64_t pairs) {
   const double mean = (double)pairs / experts_named(e, pairs);
-  return mean <= 32.0 ? 0 : mean <= 96.0 ? 1 : 2;
+  return mean <= 32.0 ? 0 : mean <= (expert_rows(e.format, 2) == 96 ? 56.0 : 96.0) ? 1 : 2;
 }
 // Whether tiles of 256 columns are enough to give every compute unit one.  INT4, 17 tile rows x 4096: 38 us, and 41 on 128 columns;
 // FP4, 8 tile rows x 4096: 103 and 68.
 static bool expert_wide(const tgm_experts& e, int64_t pairs, int64_t columns, int shape, int cus) {
-  const double named = experts_named(e, pairs), rows = named + (double)(pairs / kExpertRows[shape]) / 2;
+  const double named = experts_named(e, pairs), rows = named + (double)(pairs / expert_rows(e.format, shape)) / 2;
   return rows * (double)((columns + 255) / 256) >= cus;
 }
 
@@ -270,7 +271,7 @@ extern "C" int tgm_experts_apply(const tgm_experts* experts, const void* x, int6
   TGM_CHECK_ARG(z.most[shape] * ((most_columns + 127) / 128) < (1ll << 31), "too many tiles");
   PlanArgs plan;
   plan.ids = ids, plan.pairs = (int)z.pairs, plan.top_k = (int)top_k, plan.experts = (int)e.experts;
-  plan.rows = kExpertRows[shape];
+  plan.rows = expert_rows(e.format, shape);
   plan.tiles = (int*)(ws + z.tiles), plan.source = (int*)(ws + z.source), plan.place = (int*)(ws + z.place);
   hipLaunchKernelGGL(experts_plan, dim3(1), dim3(kPlanThreads), 0, st, plan);
   if (const int status = launch_status("tgm_experts_apply"); status != TGM_OK) return status;
@@ -283,7 +284,7 @@ extern "C" int tgm_experts_apply(const tgm_experts* experts, const void* x, int6
     p.c = ws + (up ? z.hidden : z.rows);
     p.ldc = up ? e.ffn : e.hidden;
     p.lda_bytes = (unsigned)(2 * (up ? ldx : e.ffn));
-    p.M = 0, p.N = (int)(up ? 2 * e.ffn : e.hidden), p.K = (int)(up ? e.hidden : e.ffn);
+    p.N = (int)(up ? 2 * e.ffn : e.hidden), p.K = (int)(up ? e.hidden : e.ffn);
     p.cdt = up ? (int)x_dtype : TGM_F32, p.sdt = (int)e.scale_dtype, p.is_signed = e.format == TGM_FMT_INT4;
     p.swiglu = up;
     p.tiles = plan.tiles, p.rows = up ? plan.source : nullptr;

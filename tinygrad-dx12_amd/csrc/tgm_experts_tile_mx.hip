@@ -1,5 +1,5 @@
-// The grouped products of tgm_experts_apply (tgm_gemm_w_tile.h) for FP4 and FP6 weights.
-#include "tgm_experts.h"
+// The grouped products of tgm_experts_apply (tgm_experts_tile.h) for FP4 and FP6 weights.
+#include "tgm_experts_tile.h"
 
 namespace tgm {
 
@@ -8,9 +8,9 @@ template <int F>
 static int launch_kind(const WGroupArgs& p, int shape, bool wide, int64_t most, hipStream_t st) {
   constexpr bool FP4 = F == TGM_FMT_FP4_E2M1;
   if (shape == 0)
-    return wide ? launch_experts_tile<F, 1, 8, 1, FP4 ? 3 : 2>(p, most, st) : launch_experts_tile<F, 1, 4, 1, FP4 ? 4 : 3>(p, most, st);
-  if (shape == 1) return wide ? launch_experts_tile<F, 2, 8, 1, 3>(p, most, st) : launch_experts_tile<F, 2, 4, 1, 3>(p, most, st);
-  return wide ? launch_experts_tile<F, 4, 8, 1, FP4 ? 3 : 2>(p, most, st) : launch_experts_tile<F, 4, 4, 1, 3>(p, most, st);
+    return wide ? launch_experts_tile<F, 1, 8, FP4 ? 3 : 2>(p, most, st) : launch_experts_tile<F, 1, 4, FP4 ? 4 : 3>(p, most, st);
+  if (shape == 1) return wide ? launch_experts_tile<F, 2, 8, 3>(p, most, st) : launch_experts_tile<F, 2, 4, 3>(p, most, st);
+  return wide ? launch_experts_tile<F, FP4 ? 4 : 3, 8, 3>(p, most, st) : launch_experts_tile<F, FP4 ? 4 : 3, 4, 3>(p, most, st);
 }
 
 int launch_experts_tile_mx(const WGroupArgs& p, int fmt, int shape, bool wide, int64_t most, hipStream_t st) {

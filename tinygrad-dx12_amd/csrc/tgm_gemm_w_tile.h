@@ -47,8 +47,6 @@
 // scale is added to the accumulator.
 #pragma once
 
-#include <type_traits>
-
 #include "tgm_mfma_common.h"
 
 namespace tgm {
@@ -70,7 +68,6 @@ constexpr int kind_scale_bytes(int kind) { return kind & 1 ? 4 : 2; }
 constexpr int kWtK = 128;  // K step
 
 struct WTileArgs {
-  static constexpr bool kGrouped = false;
   const uint8_t* a;
   const uint8_t* w;
   const uint8_t* scales;  // E8M0 bytes [N, K / 32] or INT4 group scales [N, K / G] of dtype sdt; null = unscaled
@@ -81,16 +78,6 @@ struct WTileArgs {
   int steps_per_split;  // > 0: blockIdx.y takes that many K steps and writes its fp32 product to part [splits][M][N]
   float* part;
   int swiglu;  // rows of W interleave gate and up: C has N / 2 columns, silu(gate) * up
-};
-
-// The same product for the rows of many experts, each with a weight of its own (tgm_experts.hip): tile row tm is entry tm
-// of a list that lies on the device, the count of them before it.  M and the rows of A are those of one entry.
-struct WGroupArgs : WTileArgs {
-  static constexpr bool kGrouped = true;
-  const int* tiles;           // [0] count; from [4] on, per tile {expert, first position, positions, 0}
-  const int* rows;            // row of A at each position; null: the position itself
-  unsigned a_bytes;           // of all rows of A, where rows name them
-  int64_t w_bytes, s_bytes;   // of an expert's codes and scales
 };
 
 // 16-bit values to LDS, one zero-extended dword per lane.
@@ -186,10 +173,10 @@ struct WTile {
   static constexpr bool kFits = 8 * FA % WN == 0 && kLoads * (NBUF - 1) < 64 && kLds <= 160 * 1024;
 };
 
-template <int KIND, int FA, int WN, int WK, int NBUF, class Args = WTileArgs>
+template <int KIND, int FA, int WN, int WK, int NBUF>
 __global__ void __launch_bounds__(64 * WN * WK) 
 __attribute__((amdgpu_waves_per_eu(WTile<KIND, FA, WN, WK, NBUF>::kOccupancy, WTile<KIND, FA, WN, WK, NBUF>::kOccupancy)))
-gemm_w_tile(Args p) {
+gemm_w_tile(WTileArgs p) {
   using T = WTile<KIND, FA, WN, WK, NBUF>;
   constexpr bool I4 = T::kI4;
   constexpr int G = T::kG;
@@ -197,42 +184,20 @@ gemm_w_tile(Args p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wave % WN, wk = wave / WN;
-  int tiles_m = (p.M + T::kBM - 1) / T::kBM;
-  const int tiles_n = (p.N + T::kBN - 1) / T::kBN;
+  const int tiles_m = (p.M + T::kBM - 1) / T::kBM, tiles_n = (p.N + T::kBN - 1) / T::kBN;
   int tm, tn;
-  if constexpr (Args::kGrouped) {  // the launch covers the most tiles that the rows can make
-    tiles_m = p.tiles[0];
-    if ((int)blockIdx.x >= tiles_m * tiles_n) return;
-  }
   tile_of_ranges(blockIdx.x, p.K, tiles_m, tiles_n, 8, tm, tn);
-  const int n0 = tn * T::kBN;
-  int m0 = tm * T::kBM, m_end = p.M;
-  const uint8_t *pa = p.a, *pw = p.w, *ps = p.scales;
-  unsigned a_bytes = (unsigned)(p.M - 1) * p.lda_bytes + (unsigned)p.K * 2u;
-  if constexpr (Args::kGrouped) {
-    const int* entry = p.tiles + 4 + 4 * tm;
-    const int expert = __builtin_amdgcn_readfirstlane(entry[0]);
-    m0 = __builtin_amdgcn_readfirstlane(entry[1]);
-    m_end = m0 + __builtin_amdgcn_readfirstlane(entry[2]);
-    pw += expert * p.w_bytes;
-    ps += p.scales ? expert * p.s_bytes : 0;
-    if (p.rows) {
-      a_bytes = p.a_bytes;
-    } else {
-      pa += (int64_t)m0 * p.lda_bytes;
-      a_bytes = (unsigned)(m_end - m0 - 1) * p.lda_bytes + (unsigned)p.K * 2u;
-    }
-  }
+  const int m0 = tm * T::kBM, n0 = tn * T::kBN;
   // split K (WK == 1 shapes only): steps s_begin .. of this workgroup
-  const int s_begin = !Args::kGrouped && WK == 1 && p.part ? (int)blockIdx.y * p.steps_per_split : 0;
-  const int nsteps = !Args::kGrouped && WK == 1 && p.part ? min(p.steps_per_split, p.K / kWtK - s_begin) : p.K / kWtK;
+  const int s_begin = WK == 1 && p.part ? (int)blockIdx.y * p.steps_per_split : 0;
+  const int nsteps = WK == 1 && p.part ? min(p.steps_per_split, p.K / kWtK - s_begin) : p.K / kWtK;
   const int nstages = (nsteps + WK - 1) / WK;
   const unsigned kbw = (unsigned)p.K / 8u * (T::kRow == 64 ? 4u : 6u);  // packed bytes per W row
-  const i32x4v ra = buffer_rsrc(pa, a_bytes);
-  const i32x4v rw = buffer_rsrc(pw, (unsigned)p.N * kbw);
+  const i32x4v ra = buffer_rsrc(p.a, (unsigned)(p.M - 1) * p.lda_bytes + (unsigned)p.K * 2u);
+  const i32x4v rw = buffer_rsrc(p.w, (unsigned)p.N * kbw);
   constexpr unsigned ssize = (unsigned)kind_scale_bytes(KIND);                   // INT4 scale bytes
   const unsigned srow = I4 ? (G ? (unsigned)(p.K / (G ? G : 1)) * ssize : 0u) : (unsigned)p.K / 32u;  // scale bytes per W row
-  const i32x4v rs = buffer_rsrc(ps, p.scales ? (unsigned)p.N * srow : 0u);
+  const i32x4v rs = buffer_rsrc(p.scales, p.scales ? (unsigned)p.N * srow : 0u);
   const unsigned lds_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
 
   // Loads: the WN waves of K group wk fill the panels of its step.  A instruction i = wn + WN q covers
@@ -242,12 +207,7 @@ gemm_w_tile(Args p) {
 #pragma unroll
   for (int q = 0; q < T::kLoadsA; ++q) {
     const int row = 4 * (wn + WN * q) + (lane >> 4);
-    unsigned at = (unsigned)(m0 + row) * p.lda_bytes;
-    if constexpr (Args::kGrouped) {  // past the entry's rows: past A, which the host keeps below 2 GiB
-      at = 0xC0000000u;
-      if (row < m_end - m0) at = (unsigned)(p.rows ? p.rows[m0 + row] : row) * p.lda_bytes;
-    }
-    voa[q] = at + (unsigned)(((lane & 15) ^ (row & 15)) * 16 + wk * kWtK * 2);
+    voa[q] = (unsigned)(m0 + row) * p.lda_bytes + (unsigned)(((lane & 15) ^ (row & 15)) * 16 + wk * kWtK * 2);
   }
 #pragma unroll
   for (int q = 0; q < T::kLoadsW; ++q) {
@@ -305,11 +265,10 @@ gemm_w_tile(Args p) {
   for (int t = 0; t < FA; ++t) {
     acc[t] = f32x16{};
   }
-  auto read_a = [&](auto blocks, int buf, int j, u32x4 (&dst)[FA]) __attribute__((always_inline)) {
-    constexpr int NF = decltype(blocks)::value;
+  auto read_a = [&](int buf, int j, u32x4 (&dst)[FA]) __attribute__((always_inline)) {
     const int col = (I4 ? 2 * j + half : 8 * half + j) ^ (l32 & 15);
 #pragma unroll
-    for (int t = 0; t < NF; ++t)
+    for (int t = 0; t < FA; ++t)
       dst[t] = *(const u32x4*)(lds + buf * T::kStage + wk * T::kStep + (32 * t + l32) * 256 + col * 16);
   };
   auto read_w = [&](int buf, unsigned (&r)[RAW], unsigned (&sb)[T::kNS ? T::kNS : 1]) __attribute__((always_inline)) {
@@ -347,10 +306,8 @@ gemm_w_tile(Args p) {
   // and substep 0's weights are decoded.  Substep j reads A of j + 2 and decodes ahead; before substep 6,
   // when every LDS read of the stage is done, the wave waits for its share of the next stage, the barrier
   // publishes it and frees this buffer, and substeps 6 and 7 cover the refill's issue, the next stage's
-  // first reads and its first decode.  Of the tile's blocks of 32 rows the first `blocks` are multiplied: the
-  // rows of an expert rarely fill its last tile.
-  auto stage = [&](auto blocks, int st, int prv, int cur, int nxt) __attribute__((always_inline)) {
-    constexpr int NF = decltype(blocks)::value;
+  // first reads and its first decode.
+  auto stage = [&](int st, int prv, int cur, int nxt) __attribute__((always_inline)) {
     f32x16 part[FA];  // the sums of the current scale group
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -359,12 +316,12 @@ gemm_w_tile(Args p) {
         wait_loads<(NBUF - 2) * T::kLoads>();
         lds_barrier();
         read_w(nxt, rawn, sbitsn);
-        read_a(blocks, nxt, 0, fa[0]);
+        read_a(nxt, 0, fa[0]);
 
       } else if (j > 8 - PD) {
-        read_a(blocks, nxt, j + PD - 8, fa[j + PD - 8]);
+        read_a(nxt, j + PD - 8, fa[j + PD - 8]);
       } else {
-        read_a(blocks, cur, j + PD, fa[(j + PD) % SL]);
+        read_a(cur, j + PD, fa[(j + PD) % SL]);
       }
       // this substep's share of the loads, one after each MFMA: stage st + NBUF into this buffer from substep
       // 8 - PD on, the rest of stage st + NBUF - 1 into the previous stage's buffer before
@@ -382,11 +339,9 @@ gemm_w_tile(Args p) {
         if (j < 7) wi[(j + 1) & 1] = decode_nibbles(raw[j + 1], nib);
 #pragma unroll
         for (int t = 0; t < FA; ++t) {
-          if (t < NF) {
-            const wt_f16x8 a = __builtin_bit_cast(wt_f16x8, fa[j % SL][t]);
-            if constexpr (G == 0) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wi[j & 1], acc[t], 0, 0, 0);
-            else part[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wi[j & 1], j % JPG ? part[t] : f32x16{}, 0, 0, 0);
-          }
+          const wt_f16x8 a = __builtin_bit_cast(wt_f16x8, fa[j % SL][t]);
+          if constexpr (G == 0) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wi[j & 1], acc[t], 0, 0, 0);
+          else part[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, wi[j & 1], j % JPG ? part[t] : f32x16{}, 0, 0, 0);
           pieces(t);
         }
         if (j == 7) wi[0] = decode_nibbles(rawn[0], nib);
@@ -395,20 +350,19 @@ gemm_w_tile(Args p) {
           const float sv = ssize == 2 && p.sdt == TGM_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)bits)
                                                           : __builtin_bit_cast(float, bits << sshift);
 #pragma unroll
-          for (int t = 0; t < NF; ++t)
+          for (int t = 0; t < FA; ++t)
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[t][v] += part[t][v] * sv;
           // pins these sums here: left to itself the compiler collects every group's at the stage's end,
           // and with them every group's 16 FA partial sums (G = 32: 512 registers)
 #pragma unroll
-          for (int t = 0; t < NF; ++t) asm volatile("" : "+v"(acc[t]));
+          for (int t = 0; t < FA; ++t) asm volatile("" : "+v"(acc[t]));
         }
       } else {
         if (j == 2) mx_block(raw, sbits[0], 1);
 #pragma unroll
         for (int t = 0; t < FA; ++t) {
-          if (t < NF)
-            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(wt_bf16x8, fa[j % SL][t]), wd[j], acc[t], 0, 0, 0);
+          acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(wt_bf16x8, fa[j % SL][t]), wd[j], acc[t], 0, 0, 0);
           pieces(t);
         }
         if (j == 7) mx_block(rawn, sbitsn[0], 0);
@@ -430,40 +384,17 @@ gemm_w_tile(Args p) {
   wait_loads<(NBUF - 2) * T::kLoads + T::first_piece(0)>();
   lds_barrier();
   read_w(0, raw, sbits);
-  int used = FA;
-  if constexpr (!Args::kGrouped) {
-    constexpr std::integral_constant<int, FA> all{};
 #pragma unroll
-    for (int j = 0; j < PD; ++j) read_a(all, 0, j, fa[j]);
-    if constexpr (I4) wi[0] = decode_nibbles(raw[0], nib);
-    else mx_block(raw, sbits[0], 0);
-    int prv = NBUF - 1, cur = 0;
+  for (int j = 0; j < PD; ++j) read_a(0, j, fa[j]);
+  if constexpr (I4) wi[0] = decode_nibbles(raw[0], nib);
+  else mx_block(raw, sbits[0], 0);
+  int prv = NBUF - 1, cur = 0;
 #pragma unroll 1
-    for (int st = 0; st < nstages; ++st) {
-      const int nxt = cur + 1 < NBUF ? cur + 1 : 0;
-      stage(all, st, prv, cur, nxt);
-      prv = cur;
-      cur = nxt;
-    }
-  } else {
-    auto stages = [&](auto blocks) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < PD; ++j) read_a(blocks, 0, j, fa[j]);
-      if constexpr (I4) wi[0] = decode_nibbles(raw[0], nib);
-      else mx_block(raw, sbits[0], 0);
-      int prv = NBUF - 1, cur = 0;
-#pragma unroll 1
-      for (int st = 0; st < nstages; ++st) {
-        const int nxt = cur + 1 < NBUF ? cur + 1 : 0;
-        stage(blocks, st, prv, cur, nxt);
-        prv = cur;
-        cur = nxt;
-      }
-    };
-    used = (m_end - m0 + 31) / 32;
-    if (FA > 1 && used == 1) stages(std::integral_constant<int, 1>{});
-    else if (FA > 2 && used == 2) stages(std::integral_constant<int, FA < 2 ? FA : 2>{});
-    else stages(std::integral_constant<int, FA>{});
+  for (int st = 0; st < nstages; ++st) {
+    const int nxt = cur + 1 < NBUF ? cur + 1 : 0;
+    stage(st, prv, cur, nxt);
+    prv = cur;
+    cur = nxt;
   }
   wait_loads<0>();
   __syncthreads();  // the epilogue reuses the LDS
@@ -488,13 +419,12 @@ gemm_w_tile(Args p) {
   float* ep = parts + (WK - 1) * WN * FA * 1024 + wn * 32 * 36;
 #pragma unroll
   for (int t = 0; t < FA; ++t) {
-    if (Args::kGrouped && t >= used) break;
-    if (!Args::kGrouped && WK == 1 && p.part)
+    if (WK == 1 && p.part)
       store_tile32(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, p.M, p.N, p.part + (int64_t)blockIdx.y * p.M * p.N, TGM_F32,
                    p.N);
-    else if ((!I4 || Args::kGrouped) && p.swiglu)
-      store_tile32_swiglu(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, m_end, p.N, p.c, p.cdt, p.ldc);
-    else store_tile32(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, m_end, p.N, p.c, p.cdt, p.ldc);
+    else if (!I4 && p.swiglu)
+      store_tile32_swiglu(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, p.M, p.N, p.c, p.cdt, p.ldc);
+    else store_tile32(acc[t], ep, lane, m0 + 32 * t, n0 + 32 * wn, p.M, p.N, p.c, p.cdt, p.ldc);
   }
 }
 
