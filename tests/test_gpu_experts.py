@@ -316,3 +316,48 @@ def test_gates_of_every_size(dev, tokens):
     gates = np64(x) @ layer.gate_up[0][::2].T
     assert gates.max() > 90 and gates.min() < -90
     layer.check(layer.e.apply(x, ids, weights, out=torch.empty((tokens, 256), device=dev)), x, ids, weights)
+
+
+@pytest.mark.parametrize("fmt,scales,block", [("fp4_e2m1", "e8m0", 32), ("fp6_e3m2", "e8m0", 32), ("int4", F16, 64)])
+def test_experts_at_the_border_of_few_tokens(dev, fmt, scales, block):
+    """Calls of 1 to 17 tokens and up to 129 pairs, more than four tokens an expert among them."""
+    layer = Layer(dev, fmt, 40, 256, 128, scales, block)
+    for tokens, top_k in ((16, 8), (16, 9), (15, 8), (17, 7), (17, 1), (1, 40), (4, 32), (4, 33), (3, 40), (14, 9), (16, 2)):
+        ids, weights = choice(dev, tokens, tokens, 40, top_k, skew=3.0)
+        x = randn(dev, top_k, tokens, 256, dtype=layer.e.dtype, scale=0.5)
+        layer.check(layer.e.apply(x, ids, weights), x, ids, weights)
+    for tokens in (5, 16):  # all of them at the same experts
+        ids = torch.tensor([[39, 2, 17]], dtype=torch.int32, device=dev).repeat(tokens, 1)
+        weights = randn(dev, 3, tokens, 3)
+        x = randn(dev, 4, tokens, 256, dtype=layer.e.dtype, scale=0.5)
+        layer.check(layer.e.apply(x, ids, weights), x, ids, weights)
+
+
+@pytest.mark.parametrize("tokens", [2, 40])
+def test_experts_past_four_gib(dev, tokens):
+    """The first and the last of experts whose codes pass 2^32 bytes give what they give alone."""
+    experts, hidden, ffn = 80, 4096, 14336
+    gen = torch.Generator(dev).manual_seed(1)
+
+    def weight(rows, k):
+        codes = torch.randint(0, 256, (experts * rows * k // 2,), dtype=torch.uint8, device=dev, generator=gen)
+        sc = torch.randint(112, 120, (experts, rows, k // 32), dtype=torch.uint8, device=dev, generator=gen).view(torch.float8_e8m0fnu)
+        return codes, sc
+
+    def pack(w, shape):
+        return PackedTensor(w[0], "fp4_e2m1", shape, w[1], 32)
+
+    def ends(w, rows, k):
+        n = rows * k // 2
+        return torch.cat((w[0][:n], w[0][-n:])), torch.cat((w[1][:1].view(torch.uint8), w[1][-1:].view(torch.uint8))).view(w[1].dtype)
+
+    up, down = weight(2 * ffn, hidden), weight(hidden, ffn)
+    assert up[0].numel() > 2 ** 32
+    every = PackedExperts(pack(up, (experts, 2 * ffn, hidden)), pack(down, (experts, hidden, ffn)))
+    two = PackedExperts(pack(ends(up, 2 * ffn, hidden), (2, 2 * ffn, hidden)), pack(ends(down, hidden, ffn), (2, hidden, ffn)))
+    ids = torch.randint(0, 2, (tokens, 2), dtype=torch.int32, device=dev, generator=gen)
+    weights, x = randn(dev, 1, tokens, 2), randn(dev, 2, tokens, hidden, dtype=BF16)
+    got, want = every.apply(x, ids * (experts - 1), weights), two.apply(x, ids, weights)
+    # sums in another order: 14336 products, of a hidden value that may have rounded the other way (2^-8); what reads
+    # another expert is off by the size of the rows
+    assert (got.double() - want.double()).norm() <= 2.0 ** -6 * want.double().norm() and torch.isfinite(want).all()

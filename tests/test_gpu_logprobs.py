@@ -6,6 +6,8 @@ add 64 roundings.  exp(d) (1 + |d|) is at most 1, so of a sum both errors are at
 the results' own roundings are half a step of d and of the logarithm.
 """
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -154,3 +156,20 @@ def test_ranks_of_tokens_that_are_ruled_out(dev, dtype):
             x[0, ::3] = -float("inf")
             for token in (0, 3, 9, 36, vocab - 1 - (vocab - 1) % 3):
                 check(x, torch.tensor([token], dtype=torch.int32, device=dev), 5)
+
+
+def test_log_probs_past_four_gib(dev):
+    """Rows on both sides of 2^32 bytes are what they are alone."""
+    rows, vocab = 70000, 32000
+    logits = torch.zeros((rows, vocab), dtype=torch.bfloat16, device=dev)
+    some = torch.tensor([0, 33553, 33554, 67107, 67108, 67109, rows - 1], device=dev)
+    logits[some] = torch.randn((7, vocab), device=dev, generator=torch.Generator(dev).manual_seed(0)).to(torch.bfloat16) * 3
+    tokens = torch.arange(rows, dtype=torch.int32, device=dev) % vocab
+    got = log_probs(logits, tokens, top=5)
+    alone = log_probs(logits[some].contiguous(), tokens[some].contiguous(), top=5)
+    assert torch.equal(got.ranks[some], alone.ranks) and torch.equal(got.top_ids[some], alone.top_ids)
+    for a, b in ((got.logprobs, alone.logprobs), (got.entropy, alone.entropy), (got.top_logprobs, alone.top_logprobs)):
+        assert torch.allclose(a[some], b, rtol=1e-5, atol=1e-5)  # two orders of 32000 terms summed in 32 bits
+    flat = torch.full_like(got.logprobs, -math.log(vocab))
+    flat[some] = got.logprobs[some]
+    assert torch.allclose(got.logprobs, flat, rtol=1e-5, atol=0)

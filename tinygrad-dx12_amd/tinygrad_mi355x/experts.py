@@ -145,6 +145,7 @@ class PackedExperts:
         ``out`` [tokens, hidden] is of x's type or float32 (x's type), with contiguous rows; it may be x.  An id outside
         0 .. experts - 1 names no expert and adds nothing, whatever its weight: a row without any is zero.  The same expert
         may be named twice.  Products and sums are float32; silu(gate) * up is rounded to x's type before the down product.
+        x starts at a multiple of 16 bytes, and its rows lie a multiple of 8 values apart.
         """
         sig = (x.shape, x.stride(), x.dtype, x.get_device(), ids.shape, ids.stride(), ids.dtype, ids.get_device(), weights.shape,
                weights.stride(), weights.dtype, weights.get_device())
