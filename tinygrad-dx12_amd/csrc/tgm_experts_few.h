@@ -6,7 +6,8 @@
 // weight rows in neighbouring lanes; loaded so, straight into it, codes and scales of 2 experts of 4096 x 14336 took 132
 // accesses a KB, and the gate|up product of one token 43 us.  So a wave loads 16 rows x 512 columns in whole lines, and the
 // activations of the tokens beside them, two such groups ahead, and turns them in a block of LDS of its own, 12 waves a
-// compute unit: a bare read in this order takes 21 us for the 117 MB of codes, in 64-byte pieces 26.
+// compute unit: 28 us, and 15 for the down product; a bare read in this order takes 21 us for the 117 MB of codes, in 64-byte
+// pieces 26.
 //
 // No sorting of tokens comes first: every workgroup makes the list from the ids by itself (pairs of a token and an expert:
 // 128 at most).  An entry of it is an expert and up to four of the tokens that name it; more make a second entry, and the

@@ -301,11 +301,9 @@ gemm_w_group(WGroupArgs p) {
   rows_of(next, voan);
   aim(next, voan);
   first_loads();
-  // A workgroup's place moves on by 3 of its XCD each round of the grid: the tiles of one place are often of one height.
   int prv = NBUF - 1, cur = 0;
-  for (int round = 1;; ++round) {
+  for (int tile = blockIdx.x + gridDim.x;; tile += gridDim.x) {
     const WGroupAt own = at;
-    const int tile = round * (int)gridDim.x + (int)((blockIdx.x + 24u * (unsigned)round) % gridDim.x);
     const bool more = tile < total, ahead = more && nstages >= NBUF;
     if (more) {
       next = find(tile);

