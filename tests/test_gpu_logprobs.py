@@ -173,3 +173,19 @@ def test_log_probs_past_four_gib(dev):
     flat = torch.full_like(got.logprobs, -math.log(vocab))
     flat[some] = got.logprobs[some]
     assert torch.allclose(got.logprobs, flat, rtol=1e-5, atol=0)
+
+
+@pytest.mark.parametrize("vocab", [32769, 65537, 70001, 131072, 400000, 1 << 20])
+@pytest.mark.parametrize("top", [1, 7, 64])
+def test_lists_of_stretches(dev, vocab, top):
+    """Rows in several stretches whose likeliest tokens lie in one of them, are all alike, are few, or are masked but for a few."""
+    print(f"stretches {vocab} {top}", flush=True)
+    x = torch.randn((6, vocab), device=dev, generator=torch.Generator(dev).manual_seed(vocab + top))
+    x[1, vocab // 2:vocab // 2 + 100] += 20
+    x[2] = 1.25
+    x[3] = float("-inf")
+    x[3, [5, vocab - 1]] = 2.0
+    x[4, :vocab - 40] = float("-inf")
+    x[5] = torch.arange(vocab, device=dev) / vocab  # rising: all of them in the last stretch
+    tokens = torch.tensor([0, vocab // 2, vocab - 1, 5, vocab - 2, 17], dtype=torch.int32, device=dev)
+    check(x, tokens, top)

@@ -12,10 +12,11 @@
 // one after another instead.
 //
 // A row that is longer than a stretch, or that would leave compute units idle, takes several, and a second launch joins
-// them: S and T scale by exp(m_stretch - m), and each listed token counts those of the other lists before it.
+// them: S and T scale by exp(m_stretch - m), and the lists' entries that reach a bound count those before them.
 //
-// What bounds it: HBM with many rows (4000 x 32000 bf16, top 5: 57 us, 4.5 TB/s, where 32 logits a thread take 72), the chain
-// of reductions and barriers with few (8 x 32000, top 20: 13 us; 131072 in stretches 11, and the join 4).
+// What bounds it: HBM with many rows (4000 x 32000 bf16, top 5: 56 us, 4.6 TB/s, where 32 logits a thread take 72), the chain
+// of reductions and barriers with few (8 x 32000, top 20: 10.2 us; 131072, top 5: 6.3 in nine stretches, and the join 3; in
+// four of 1024 threads 7, in 17 of 256 7.8 and 3.9).
 #include <math.h>
 
 #include "../../include/tgm_serving.h"
@@ -24,7 +25,7 @@
 
 namespace tgm {
 
-constexpr int kLpMost = 1024, kLpTop = 64, kLpList = 512, kLpJoin = 256;
+constexpr int kLpMost = 1024, kLpTop = 64, kLpList = 512, kLpJoin = 256, kLpStretches = 64;
 typedef unsigned long long lp_u64;
 typedef unsigned lp_u32x4 __attribute__((ext_vector_type(4)));
 
@@ -223,18 +224,17 @@ __global__ void __launch_bounds__(32 * kLpMost / EACH) __attribute__((amdgpu_wav
   dot = (dot - low * sum) * 0.69314718055994530942f;
   const float by = __builtin_amdgcn_exp2f(-low);
   if (lane == 0) wave_sum[wave] = sum * by, wave_dot[wave] = dot * by, wave_rank[wave] = (float)rank;  // at most 2^20
-  // list what reaches the bound
-  if (a.top && __any(top >= bound)) {
-    lp_u64 reaches = 0;
+  // list what reaches the bound; of -infinities alone, which all do, nothing
+  if (a.top && max > -INFINITY && __any(top >= bound)) {
 #pragma unroll
-    for (int r = 0; r < EACH; ++r) reaches |= value(r) >= bound ? 1ull << r : 0ull;
-    while (reaches) {
-      const int r = __builtin_ctzll(reaches);
-      reaches &= reaches - 1;
-      const int i = (v0 + r / VEC * (int)blockDim.x) * VEC - shift + r % VEC;
-      if ((unsigned)i >= (unsigned)a.n) continue;
-      const int o = atomicAdd(&listed, 1);
-      if (o < kLpList) list[o] = lp_entry(lp_key(lp_load<DT>(base, i)), i);
+    for (int r = 0; r < EACH; ++r) {
+      const float x = value(r);
+      if (x >= bound) {
+        const int i = (v0 + r / VEC * (int)blockDim.x) * VEC - shift + r % VEC;
+        const int o = (unsigned)i < (unsigned)a.n ? atomicAdd(&listed, 1) : kLpList;
+        if (o < kLpList) list[o] = lp_entry(lp_key(x), i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   __syncthreads();
@@ -242,11 +242,10 @@ __global__ void __launch_bounds__(32 * kLpMost / EACH) __attribute__((amdgpu_wav
   const int begin = stretch * (int)blockDim.x * EACH - shift, end = begin + (int)blockDim.x * EACH;
   const int held = (end < a.n ? end : a.n) - (begin > 0 ? begin : 0);  // elements of the stretch; fewer than top end its list
   const bool in_turn = c > kLpList || c < (held < a.top ? held : a.top);
-  if (wave > 0 && !in_turn) return;
   sum = lp_row_sum(w16 < waves ? wave_sum[w16] : 0.0f);
   dot = lp_row_sum(w16 < waves ? wave_dot[w16] : 0.0f);
   rank = (int)lp_row_sum(w16 < waves ? wave_rank[w16] : 0.0f);
-  if (stretch == 0 && named) {
+  if (stretch == 0 && named && wave == 0) {
     const int before = (tok + shift) % VEC, i = tok - before + lane;  // in the token's vector
     rank += __builtin_popcountll(__ballot(lane < before && i >= 0 && lp_load<DT>(base, i < 0 ? 0 : i) == at));
     if (at == -INFINITY && VEC - shift <= tok) rank -= shift;  // what the first vector holds before the row
@@ -266,15 +265,19 @@ __global__ void __launch_bounds__(32 * kLpMost / EACH) __attribute__((amdgpu_wav
       a.lists[(int64_t)blockIdx.x * a.top + at_place] = entry;
     }
   };
-  if (!in_turn) {
-    for (int i = lane; i < c; i += 64) {
+  if (!in_turn) {  // eight lanes an entry
+    for (int i = threadIdx.x >> 3; i < c; i += blockDim.x >> 3) {
       const lp_u64 mine = list[i];
       int before = 0;
 #pragma unroll 8
-      for (int o = 0; o < c; ++o) before += list[o] > mine;
-      if (before < a.top) place(before, mine);
+      for (int o = lane & 7; o < c; o += 8) before += list[o] > mine;
+      float all = (float)before;
+      all += xor1(all);
+      all += xor2(all);
+      all += xor4(all);
+      if ((lane & 7) == 0 && (int)all < a.top) place((int)all, mine);
     }
-    for (int i = c + lane; i < a.top; i += 64) place(i, 0);
+    for (int i = c + (int)threadIdx.x; i < a.top; i += blockDim.x) place(i, 0);
     return;
   }
   // one after another, read again: the largest entry below the last one; 0 where the stretch has no more elements
@@ -305,8 +308,14 @@ template <int DT>
 __global__ void __launch_bounds__(kLpJoin) logprob_join(LpArgs a) {
   const int64_t row = blockIdx.x;
   const LpPart* parts = a.parts + row * a.stretches;
-  const lp_u64* lists = a.lists + row * a.stretches * a.top;
-  const int lane = threadIdx.x & 63;  // a stretch each: at most 33
+  const lp_u64* from = a.lists + row * a.stretches * a.top;
+  __shared__ lp_u64 lists[kLpStretches * kLpTop], near[kLpList], bound;
+  __shared__ int nears, full;
+  const int listed = a.stretches * a.top;
+  for (int i = threadIdx.x; i < listed; i += kLpJoin) lists[i] = from[i];
+  const bool deep = a.top >= a.stretches;
+  if (threadIdx.x == 0) nears = full = 0, bound = deep ? ~0ull : 1;
+  const int lane = threadIdx.x & 63;  // a stretch each
   LpPart p{-INFINITY, 0.0f, 0.0f, 0};
   if (lane < a.stretches) p = parts[lane];
   const float max = lp_wave_max(p.max);
@@ -321,9 +330,51 @@ __global__ void __launch_bounds__(kLpJoin) logprob_join(LpArgs a) {
     lp_write(a, row, max, sum, dot, rank, at, named);
   }
   const float log_sum = logf(sum);
-  for (int i = threadIdx.x; i < a.stretches * a.top; i += kLpJoin) {
+  auto place = [&](int before, lp_u64 mine) __attribute__((always_inline)) {
+    a.top_ids[row * a.top + before] = (int)~(unsigned)mine;
+    a.top_logprobs[row * a.top + before] = (lp_unkey((unsigned)(mine >> 32)) - max) - log_sum;
+  };
+  // A bound that `top` entries reach, or 1 (0 is no entry): the top-th largest of the lists' first entries, or the least of
+  // the q-th entries of those that have so many, as all but the last list do where nothing is masked.
+  __syncthreads();
+  const int q = deep ? (a.top + a.stretches - 2) / (a.stretches - 1) : 1;
+  if ((int)threadIdx.x < a.stretches && a.top) {
+    const lp_u64 mine = lists[threadIdx.x * a.top + q - 1];
+    if (deep) {
+      if (mine) atomicMin(&bound, mine), atomicAdd(&full, 1);
+    } else {
+      int before = 0;
+#pragma unroll 4
+      for (int s = 0; s < a.stretches; ++s) before += lists[s * a.top] > mine;
+      if (mine && before == a.top - 1) bound = mine;
+    }
+  }
+  __syncthreads();
+  const lp_u64 least = deep && full * q < a.top ? 1 : bound;
+  for (int i = threadIdx.x; i < listed; i += kLpJoin)
+    if (lists[i] >= least) {
+      const int o = atomicAdd(&nears, 1);
+      if (o < kLpList) near[o] = lists[i];
+    }
+  __syncthreads();
+  const int c = nears;
+  if (c <= kLpList) {  // eight lanes an entry, as above
+    for (int i = threadIdx.x >> 3; i < c; i += kLpJoin >> 3) {
+      const lp_u64 mine = near[i];
+      int before = 0;
+#pragma unroll 8
+      for (int o = lane & 7; o < c; o += 8) before += near[o] > mine;
+      float all = (float)before;
+      all += xor1(all);
+      all += xor2(all);
+      all += xor4(all);
+      if ((lane & 7) == 0 && (int)all < a.top) place((int)all, mine);
+    }
+    return;
+  }
+  for (int i = threadIdx.x; i < listed; i += kLpJoin) {
     const lp_u64 mine = lists[i];
-    if (mine == 0) continue;  // its stretch had fewer
+    if (mine < least) continue;
     const int own = i / a.top;
     int before = i - own * a.top;
     for (int s = 0; s < a.stretches && before < a.top; ++s) {
@@ -336,9 +387,7 @@ __global__ void __launch_bounds__(kLpJoin) logprob_join(LpArgs a) {
       }
       before += low;
     }
-    if (before >= a.top) continue;
-    a.top_ids[row * a.top + before] = (int)~(unsigned)mine;
-    a.top_logprobs[row * a.top + before] = (lp_unkey((unsigned)(mine >> 32)) - max) - log_sum;
+    if (before < a.top) place(before, mine);
   }
 }
 
@@ -346,7 +395,7 @@ struct LpSizes {
   int each, threads, stretches;
   int64_t lists, bytes;
 };
-// Threads of a workgroup and stretches of a row.
+// Threads of a workgroup and stretches of a row: one where a row fits it, short ones where few rows do not.
 static LpSizes lp_sizes(int64_t rows, int64_t vocab, int64_t dtype, int64_t top) {
   const int vec = dtype == TGM_F32 ? 4 : 8;
   const int64_t vectors = (vocab + 2 * vec - 2) / vec;  // at most, by the alignment of the row
@@ -355,6 +404,12 @@ static LpSizes lp_sizes(int64_t rows, int64_t vocab, int64_t dtype, int64_t top)
   const int64_t need = (vectors + z.each / vec - 1) / (z.each / vec);  // threads for one stretch
   const int most = 32 * kLpMost / z.each;
   z.threads = need >= most ? most : (int)((need + 63) / 64 * 64);
+  if (need > most) {
+    for (z.threads = 512; z.threads < most; z.threads *= 2) {
+      const int64_t stretches = (need + z.threads - 1) / z.threads;
+      if (stretches <= kLpStretches && rows * stretches * z.threads <= 256 * 1024) break;
+    }
+  }
   z.stretches = (int)((need + z.threads - 1) / z.threads);
   z.lists = (rows * z.stretches * (int64_t)sizeof(LpPart) + 255) / 256 * 256;
   z.bytes = z.stretches == 1 ? 0 : z.lists + rows * z.stretches * top * 8;

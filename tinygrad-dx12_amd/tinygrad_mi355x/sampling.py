@@ -129,15 +129,14 @@ def log_probs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> Lo
     if plan is None:
         plan = _log_probs_plan(sig, logits, tokens, top)
     head, rows, need, index = plan
-    numbers = logits.new_empty((2, rows), dtype=torch.float32)
-    ranks = logits.new_empty(rows, dtype=torch.int32)
-    top_ids, top_logprobs = logits.new_empty((rows, top), dtype=torch.int32), logits.new_empty((rows, top), dtype=torch.float32)
+    f32, i32 = torch.float32, torch.int32
+    got = LogProbs(logits.new_empty(rows, dtype=f32), logits.new_empty(rows, dtype=i32), logits.new_empty(rows, dtype=f32),
+                   logits.new_empty((rows, top), dtype=i32), logits.new_empty((rows, top), dtype=f32))
     # of the caching allocator and held until the launch, as in sample
     workspace = logits.new_empty(need, dtype=torch.uint8) if need else None
-    got = LogProbs(numbers[0], ranks, numbers[1], top_ids, top_logprobs)
     if rows:
-        K.call("tgm_log_probs", logits.data_ptr(), *head, tokens.data_ptr(), top, got.logprobs.data_ptr(), ranks.data_ptr(),
-               got.entropy.data_ptr(), top_ids.data_ptr(), top_logprobs.data_ptr(), K.ptr(workspace), need, K.stream_on(index))
+        K.call("tgm_log_probs", logits.data_ptr(), *head, tokens.data_ptr(), top, *[t.data_ptr() for t in got], K.ptr(workspace),
+               need, K.stream_on(index))
     return got
 
 
