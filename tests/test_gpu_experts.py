@@ -361,3 +361,15 @@ def test_experts_past_four_gib(dev, tokens):
     # sums in another order: 14336 products, of a hidden value that may have rounded the other way (2^-8); what reads
     # another expert is off by the size of the rows
     assert (got.double() - want.double()).norm() <= 2.0 ** -6 * want.double().norm() and torch.isfinite(want).all()
+
+
+@pytest.mark.parametrize("tokens,top_k", [(4096, 4), (4097, 4), (2500, 13)])
+def test_more_pairs_than_registers_hold(dev, tokens, top_k):
+    """16384 pairs and more, some of them of no expert: a row is what it is in a call of few tokens."""
+    layer = Layer(dev, "fp4_e2m1", 16, 128, 128)
+    ids, weights = choice(dev, tokens, tokens, 16, top_k)
+    ids[torch.rand(ids.shape, generator=torch.Generator().manual_seed(1)).to(dev) < 0.1] = -1
+    x = randn(dev, 1, tokens, 128, dtype=BF16, scale=0.5)
+    got = layer.e.apply(x, ids, weights)
+    layer.check(got, x, ids, weights)
+    assert torch.equal(layer.e.apply(x, ids, weights), got)
