@@ -9,7 +9,7 @@ static int launch_kind(const WGroupArgs& p, int shape, bool wide, int64_t most, 
   if (shape == 0)
     return wide ? launch_experts_tile<KIND, 1, 8, FINE ? 2 : 3>(p, most, st) : launch_experts_tile<KIND, 1, 4, FINE ? 3 : 4>(p, most, st);
   if (shape == 1) return wide ? launch_experts_tile<KIND, 2, 8, 3>(p, most, st) : launch_experts_tile<KIND, 2, 4, 3>(p, most, st);
-  return wide ? launch_experts_tile<KIND, 4, 8, 2>(p, most, st) : launch_experts_tile<KIND, 4, 4, 2>(p, most, st);
+  return wide ? launch_experts_tile<KIND, 4, 8, FINE ? 2 : 3>(p, most, st) : launch_experts_tile<KIND, 4, 4, 2>(p, most, st);
 }
 
 int launch_experts_tile_i4(const WGroupArgs& p, int64_t group, int shape, bool wide, int64_t most, hipStream_t st) {
