@@ -11,7 +11,8 @@
 // bits, one a lane, and put in order; where it does not end in time, or groups on either side of their border are that
 // near, the wave does the choice again in 64 bits.
 //
-// What bounds it: instructions.  8192 tokens of 256 experts in 8 groups read 8.4 MB, 2 us of memory time, and take 15.6: a
+// What bounds it: instructions.  8192 tokens of 256 experts in 8 groups read 8.4 MB, 2 us of memory time, and take 12.6 (15.2
+// with expf and a division in the keys, whose errors the list allows for): a
 // sigmoid an expert, the two largest of each group, eight rounds of a maximum over 16 lanes.  With 32 or 64 lanes a token
 // the rounds are longer and the time the same.
 #include <math.h>
@@ -293,16 +294,22 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
   if (biased || limited) {
     float c[R];
     sum = 0.0f;
+    if (soft) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      c[r] = score(x[r]);
-      sum += c[r];
+      for (int r = 0; r < R; ++r) {
+        c[r] = score(x[r]);
+        sum += c[r];
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) c[r] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[r] * -1.44269504f));
     }
     sum = soft ? lanes_sum<W>(sum) : 1.0f;
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    // Errors of two scores.  Sigmoid: exp, sum and quotient are off by 2^-23, 2^-24 and 2^-24 of at most 1.  Softmax: of the
+    // Errors of two scores.  Sigmoid, 1 / (1 + 2^t): t is off by 1.5 half steps, which changes p by p (1 - p) |x| 1.5 2^-24, at
+    // most 0.34 2^-24; the power, the sum and the quotient by 2^-25, 2^-24 and 2^-23: together less than 2.4e-7.  Softmax: of the
     // largest, inv, a difference of logits up to 104 (below, the score is 0), exp, R + 6 sums and two products, 2^-16.
-    const float tol = soft ? 3.1e-5f * inv + 1e-37f : 4.8e-7f;
+    const float tol = soft ? 3.1e-5f * inv + 1e-37f : 5e-7f;
     float b[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) b[r] = 0.0f;
@@ -324,7 +331,6 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
     for (int r = 0; r < R; ++r) {
       const int e = l * R + r;
       c[r] = c[r] * inv + b[r];
-      c[r] = x[r] != x[r] ? x[r] : c[r];
       key[r] = e < a.experts ? route_key(biased ? c[r] : x[r]) : 0u;
     }
     if (limited) again = route_groups<W, R>(a, l, c, key, (float*)sums[slot], 2 * tol);
