@@ -373,3 +373,30 @@ def test_more_pairs_than_registers_hold(dev, tokens, top_k):
     got = layer.e.apply(x, ids, weights)
     layer.check(got, x, ids, weights)
     assert torch.equal(layer.e.apply(x, ids, weights), got)
+
+
+def test_calls_of_several_threads(dev):
+    """Threads on one stream and on their own, of one layer and with other sizes in between."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from tinygrad_mi355x.sampling import log_probs
+
+    layer = Layer(dev, "fp4_e2m1", 8, 256, 384)
+    work = []
+    for tokens in (1, 9, 40, 300):
+        ids, weights = choice(dev, tokens, tokens, 8, 2)
+        x = randn(dev, tokens, tokens, 256, dtype=BF16)
+        logits, drawn = randn(dev, tokens, tokens, 40000), torch.arange(tokens, dtype=torch.int32, device=dev)
+        work.append(lambda a=(x, ids, weights), b=(logits, drawn): (layer.e.apply(*a), *log_probs(*b, top=6), *route(b[0][:, :96], 8)))
+    want = [w() for w in work]
+    torch.cuda.synchronize()
+
+    def one(i):
+        stream = torch.cuda.Stream() if i % 2 else torch.cuda.current_stream()
+        with torch.cuda.stream(stream):
+            got = [work[(i + j) % 4]() for j in range(12)]
+        stream.synchronize()
+        return all(torch.equal(a, b) for j, g in enumerate(got) for a, b in zip(g, want[(i + j) % 4]))
+
+    with ThreadPoolExecutor(6) as pool:
+        assert all(pool.map(one, range(12)))
