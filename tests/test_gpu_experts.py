@@ -376,7 +376,7 @@ def test_more_pairs_than_registers_hold(dev, tokens, top_k):
 
 
 def test_calls_of_several_threads(dev):
-    """Threads on one stream and on their own, of one layer and with other sizes in between."""
+    """Threads that share two streams, of one layer and with other sizes in between."""
     from concurrent.futures import ThreadPoolExecutor
 
     from tinygrad_mi355x.sampling import log_probs
@@ -391,8 +391,10 @@ def test_calls_of_several_threads(dev):
     want = [w() for w in work]
     torch.cuda.synchronize()
 
+    streams = torch.cuda.current_stream(), torch.cuda.Stream()
+
     def one(i):
-        stream = torch.cuda.Stream() if i % 2 else torch.cuda.current_stream()
+        stream = streams[i % 2]
         with torch.cuda.stream(stream):
             got = [work[(i + j) % 4]() for j in range(12)]
         stream.synchronize()
