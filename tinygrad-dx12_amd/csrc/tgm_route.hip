@@ -283,10 +283,6 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
   const unsigned long long seen = __ballot(bad);
   bad = ((W == 64 ? seen : seen >> ((threadIdx.x & 63) / W * W) & ((1ull << (W & 63)) - 1))) != 0;
   const float zero = top == -INFINITY ? 0.0f : top;
-  auto score = [&](float v) __attribute__((always_inline)) {  // under a softmax still to be divided by their sum
-    return soft ? expf(v - zero) : 1.0f / (1.0f + expf(-v));
-  };
-
   unsigned key[R];
   float sum = 1.0f;
   bool near = false, again = false;
@@ -297,7 +293,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
     if (soft) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        c[r] = score(x[r]);
+        c[r] = expf(x[r] - zero);
         sum += c[r];
       }
     } else {
@@ -389,16 +385,31 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
   }
   wave_lds_fence();
 
-  // the weights, an entry a lane
-  float chosen = 0.0f;
-  for (int j = l; j < a.top_k; j += W) chosen += score(load_f32(a.logits, DT, base + list[j]));
+  // The weights, an entry a lane.  Their scores are e^x of a softmax, over its sum, or e^min(x, 0) / (1 + e^-|x|), all of them times
+  // e^-from: from the row's largest logit, and in renormalised ones from the largest chosen, which a bias may have picked far
+  // below it and which may be low itself, so that the chosen ones' sum is at least a half.
+  const int own = l < a.top_k ? list[l] : 0;
+  const float mine = load_f32(a.logits, DT, base + own);
+  auto logit = [&](int j) __attribute__((always_inline)) { return j < W ? mine : load_f32(a.logits, DT, base + list[j]); };
+  float from = soft ? zero : 0.0f;
+  if (a.renormalize) {
+    float most = -INFINITY;
+    for (int j = l; j < a.top_k; j += W) most = fmaxf(most, logit(j));
+    most = lanes_max<W>(most);
+    from = most == -INFINITY ? 0.0f : soft ? most : fminf(most, 0.0f);
+  }
+  auto score = [&](float v) __attribute__((always_inline)) {
+    return soft ? expf(v - from) : expf(fminf(v, 0.0f) - from) / (1.0f + expf(-fabsf(v)));
+  };
+  const float first = score(mine);
+  float chosen = l < a.top_k ? first : 0.0f;
+  for (int j = l + W; j < a.top_k; j += W) chosen += score(logit(j));
   chosen = a.renormalize ? lanes_sum<W>(chosen) : sum;
-  const float by = chosen > 0.0f ? a.scale / chosen : 0.0f;
   if (!live) return;
   for (int j = l; j < a.top_k; j += W) {
-    const int e = list[j];
-    a.ids[token * a.top_k + j] = e;
-    a.weights[token * a.top_k + j] = bad ? NAN : score(load_f32(a.logits, DT, base + e)) * by;
+    const float part = (j < W ? first : score(logit(j))) / chosen;
+    a.ids[token * a.top_k + j] = j < W ? own : list[j];
+    a.weights[token * a.top_k + j] = bad ? NAN : chosen > 0.0f ? part * a.scale : 0.0f;
   }
 }
 
