@@ -174,6 +174,10 @@ struct FewSource {
   using G = FewGroup<KIND>;
   __amdgpu_buffer_rsrc_t w, scales, act;
   unsigned w_off[G::kLoads], s_off, a_off[kFewRows];  // of the lane in group 0
+  // Bytes from a group's scales to the next, as the loads' scalar offset; 0 without scales, whose buffer is empty: a bounds check
+  // against the size less a scalar offset above it would wrap.  Codes' and activations' stays below their buffers' sizes, or
+  // passes them by 256 bytes and more, where the wrapped limit is still kFewNone or less.
+  int s_group;
 };
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t few_buffer(const uint8_t* base, unsigned bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
@@ -194,6 +198,7 @@ __device__ __forceinline__ void few_rows(FewSource<KIND>& from, const FewArgs& p
   }
   const int r = lane >> 2;  // step lane % 4 of row lane / 4
   from.s_off = r < rows ? (unsigned)(row + r) * (unsigned)(steps * G::kScale) + (unsigned)((lane & 3) * G::kScale) : kFewNone;
+  from.s_group = scaled ? 4 * G::kScale : 0;
 }
 
 // Group `group` of a weight's rows, which have `steps` steps, and of the tokens'; what lies past a row's end is zero.
@@ -208,7 +213,7 @@ __device__ __forceinline__ void few_load(FewGroup<KIND>& g, const FewSource<KIND
     g.codes[i] = __builtin_amdgcn_raw_buffer_load_b128(from.w, off, group * 4 * G::kStep, NT);
   }
   const unsigned s_off = (lane & 3) < left ? from.s_off : kFewNone;
-  const int s_at = group * 4 * G::kScale;
+  const int s_at = group * from.s_group;
   if constexpr (G::kScale == 2) {
     g.scale[0] = __builtin_amdgcn_raw_buffer_load_b16(from.scales, s_off, s_at, 0);
   } else if constexpr (G::kScale == 4) {
