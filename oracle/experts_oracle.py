@@ -78,5 +78,5 @@ def log_probs(logits, tokens, top):
             order = np.lexsort((np.arange(n), -np.where(x != x, -np.inf, x), x != x))
             got[3][r], got[4][r] = order[:top], logp[order[:top]]
             if 0 <= tokens[r] < n:
-                got[0][r], got[1][r] = logp[tokens[r]], (x > x[tokens[r]]).sum() + (x[:tokens[r]] == x[tokens[r]]).sum()
+                got[0][r], got[1][r] = logp[tokens[r]], np.nonzero(order == tokens[r])[0][0]  # NaN behind everything
     return got

@@ -15,7 +15,7 @@
 // them: S and T scale by exp(m_stretch - m), and the lists' entries that reach a bound count those before them.
 //
 // What bounds it: HBM with many rows (4000 x 32000 bf16, top 5: 56 us, 4.6 TB/s, where 32 logits a thread take 72), the chain
-// of reductions and barriers with few (8 x 32000, top 20: 10.2 us; 131072, top 5: 6.3 in nine stretches, and the join 3; in
+// of reductions and barriers with few (8 x 32000, top 20: 10.2 us; 131072, top 5: 6.4 in nine stretches, and the join 3; in
 // four of 1024 threads 7, in 17 of 256 7.8 and 3.9).
 #include <math.h>
 
@@ -191,10 +191,11 @@ __global__ void __launch_bounds__(32 * kLpMost / EACH) __attribute__((amdgpu_wav
   // unpacked anew: kept from one pass to the next, the values would not fit the registers
 #pragma unroll
   for (int q = 0; q < NV; ++q) asm volatile("" : "+v"(raw[q]));
-  // The rank counts equal logits before the token: vectors before its own compare with the next number below it (NaN below
-  // -infinity, where all of them count), its own vector's are counted at the end.
+  // The rank counts what is larger, and equal logits before the token: vectors before its own compare with it, later ones with the
+  // next number above it, and its own vector's equal ones are counted at the end.  A comparison with a NaN does not hold, so
+  // that NaN logits count for no number; a token that is NaN itself is counted apart.
   int rank = 0;
-  const float below = at == 0.0f ? -bits_f32(1u) : bits_f32(f32_bits(at) + (at > 0.0f ? -1 : 1));
+  const float above = at == 0.0f ? bits_f32(1u) : bits_f32(f32_bits(at) + (at > 0.0f ? 1 : -1));  // of +infinity a NaN: none is above
   // exp(x - m) = 2^(x L - m L), L = log2 e.  With m L in two parts, of which the second is left out of every term, one
   // fused step gives an exponent that is off by its own rounding alone; from 2^20 on the second part is not small, and the
   // difference comes first.
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(32 * kLpMost / EACH) __attribute__((amdgpu_wav
   auto pass = [&](auto exponent) __attribute__((always_inline)) {
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
-      const float over = (v0 + q * (int)blockDim.x + 1) * VEC - shift <= tok ? below : at;
+      const float least = (v0 + q * (int)blockDim.x + 1) * VEC - shift <= tok ? at : above;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float x = value(q * VEC + i);
@@ -212,13 +213,22 @@ __global__ void __launch_bounds__(32 * kLpMost / EACH) __attribute__((amdgpu_wav
         const float e = __builtin_amdgcn_exp2f(d);
         sum += e;
         dot = __builtin_fmaf(e, fmaxf(d, -1000.0f), dot);  // nothing times infinity adds nothing
-        rank += __builtin_popcountll(__ballot(!(x <= over)));
+        rank += __builtin_popcountll(__ballot(x >= least));
       }
       __builtin_amdgcn_sched_barrier(0);  // ahead of its vector's turn, an unpacked value takes a register
     }
   };
   if (fabsf(zero) < 0x1p20f) pass([&](float x) __attribute__((always_inline)) { return __builtin_fmaf(x, L, -zero_l); });
   else pass([&](float x) __attribute__((always_inline)) { return (x - zero) * L; });
+  const int begin = stretch * (int)blockDim.x * EACH - shift, end = begin + (int)blockDim.x * EACH;
+  if (named && at != at) {  // behind every number and the NaNs before it
+    rank = 0;
+    for (int i = begin + (int)threadIdx.x; i < end; i += blockDim.x) {
+      const bool in = (unsigned)i < (unsigned)a.n;
+      const float x = in ? lp_load<DT>(base, i) : NAN;
+      rank += __builtin_popcountll(__ballot(in && (x == x || i < tok)));
+    }
+  }
   sum = lp_wave_sum(sum), dot = lp_wave_sum(dot);
   // back to sums of exp(d) and exp(d) d: max is finite, or they are 0 or NaN
   dot = (dot - low * sum) * 0.69314718055994530942f;
@@ -239,7 +249,6 @@ __global__ void __launch_bounds__(32 * kLpMost / EACH) __attribute__((amdgpu_wav
   }
   __syncthreads();
   const int c = listed;
-  const int begin = stretch * (int)blockDim.x * EACH - shift, end = begin + (int)blockDim.x * EACH;
   const int held = (end < a.n ? end : a.n) - (begin > 0 ? begin : 0);  // elements of the stretch; fewer than top end its list
   const bool in_turn = c > kLpList || c < (held < a.top ? held : a.top);
   sum = lp_row_sum(w16 < waves ? wave_sum[w16] : 0.0f);
