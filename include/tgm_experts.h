@@ -31,9 +31,10 @@ enum tgm_route_score { TGM_ROUTE_SOFTMAX = 0, TGM_ROUTE_SIGMOID = 1 };
  *   weights[t, j] = scale p, divided by the chosen ones' sum with renormalize
  *
  * Equal keys rank by index, groups too.  The choice is that of keys in 64 bits.  A NaN key ranks behind
- * every other; a row with a NaN among its logits, or with +infinity under a softmax, has NaN weights.
- * Renormalised weights are those of the chosen logits however far below the row's largest, or 0, they lie;
- * chosen logits of -infinity alone have the weights 0.  ids int32 and weights float32 are [tokens, top_k]. */
+ * every other and counts as -infinity in its group's sum; a row with a NaN among its logits, or with
+ * +infinity under a softmax, has NaN weights, and under a softmax its keys are NaN.  Renormalised weights
+ * are those of the chosen logits however far below the row's largest, or 0, they lie; chosen logits of
+ * -infinity alone have the weights 0.  ids int32 and weights float32 are [tokens, top_k]. */
 int tgm_route(const void* logits, int64_t dtype, int64_t tokens, int64_t experts, int64_t ld, const float* bias,
               int64_t score, int64_t groups, int64_t top_groups, int64_t top_k, int64_t renormalize, double scale,
               int32_t* ids, float* weights, void* stream);

@@ -28,7 +28,8 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, 
             rank = x if bias is None else key
             left = []
             if top_groups < groups:
-                best = [np.sort(key[g * (n // groups):(g + 1) * (n // groups)])[::-1][:2].sum() for g in range(groups)]
+                numbers = np.where(key != key, -np.inf, key)
+                best = [np.sort(numbers[g * (n // groups):(g + 1) * (n // groups)])[::-1][:2].sum() for g in range(groups)]
                 keep = set(descending(np.array(best))[:top_groups].tolist())
                 left = [e for e in range(n) if e // (n // groups) not in keep]
             order = [e for e in descending(rank) if e not in left]

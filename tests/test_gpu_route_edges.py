@@ -75,3 +75,46 @@ def test_weights_without_a_score(dev):
     for score in ("softmax", "sigmoid"):
         got = check(dev, x, 2, [5, 5, 0, 0], score=score)
         assert got.weights[[0, 1, 3]].eq(0).all() and got.weights[2].tolist() == [1.0, 0.0]
+
+
+# ----------------------------------------------------------------------------- rows that are not finite
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,top_k", [(8, 1, 4), (64, 1, 14), (64, 1, 15), (64, 8, 14), (96, 3, 13), (256, 8, 12), (512, 1, 30),
+                                                  (1024, 4, 40)])
+def test_route_of_rows_with_a_nan(dev, score, experts, groups, top_k):
+    """Rows with a NaN or +infinity beside rows whose keys lie next to a border: their experts too are those of 64-bit keys,
+    each named once; under a softmax every key of such a row is NaN, and the experts come by index."""
+    rng = np.random.default_rng(experts + top_k)
+    x = rng.standard_normal((60, experts))
+    x[15:45] = np.round(x[15:45])  # many equal ones
+    x[::3, rng.integers(0, experts, 20)] = np.nan
+    x[1::7, experts // 3] = np.inf
+    x[4::9, rng.integers(0, experts, 7)] = -np.inf
+    undone = -(1 / (1 + np.exp(-np.nan_to_num(x[1].astype(np.float32).astype(np.float64), posinf=0, neginf=0))))
+    for bias in (undone + rng.standard_normal(experts) * 1e-9, np.zeros(experts), np.round(rng.standard_normal(experts)) * 1000,
+                 np.where(np.arange(experts) % 3 == 0, -np.inf, 0.25), None):
+        for top_groups in sorted({groups, (groups + 1) // 2}):
+            got = check(dev, x, top_k, bias, score=score, groups=groups, top_groups=top_groups)
+            assert all(len(set(row)) == top_k for row in got.ids.tolist())
+
+
+def test_rows_with_a_nan_next_to_a_border(dev):
+    """Rows with a NaN whose keys differ in 64 bits alone: all of them, and four around the last chosen one beside rows of the
+    same wave that have them earlier."""
+    for seed in range(12):
+        rng = np.random.default_rng(seed)
+        for experts, top_k in ((8, 3), (64, 9), (256, 8)):
+            x = np.repeat(rng.standard_normal((1, experts)), 24, 0).astype(np.float32)
+            bias = rng.standard_normal(experts) * 1e-9 - 1 / (1 + np.exp(-x[0].astype(np.float64)))
+            x[::2, 2] = x[1::2, experts - 1] = np.nan
+            check(dev, x, top_k, bias, score="sigmoid")
+        route(torch.randn((64, 64), device=dev), 1, groups=64, top_groups=63)
+        x = np.repeat(rng.standard_normal((1, 64)), 40, 0).astype(np.float32)
+        x[:, :3] = 8
+        keys = 2 - 0.01 * np.arange(64)
+        keys[13:17] = keys[13] - 1e-7 * rng.permutation(4)
+        bias = keys - 1 / (1 + np.exp(-x[0].astype(np.float64)))
+        x[::2, :3] = -np.inf
+        x[1::2, 63] = np.nan
+        got = check(dev, x, 14, bias, score="sigmoid")
+        assert all(len(set(row)) == 14 for row in got.ids.tolist())

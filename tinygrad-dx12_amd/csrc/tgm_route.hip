@@ -8,8 +8,8 @@
 // The keys' order is that of 64 bits, which are needed next to a border only.  Without a bias the logits' own order is the
 // keys' and 32 bits hold it exactly.  With one, keys are computed in 32 bits first, and the list goes on to the first
 // distance that is larger than their errors allow.  Where neighbours in it are nearer, its entries' keys are computed in 64
-// bits, one a lane, and put in order; where it does not end in time, or groups on either side of their border are that
-// near, the wave does the choice again in 64 bits.
+// bits, one a lane, and put in order; where it does not end in time, where groups on either side of their border are that
+// near, or where a row has a NaN, the wave does the choice again in 64 bits.
 //
 // What bounds it: instructions.  8192 tokens of 256 experts in 8 groups read 8.4 MB, 2 us of memory time, and take 12.6 (15.2
 // with expf and a division in the keys, whose errors the list allows for): a
@@ -329,7 +329,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
       c[r] = c[r] * inv + b[r];
       key[r] = e < a.experts ? route_key(biased ? c[r] : x[r]) : 0u;
     }
-    if (limited) again = route_groups<W, R>(a, l, c, key, (float*)sums[slot], 2 * tol);
+    // rows that are not finite have neither errors as above nor, under a softmax, keys that are numbers
+    again = bad;
+    if (limited) again |= route_groups<W, R>(a, l, c, key, (float*)sums[slot], 2 * tol);
     entries = route_choose<W, R>(a, l, key, list, biased, tol, near);
     again |= entries < 0 || (near && entries > W);
   } else {
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
     for (int r = 0; r < R; ++r) key[r] = l * R + r < a.experts ? route_key(x[r]) : 0u;
     entries = route_choose<W, R>(a, l, key, list, false, 0.0f, near);
   }
-  if (__any((near || again) && !bad)) {
+  if (__any(near || again)) {
     double total = 1.0;
     if (soft) {
       total = 0.0;
@@ -353,9 +355,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_rows(RouteArgs a) {
     }
     auto wide_key = [&](float v, int e) __attribute__((always_inline)) {
       const double p = soft ? exp((double)v - (double)zero) : 1.0 / (1.0 + exp(-(double)v));
-      return v != v ? (double)v : (total > 0.0 ? p / total : 0.0) + (biased ? (double)a.bias[e] : 0.0);
+      return (total == 0.0 ? 0.0 : p / total) + (biased ? (double)a.bias[e] : 0.0);
     };
-    if (__any(again && !bad)) {  // the whole wave
+    if (__any(again)) {  // the whole wave
       unsigned long long wide[R];
       double c[R];
 #pragma unroll

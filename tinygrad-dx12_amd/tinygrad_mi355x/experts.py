@@ -43,8 +43,8 @@ def route(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: tor
     ``top_groups`` best groups (all of them).  Equal ones rank by index; the choice is that of values in 64 bits.  The
     weights are the chosen experts' scores, divided by their sum with ``renormalize``, times ``scale``.
 
-    NaN ranks behind everything; a row with a NaN, or with +infinity under a softmax, has NaN weights; chosen logits that
-    are all -infinity have weights of zero.
+    NaN ranks behind everything and counts as -infinity in a group's sum; a row with a NaN, or with +infinity under a softmax,
+    has NaN weights (and softmax scores of NaN); chosen logits that are all -infinity have weights of zero.
     """
     top_groups = groups if top_groups is None else top_groups
     sig = (logits.shape, logits.stride(), logits.dtype, logits.get_device(), top_k, score, groups, top_groups, renormalize,
