@@ -290,6 +290,8 @@ class Decoder:
                 raise ValueError(f"a layer must hold {cfg.experts} experts of {cfg.hidden} x {cfg.ffn} in an FP4 or FP6 format")
             if L.router is None or L.router.shape != (cfg.experts, cfg.hidden) or L.router.dtype is not torch.bfloat16:
                 raise ValueError(f"a layer's router must be bfloat16 [{cfg.experts}, {cfg.hidden}]")
+            if not L.router.is_contiguous() or L.router.device != self.device or e.device != self.device:
+                raise ValueError(f"a layer's router must be contiguous, and lie with its experts on {self.device}")
         f32, k = dict(dtype=torch.float32, device=self.device), cfg.experts_per_token
         self.router_logits = torch.empty((rows, cfg.experts), **f32)
         self.expert_ids = torch.empty((rows, k), dtype=torch.int32, device=self.device)
