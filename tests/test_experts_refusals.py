@@ -1,0 +1,21 @@
+"""Refusals of the mixture-of-experts operators at the ends of their arguments: no GPU needed."""
+
+import pytest
+import torch
+
+from tinygrad_mi355x.experts import route
+from tinygrad_mi355x.runtime import kernels as K
+
+
+@pytest.mark.parametrize("kw", [dict(scale=torch.tensor(2.0)), dict(scale=1e39), dict(scale=-1e39), dict(scale=10 ** 400), dict(scale=float("nan")),
+                                dict(scale=None), dict(scale="2"), dict(renormalize=torch.tensor(True))])
+def test_route_refuses_what_is_no_number(kw):
+    """A tensor's value could change between calls that look alike; a scale beyond 32 bits would be infinite."""
+    with pytest.raises(ValueError):
+        route(torch.zeros(4, 8), 2, **kw)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39])
+def test_route_entry_point_refuses_scales(scale):
+    with pytest.raises(ValueError, match="scale"):
+        K.call("tgm_route", 4096, 13, 4, 8, 8, None, 0, 1, 1, 2, 1, scale, 4096, 4096, None)

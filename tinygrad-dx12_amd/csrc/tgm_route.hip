@@ -15,6 +15,7 @@
 // with expf and a division in the keys, whose errors the list allows for): a
 // sigmoid an expert, the two largest of each group, eight rounds of a maximum over 16 lanes.  With 32 or 64 lanes a token
 // the rounds are longer and the time the same.
+#include <float.h>
 #include <math.h>
 
 #include "../../include/tgm_experts.h"
@@ -449,7 +450,7 @@ extern "C" int tgm_route(const void* logits, int64_t dtype, int64_t tokens, int6
                 "groups must be 1 to %d and divide the experts", kRouteMaxGroups);
   TGM_CHECK_ARG(top_groups >= 1 && top_groups <= groups, "top_groups must be 1 to groups");
   TGM_CHECK_ARG(top_k >= 1 && top_k <= experts / groups * top_groups, "top_k must be 1 to the experts of top_groups groups");
-  TGM_CHECK_ARG(scale == scale && scale - scale == 0.0, "scale must be finite");
+  TGM_CHECK_ARG(fabs(scale) <= FLT_MAX, "scale must be a finite number of 32 bits");
   if (tokens == 0) return TGM_OK;
   TGM_CHECK_ARG(logits && ids && weights, "null operand");
   RouteArgs a;

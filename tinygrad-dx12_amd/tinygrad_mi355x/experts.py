@@ -13,7 +13,7 @@ Results and workspaces come from torch's caching allocator: to replay calls as a
 
 from __future__ import annotations
 
-import math
+import numbers
 import struct
 from typing import NamedTuple
 
@@ -80,8 +80,11 @@ def _route_plan(sig, logits, top_k, score, bias, groups, top_groups, renormalize
         raise ValueError(f"top_groups must be 1 to {groups}, got {top_groups}")
     if not 1 <= top_k <= experts // groups * top_groups:
         raise ValueError(f"top_k must be 1 to {experts // groups * top_groups}, the experts of {top_groups} groups, got {top_k}")
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    # plans are looked up by the values of both, which a tensor would change behind its place in the look-up
+    if not isinstance(scale, numbers.Real) or not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"scale must be a finite number of 32 bits, got {scale!r}")
+    if isinstance(renormalize, torch.Tensor):
+        raise ValueError("renormalize must be a truth value, not a tensor")
     if bias is not None:
         if bias.dtype is not torch.float32 or bias.shape != (experts,) or not bias.is_contiguous():
             raise ValueError(f"bias must be contiguous float32 [{experts}], got {bias.dtype} {tuple(bias.shape)}")
