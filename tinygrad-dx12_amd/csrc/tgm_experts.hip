@@ -212,7 +212,8 @@ extern "C" int tgm_experts_apply(const tgm_experts* experts, const void* x, int6
   const bool ints = expert_ints(e.format), scaled = e.scale_dtype != TGM_NONE;
   TGM_CHECK_ARG(x_dtype == (ints ? TGM_F16 : TGM_BF16), "x must be %s beside these weights", ints ? "f16" : "bf16");
   TGM_CHECK_ARG(y_dtype == x_dtype || y_dtype == TGM_F32, "y must be of x's type or f32");
-  TGM_CHECK_ARG((ldx >= e.hidden && ldx % 8 == 0 && ldy >= e.hidden) || tokens <= 1, "rows must be apart, those of x by a multiple of 8");
+  TGM_CHECK_ARG((ldx >= e.hidden && ldx % 8 == 0 && ldx < (1ll << 31) && ldy >= e.hidden && ldy < (1ll << 36)) || tokens <= 1,
+                "rows must be apart, those of x by a multiple of 8");
   if (tokens == 0) return TGM_OK;
   if (tokens == 1) ldx = ldy = e.hidden;
   TGM_CHECK_ARG(((tokens - 1) * ldx + e.hidden) * 2 < (1ll << 31), "x must be less than 2 GiB");

@@ -459,7 +459,7 @@ extern "C" int tgm_log_probs(const void* logits, int64_t dtype, int64_t rows, in
                              float* top_logprobs, void* workspace, int64_t workspace_bytes, void* stream) {
   clear_error();
   if (const int status = lp_check(dtype, rows, vocab, top); status != TGM_OK) return status;
-  TGM_CHECK_ARG(ld >= vocab || rows <= 1, "the row stride is less than a row");
+  TGM_CHECK_ARG((ld >= vocab && ld < (1ll << 36)) || rows <= 1, "the row stride is less than a row, or too large");
   if (rows == 0) return TGM_OK;
   TGM_CHECK_ARG(logits && tokens && logprobs && ranks && entropy && (!top || (top_ids && top_logprobs)), "null operand");
   TGM_CHECK_ARG((uintptr_t)logits % dtype_size((int)dtype) == 0, "misaligned logits");

@@ -444,7 +444,7 @@ extern "C" int tgm_route(const void* logits, int64_t dtype, int64_t tokens, int6
   TGM_CHECK_ARG(dtype == TGM_F32 || dtype == TGM_F16 || dtype == TGM_BF16, "logits must be f32, f16 or bf16");
   TGM_CHECK_ARG(tokens >= 0 && tokens < (1ll << 24), "invalid token count");
   TGM_CHECK_ARG(experts >= 1 && experts <= 1024, "a router chooses among 1 to 1024 experts");
-  TGM_CHECK_ARG(ld >= experts || tokens <= 1, "the row stride is less than a row");
+  TGM_CHECK_ARG((ld >= experts && ld < (1ll << 36)) || tokens <= 1, "the row stride is less than a row, or too large");
   TGM_CHECK_ARG(score == TGM_ROUTE_SOFTMAX || score == TGM_ROUTE_SIGMOID, "unknown score");
   TGM_CHECK_ARG(groups >= 1 && groups <= kRouteMaxGroups && experts % groups == 0,
                 "groups must be 1 to %d and divide the experts", kRouteMaxGroups);
