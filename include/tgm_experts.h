@@ -60,13 +60,13 @@ typedef struct tgm_experts {
 /* y[t] = sum_j weights[t, j] down_e . (silu(gate_e . x[t]) * (up_e . x[t])),  e = ids[t, j]
  *
  * x [tokens, hidden] (row stride ldx, a multiple of 8; 16-byte aligned), ids and weights [tokens, top_k]
- * contiguous, y [tokens, hidden] (row stride ldy) of x's type or F32; y may be x.  An id
- * outside [0, experts) names no expert and adds nothing; the same expert may be named twice.  Products
- * and sums over K, experts and tokens are float32; silu(gate) * up is rounded to x's type on its way into
- * the down product.  Repeated calls agree to the bit.  A token's result depends on the other tokens of the
- * call in the rounding of sums alone, whose order goes by the call's sizes and, for up to 16 tokens, by the
- * experts that they name.  tokens times top_k must be less than 2^24, x less than 2 GiB and the weight of an
- * expert less than 4 GiB.
+ * contiguous, y [tokens, hidden] (row stride ldy) of x's type or F32; y may be x and shares no memory
+ * with weights.  An id outside [0, experts) names no expert and adds nothing; the same expert may be
+ * named twice.  Products and sums over K, experts and tokens are float32; silu(gate) * up is rounded to
+ * x's type on its way into the down product.  Repeated calls agree to the bit.  A token's result depends
+ * on the other tokens of the call in the rounding of sums alone, whose order goes by the call's sizes
+ * and, for up to 16 tokens, by the experts that they name.  tokens times top_k must be less than 2^24, x
+ * less than 2 GiB and the weight of an expert less than 4 GiB.
  * workspace: tgm_experts_workspace() bytes, 16-byte aligned. */
 int64_t tgm_experts_workspace(const tgm_experts* experts, int64_t tokens, int64_t top_k);
 int tgm_experts_apply(const tgm_experts* experts, const void* x, int64_t x_dtype, int64_t tokens, int64_t ldx,

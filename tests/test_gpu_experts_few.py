@@ -2,6 +2,7 @@
 tolerances as in test_gpu_experts."""
 
 import pytest
+import torch
 
 from test_gpu_experts import Layer, choice, randn
 
@@ -21,3 +22,27 @@ def test_unscaled_experts_of_several_groups(dev, fmt, hidden, ffn):
     layer = Layer(dev, fmt, 3, hidden, ffn, None)
     for tokens, top_k in ((1, 1), (1, 3), (5, 2), (16, 2)):
         check(dev, layer, tokens, top_k, 0.002)
+
+
+@pytest.mark.parametrize("tokens", [3, 40])
+def test_outputs_over_the_weights_are_refused(dev, tokens):
+    """A token's output is written while another's weights are read."""
+    layer = Layer(dev, "fp4_e2m1", 4, 128, 128)
+    ids, weights = choice(dev, 1, tokens, 4, 2)
+    x = randn(dev, 2, tokens, 128, dtype=layer.e.dtype, scale=0.5)
+    held = torch.zeros(tokens * 128 + 2 * tokens, device=dev)
+    out, behind = held[:tokens * 128].view(tokens, 128), held[tokens * 128:].view(tokens, 2)
+    behind.copy_(weights)
+    want = layer.e.apply(x, ids, weights, out=torch.empty_like(out))
+    assert torch.equal(layer.e.apply(x, ids, behind, out=out), want)  # next to each other
+    for at in (0, 7, tokens * 128 - 1):
+        over = held[at:at + 2 * tokens].view(tokens, 2)
+        over.copy_(weights)
+        with pytest.raises(ValueError):
+            layer.e.apply(x, ids, over, out=out)
+    rows = torch.zeros((tokens, 130), device=dev)  # weights in the gaps of out's rows, all in one row
+    gaps = rows.view(-1)[128:128 + 2].view(1, 2)
+    gaps.copy_(weights[:1])
+    got = layer.e.apply(x[:1], ids[:1], gaps, out=rows[:1, :128])
+    assert torch.equal(gaps, weights[:1])
+    layer.check(got, x[:1], ids[:1], weights[:1])

@@ -22,6 +22,7 @@ import torch
 from tinygrad_mi355x.codegen.decomp.mi355x import MX_FORMATS, PackedTensor
 from tinygrad_mi355x.rotary import _DT, Plans
 from tinygrad_mi355x.runtime import kernels as K
+from tinygrad_mi355x.runtime.overlap import Apart
 
 SCORES = {"softmax": 0, "sigmoid": 1}  # enum tgm_route_score
 MAX_EXPERTS, MAX_GROUPS = 1024, 64
@@ -145,9 +146,10 @@ class PackedExperts:
         """The weighted sum of each token's experts: x [tokens, hidden] of ``dtype``, ids (int32) and weights (float32)
         [tokens, top_k] as ``route`` gives them.
 
-        ``out`` [tokens, hidden] is of x's type or float32 (x's type), with contiguous rows; it may be x.  An id outside
-        0 .. experts - 1 names no expert and adds nothing, whatever its weight: a row without any is zero.  The same expert
-        may be named twice.  Products and sums are float32; silu(gate) * up is rounded to x's type before the down product.
+        ``out`` [tokens, hidden] is of x's type or float32 (x's type), with contiguous rows; it may be x, and shares no memory
+        with weights.  An id outside 0 .. experts - 1 names no expert and adds nothing, whatever its weight: a row without any
+        is zero.  The same expert may be named twice.  Products and sums are float32; silu(gate) * up is rounded to x's type
+        before the down product.
         x starts at a multiple of 16 bytes, and its rows lie a multiple of 8 values apart.
         """
         sig = (x.shape, x.stride(), x.dtype, x.get_device(), ids.shape, ids.stride(), ids.dtype, ids.get_device(), weights.shape,
@@ -157,9 +159,11 @@ class PackedExperts:
         plan = self._plans.get(sig)
         if plan is None:
             plan = self._apply_plan(sig, x, ids, weights, out)
-        head, top_k, tail, need, index = plan
+        head, top_k, tail, need, index, apart = plan
         if out is None:
             out = x.new_empty(x.shape)
+        else:
+            apart.check(out, weights, "weights")  # which are read while it is written
         if x.shape[0]:
             # the workspace is of the caching allocator, so that calls on several streams never share one; held until the
             # launches, or another thread's call on this stream could be given its memory before them
@@ -195,7 +199,8 @@ class PackedExperts:
             raise ValueError(f"rows of x must be 16-byte aligned, got a stride of {ldx}")
         K.require_device(x)
         need = self.workspace_bytes(tokens, ids.shape[1])
-        return self._plans.keep(sig, ((_DT[x.dtype], tokens, ldx), ids.shape[1], (_DT[odt], ldy), need, x.get_device()))
+        return self._plans.keep(sig, ((_DT[x.dtype], tokens, ldx), ids.shape[1], (_DT[odt], ldy), need, x.get_device(),
+                                       None if out is None else Apart(out, weights)))
 
 
 def _scales(w: PackedTensor) -> tuple:

@@ -71,3 +71,14 @@ class OutLayout:
         delta = out.data_ptr() - x.data_ptr()
         if self.before < delta < self.behind and not (self.same and delta == 0) and overlap(x, out):
             raise ValueError(f"out must be {name} itself or share no memory with it")
+
+
+class Apart:
+    """Refuses tensors of the layouts of ``out`` and ``t`` that share memory, for calls with any addresses."""
+
+    def __init__(self, out: torch.Tensor, t: torch.Tensor) -> None:
+        self.before, self.behind = -_extent(t, _spans(t)), _extent(out, _spans(out))
+
+    def check(self, out: torch.Tensor, t: torch.Tensor, name: str) -> None:
+        if self.before < t.data_ptr() - out.data_ptr() < self.behind and overlap(out, t):
+            raise ValueError(f"out must share no memory with {name}")
