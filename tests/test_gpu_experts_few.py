@@ -4,7 +4,7 @@ tolerances as in test_gpu_experts."""
 import pytest
 import torch
 
-from test_gpu_experts import Layer, choice, randn
+from test_gpu_experts import BF16, F16, F32, FORMATS, Layer, choice, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -22,6 +22,26 @@ def test_unscaled_experts_of_several_groups(dev, fmt, hidden, ffn):
     layer = Layer(dev, fmt, 3, hidden, ffn, None)
     for tokens, top_k in ((1, 1), (1, 3), (5, 2), (16, 2)):
         check(dev, layer, tokens, top_k, 0.002)
+
+
+@pytest.mark.parametrize("fmt,scales,block", [f for f in FORMATS if f[1] is not None])
+@pytest.mark.parametrize("hidden,ffn", [(640, 1152), (2176, 640), (3712, 256)])
+def test_experts_of_several_groups(dev, fmt, scales, block, hidden, ffn):
+    """Rows of 2 to 8 groups, whose last one is not full, whole and in two and four slices of waves."""
+    print(f"groups {fmt} {scales} {block} {hidden} {ffn}", flush=True)
+    layer = Layer(dev, fmt, 3, hidden, ffn, scales, block)
+    for tokens, top_k in ((1, 1), (1, 3), (5, 2), (16, 2)):
+        check(dev, layer, tokens, top_k, 0.3)
+
+
+@pytest.mark.parametrize("fmt,scales,block", [("fp4_e2m1", "e8m0", 32), ("fp6_e2m3", "e8m0", 32), ("fp6_e3m2", "e8m0", 32), ("int4", F16, 32),
+                                              ("int4", F32, 32), ("uint4", BF16, 64), ("uint4", F32, 64), ("int4", F32, 128)])
+def test_waves_of_many_groups(dev, fmt, scales, block):
+    """More rows than waves: each goes through several units, with the next groups always on their way."""
+    print(f"many groups {fmt} {scales} {block}", flush=True)
+    layer = Layer(dev, fmt, 8, 2176, 2176, scales, block)
+    for tokens, top_k in ((16, 4), (15, 8), (16, 1)):
+        check(dev, layer, tokens, top_k, 0.3)
 
 
 @pytest.mark.parametrize("tokens", [3, 40])
