@@ -2,7 +2,8 @@
 //
 //   y[t] = sum_j weights[t, j] down_e . (silu(gate_e . x[t]) * (up_e . x[t])),  e = ids[t, j]
 //
-// A token and one of its experts is a pair.  Four launches:
+// A token and one of its experts is a pair.  Up to 16 tokens and 128 pairs take the two launches of tgm_experts_few.h, more of
+// them four:
 //
 //   experts_plan  puts the pairs in the order of their experts (a position each), and cuts each expert's positions into
 //                 tiles of rows;

@@ -11,10 +11,10 @@
 // bits, one a lane, and put in order; where it does not end in time, where groups on either side of their border are that
 // near, or where a row has a NaN, the wave does the choice again in 64 bits.
 //
-// What bounds it: instructions.  8192 tokens of 256 experts in 8 groups read 8.4 MB, 2 us of memory time, and take 12.6 (15.2
-// with expf and a division in the keys, whose errors the list allows for): a
-// sigmoid an expert, the two largest of each group, eight rounds of a maximum over 16 lanes.  With 32 or 64 lanes a token
-// the rounds are longer and the time the same.
+// What bounds it: instructions.  8192 tokens of 256 experts in 8 groups read 8.4 MB, 2 us of memory time, and take 11 to 12 (some
+// 3 more with expf and a division in the keys, whose errors the list allows for): a sigmoid an expert, the two largest of each
+// group, eight rounds of a maximum over 16 lanes.  With 32 or 64 lanes a token the rounds are longer and the time the same.  A
+// wave that does the choice again takes 9 more, which the launch waits for: one set of such inputs in eight has one.
 #include <float.h>
 #include <math.h>
 
